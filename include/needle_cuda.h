@@ -326,6 +326,137 @@ int needle_cuda_attention_dev_fast(const float* q, const int8_t* key_codes, cons
                                    const int32_t* counts, int32_t batch, int32_t capacity,
                                    float* out, void* stream);
 
+/* ---- Serving operators (device pointers; the caller owns every buffer) ----
+ * The steps of a decode loop around its matvecs, for any head layout and element type:
+ * needle_cuda_rope_append_dev -> needle_cuda_prefix_attention_dev -> ... ->
+ * needle_cuda_logits_select_dev.  They run on `stream` without synchronising, allocate nothing and keep
+ * nothing between calls, so they can be captured into CUDA graphs; the buffers, the stream and the
+ * current device must belong together (a host pointer, or an output on another device, is refused with
+ * BACKEND_UNAVAILABLE).  Lists of positions, slots, lengths and ids are device memory and are bounded in
+ * the kernels: an index outside its range is left out, never followed. */
+
+typedef enum needle_type { NEEDLE_TYPE_F32 = 0, NEEDLE_TYPE_F16 = 1, NEEDLE_TYPE_BF16 = 2 } needle_type;
+
+/* Query / key norms, rotary positions and the int8 cache append of `tokens` tokens (the Q / K / V path of
+ * NeedleRuntime.step, runtime.ts:471-501, and #storeKV, runtime.ts:679-717).  Strides are in elements
+ * between tokens; heads are head_dim apart and dense, so q, k and v may be views of one fused buffer.
+ * Per head: y = (1 + norm) x / sqrt(mean x^2 + 1e-6) where a norm is given; pairs (i, i + rotary_dim / 2),
+ * or (2i, 2i + 1) when `interleaved`, of the first rotary_dim dimensions turn by position * inverse
+ * frequency i and grow by `magnitude`; q_out gets the queries.  Keys and values are rounded to int8 with
+ * scale max(1e-12, max |y|) / 127 and stored at (slot, entry) of
+ *   codes [slot_count][kv_heads][capacity][head_dim], scales [slot_count][kv_heads][capacity];
+ * a token whose slot or entry is out of range (-1: padding) is rotated but not stored.  Two tokens of one
+ * call must not name the same (slot, entry).  k_out / v_out (optional) get the keys and values as the
+ * cache holds them, code * scale: what an attention over the new tokens themselves has to read.  q_out may
+ * be q, k_out k and v_out v. */
+typedef struct needle_rope_append {
+  const void *q, *k, *v;        /* [tokens][heads | kv_heads | kv_heads][head_dim] of `type` */
+  void *q_out, *k_out, *v_out;  /* k_out, v_out may be NULL */
+  int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, v_out_stride;
+  const float *q_norm, *k_norm; /* head_dim zero-centred norm scales, or NULL: no norm */
+  const int32_t *positions, *slots, *entries; /* [tokens] */
+  int8_t* key_codes;            /* 16-byte aligned, as value_codes */
+  float* key_scales;
+  int8_t* value_codes;
+  float* value_scales;
+  double magnitude;             /* 1 unless the frequencies' scaling says otherwise */
+  int32_t type, tokens, heads, kv_heads, head_dim /* 64 or 128 */, rotary_dim /* even, 0..head_dim */,
+      interleaved, slot_count, capacity;
+} needle_rope_append;
+
+/* `inverse_frequencies`: rotary_dim / 2 HOST doubles (needle_cuda_rope_frequencies). */
+int needle_cuda_rope_append_dev(const needle_rope_append* args, const double* inverse_frequencies, void* stream);
+
+enum {
+  NEEDLE_ROPE_PLAIN = 0,  /* theta^(-2i / rotary_dim) */
+  NEEDLE_ROPE_LINEAR = 1, /* position interpolation: the plain frequencies / factor */
+  NEEDLE_ROPE_NTK = 2,    /* theta * factor^(rotary_dim / (rotary_dim - 2)) in place of theta */
+  NEEDLE_ROPE_PARTS = 3   /* by parts (YaRN): pairs that turn fast_turns times and more over trained_length
+                             keep their frequency, slow_turns and fewer are interpolated, linear in between;
+                             magnitude 0.1 ln(factor) + 1 */
+};
+
+typedef struct needle_rope_scaling {
+  double theta, factor, trained_length, fast_turns, slow_turns; /* the last three: NEEDLE_ROPE_PARTS */
+  int32_t kind;
+} needle_rope_scaling;
+
+/* The inverse frequencies (rotary_dim / 2 doubles, rotary_dim 2..128) and magnitude of a scaling; host
+ * only, no GPU needed. */
+int needle_cuda_rope_frequencies(const needle_rope_scaling* scaling, int32_t rotary_dim, double* inverse_frequencies,
+                                 double* magnitude);
+
+/* Decode attention of a batch that shares a prompt prefix (needle_cuda_attention_dev_fast with the prefix
+ * held and read once for all rows): row r attends over prefix positions 0 .. prefix_length - 1 and over
+ * entries 0 .. counts[r] - 1 of its own cache slot slots[r] (NULL: slot r), in binary32.
+ *   prefix codes [kv_heads][prefix_capacity][head_dim], scales [kv_heads][prefix_capacity]
+ *   own codes [slot_count][kv_heads][capacity][head_dim], scales [slot_count][kv_heads][capacity]
+ * Query head h reads KV head h / (heads / kv_heads).  Several rows may name one slot.  counts are taken
+ * within [0, capacity].  A row whose slot is out of range (-1: padding) is left as it was.  A row with
+ * nothing to attend to gets zeros and lse -inf.  lse (optional, [rows][heads]): the natural logarithm of
+ * each head's softmax denominator, with which outputs over different prefixes can be merged. */
+typedef struct needle_prefix_attention {
+  const void* q;   /* [rows][heads][head_dim] of `type`, rows q_stride elements apart */
+  void* out;       /* the same shape, rows out_stride elements apart */
+  float* lse;
+  int64_t q_stride, out_stride;
+  const int8_t* prefix_key_codes; /* codes 16-byte aligned */
+  const float* prefix_key_scales;
+  const int8_t* prefix_value_codes;
+  const float* prefix_value_scales;
+  const int8_t* key_codes;
+  const float* key_scales;
+  const int8_t* value_codes;
+  const float* value_scales;
+  const int32_t *slots, *counts; /* [rows] */
+  float scale;                   /* of q . k; 0: 1 / sqrt(head_dim) */
+  int32_t type, rows, heads, kv_heads, head_dim /* 64 or 128 */, prefix_length, prefix_capacity, slot_count, capacity;
+} needle_prefix_attention;
+
+/* Bytes of workspace a call with these arguments needs.  Reads no device memory; depends only on the sizes,
+ * so a caller may size it once for its largest batch and longest prefix. */
+int needle_cuda_prefix_attention_workspace(const needle_prefix_attention* args, size_t* bytes);
+
+/* `workspace`: 16-byte aligned device memory (NULL when none is needed), not read before it is written;
+ * calls that may run at the same time, two captured graphs among them, need one each. */
+int needle_cuda_prefix_attention_dev(const needle_prefix_attention* args, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
+/* Rules on the logits of `rows` rows before a token is chosen, in this order, each step rounded to
+ * binary32:
+ *   an id in the row's history: l / repetition where l > 0, else l * repetition;
+ *   an id answered c > 0 times (history entries from prompt_lengths[r] on): - frequency * c, - presence;
+ *   an id with a bias: + its value (of several biases of one id the last counts);
+ *   an id that mask slot mask_slots[r] leaves out: -inf (masks as in the device mask pool: bit id % 32 of
+ *   word id / 32, ceil(vocab / 32) words per slot; slot -1: every id is allowed; a slot of mask_count or
+ *   more allows none).
+ * Ids outside [0, vocab) in the lists (-1: padding) are left out; lengths and counts are taken within
+ * [0, stride].  Any list or array of rules may be NULL: that rule does not apply. */
+typedef struct needle_logits_rules {
+  const void* logits;             /* [rows][vocab] of `type`, rows logits_stride elements apart */
+  int64_t logits_stride;
+  const int32_t* history;         /* [rows][history_stride] ids: the prompt, then the answer so far */
+  int64_t history_stride;
+  const int32_t *history_lengths, *prompt_lengths; /* [rows]; prompt_lengths NULL: 0 */
+  const float *repetition, *presence, *frequency;  /* [rows] */
+  const int32_t* bias_ids;        /* [rows][bias_stride] */
+  const float* bias_values;       /* [rows][bias_stride] */
+  int64_t bias_stride;
+  const int32_t* bias_counts;     /* [rows] */
+  const uint32_t* masks;          /* [mask_count][ceil(vocab / 32)] */
+  const int32_t* mask_slots;      /* [rows] */
+  int32_t mask_count, type, rows /* at most 65535 */, vocab;
+} needle_logits_rules;
+
+/* The ruled logits, rounded to `type`, rows out_stride elements apart; out may be logits (same stride). */
+int needle_cuda_logits_rules_dev(const needle_logits_rules* args, void* out, int64_t out_stride, void* stream);
+
+/* selectToken (runtime.ts:880-899) on the ruled logits, which are not written: ids[r] is the allowed id with
+ * the largest ruled logit, the lowest on ties (NaN counts as -inf), and log_probabilities[r] its log
+ * probability under the raw logits, l - max - log sum exp(l - max), as needle_selected.  A row whose mask
+ * leaves nothing gets id -1 and -inf. */
+int needle_cuda_logits_select_dev(const needle_logits_rules* args, int32_t* ids, float* log_probabilities, void* stream);
+
 /* ---- Bounded device waits ----
  * The kernels that wait on asynchronous copies or barriers -- the fast attention, the table matvec and
  * the tensor-core matvec -- give up after 2 s instead of spinning forever.  The outputs of that call

@@ -1,0 +1,88 @@
+// serving.cuh -- what the serving operators (rope.cu, prefix_attn.cu, logits.cu) share: element
+// types, vector access, argument checks and the guard of their C entries.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <exception>
+#include <string>
+
+#include "../../include/needle_cuda.h"
+#include "engine.cuh"
+
+namespace needle {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// N consecutive elements in one access (sizeof(T) * N of 2, 4, 8 or 16 bytes, aligned to its size).
+template <class T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+inline size_t type_bytes(int32_t type) { return type == NEEDLE_TYPE_F32 ? 4 : 2; }
+
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// Calls f(T{}) with the element type of a needle_type.
+template <class F>
+cudaError_t with_type(int32_t type, F f) {
+  if (type == NEEDLE_TYPE_F32) return f(float{});
+  if (type == NEEDLE_TYPE_F16) return f(__half{});
+  return f(__nv_bfloat16{});
+}
+
+inline int refuse(const std::string& msg) {
+  set_last_error(msg);
+  return NEEDLE_BACKEND_UNAVAILABLE;
+}
+
+inline int refuse_cuda(const char* op, cudaError_t e) { return refuse(std::string(op) + ": " + cudaGetErrorString(e)); }
+
+// Whether `p` is memory that kernels of the current device `device` can use: a host pointer or a
+// buffer of another GPU is refused before a launch, where it would fault or cross the link unseen.
+inline int check_buffer(const void* p, const char* name, int device) {
+  cudaPointerAttributes a{};
+  const cudaError_t e = cudaPointerGetAttributes(&a, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return refuse(std::string(name) + ": " + cudaGetErrorString(e));
+  }
+  if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged)
+    return refuse(std::string(name) + " is not device memory");
+  if (a.type == cudaMemoryTypeDevice && a.device != device)
+    return refuse(std::string(name) + " is on device " + std::to_string(a.device) + ", the current device is " +
+                  std::to_string(device));
+  return NEEDLE_OK;
+}
+
+// Runs an entry's body; no C++ exception crosses the C boundary.
+template <class F>
+int entry(F f) noexcept {
+  try {
+    return f();
+  } catch (const std::exception& e) {
+    try {
+      return refuse(e.what());
+    } catch (...) {
+      return NEEDLE_BACKEND_UNAVAILABLE;
+    }
+  } catch (...) {
+    return NEEDLE_BACKEND_UNAVAILABLE;
+  }
+}
+
+}  // namespace needle

@@ -68,6 +68,44 @@ class CqMatrixDesc(C.Structure):
                 ("input_size", C.c_int32), ("group_size", C.c_int32), ("bits", C.c_int32)]
 
 
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2  # needle_type
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_PARTS = 0, 1, 2, 3  # NEEDLE_ROPE_*
+
+
+class RopeAppend(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_out", "v_out")] + [
+        (n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride",
+                                 "v_out_stride")] + [
+        (n, C.c_void_p) for n in ("q_norm", "k_norm", "positions", "slots", "entries", "key_codes", "key_scales",
+                                  "value_codes", "value_scales")] + [("magnitude", C.c_double)] + [
+        (n, C.c_int32) for n in ("type", "tokens", "heads", "kv_heads", "head_dim", "rotary_dim", "interleaved",
+                                 "slot_count", "capacity")]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ("theta", "factor", "trained_length", "fast_turns", "slow_turns")] + [
+        ("kind", C.c_int32)]
+
+
+class PrefixAttention(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "out", "lse")] + [
+        ("q_stride", C.c_int64), ("out_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("prefix_key_codes", "prefix_key_scales", "prefix_value_codes",
+                                  "prefix_value_scales", "key_codes", "key_scales", "value_codes", "value_scales",
+                                  "slots", "counts")] + [("scale", C.c_float)] + [
+        (n, C.c_int32) for n in ("type", "rows", "heads", "kv_heads", "head_dim", "prefix_length",
+                                 "prefix_capacity", "slot_count", "capacity")]
+
+
+class LogitsRules(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("logits_stride", C.c_int64), ("history", C.c_void_p),
+                ("history_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("history_lengths", "prompt_lengths", "repetition", "presence", "frequency",
+                                  "bias_ids", "bias_values")] + [("bias_stride", C.c_int64)] + [
+        (n, C.c_void_p) for n in ("bias_counts", "masks", "mask_slots")] + [
+        (n, C.c_int32) for n in ("mask_count", "type", "rows", "vocab")]
+
+
 EXPORTS = {
     "needle_cuda_last_error": (C.c_char_p, []),
     "needle_cuda_default_opts": (C.c_int, [C.POINTER(Opts)]),
@@ -105,6 +143,14 @@ EXPORTS = {
                                                                 C.c_void_p]),
     "needle_cuda_attention_dev_fast": (C.c_int, [C.c_void_p] * 6 + [C.c_int32, C.c_int32, C.c_void_p,
                                                                      C.c_void_p]),
+    "needle_cuda_rope_append_dev": (C.c_int, [C.POINTER(RopeAppend), C.POINTER(C.c_double), C.c_void_p]),
+    "needle_cuda_rope_frequencies": (C.c_int, [C.POINTER(RopeScaling), C.c_int32, C.POINTER(C.c_double),
+                                               C.POINTER(C.c_double)]),
+    "needle_cuda_prefix_attention_workspace": (C.c_int, [C.POINTER(PrefixAttention), C.POINTER(C.c_size_t)]),
+    "needle_cuda_prefix_attention_dev": (C.c_int, [C.POINTER(PrefixAttention), C.c_void_p, C.c_size_t,
+                                                   C.c_void_p]),
+    "needle_cuda_logits_rules_dev": (C.c_int, [C.POINTER(LogitsRules), C.c_void_p, C.c_int64, C.c_void_p]),
+    "needle_cuda_logits_select_dev": (C.c_int, [C.POINTER(LogitsRules), C.c_void_p, C.c_void_p, C.c_void_p]),
     "needle_cuda_wait_status": (C.c_int, [C.c_int32, C.POINTER(C.c_uint32), C.c_int32]),
     "needle_cuda_wait_selftest": (C.c_int, [C.c_uint64, C.c_void_p]),
     "needle_cuda_stream": (C.c_void_p, [C.c_void_p]),
