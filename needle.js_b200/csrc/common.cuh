@@ -187,4 +187,8 @@ __device__ __forceinline__ void report_wait_timeout(uint32_t* words, int kind) {
 // pinned mapping cannot be made.
 uint32_t* wait_status_words(int device);
 
+// Reports (and clears) the bounded waits of earlier calls on `device` that ran out: NEEDLE_OK, or
+// BACKEND_UNAVAILABLE with the message set.
+int check_wait_status(int device);
+
 }  // namespace needle

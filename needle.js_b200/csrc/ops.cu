@@ -80,23 +80,6 @@ bool g_status_failed = false;
 
 const char* kWaitKindNames[kWaitKinds] = {"fast attention", "table matvec", "tensor-core matvec", "wait self-test"};
 
-// Reports (and clears) the bounded waits of earlier calls on `device` that ran out.
-int check_wait_status(int device) {
-  uint32_t* w = wait_status_words(device);
-  if (!w) return NEEDLE_OK;
-  std::string names;
-  for (int k = 0; k < kWaitKinds; k++) {
-    volatile uint32_t* v = w + k;
-    if (*v) {
-      names += (names.empty() ? "" : ", ") + std::string(kWaitKindNames[k]);
-      *v = 0;
-    }
-  }
-  if (names.empty()) return NEEDLE_OK;
-  return op_fail(NEEDLE_BACKEND_UNAVAILABLE, "a bounded device wait ran out on device " + std::to_string(device) +
-                                                 " (" + names + "); that call's outputs are NaN");
-}
-
 __device__ int g_never_set;  // nothing writes it: the self-test's wait always runs out
 
 __global__ void k_wait_selftest(uint64_t limit_ns, uint32_t* words) {
@@ -116,13 +99,35 @@ __global__ void k_wait_selftest(uint64_t limit_ns, uint32_t* words) {
 
 }  // namespace
 
+// Reports (and clears) the bounded waits of earlier calls on `device` that ran out.
+int needle::check_wait_status(int device) {
+  uint32_t* w = wait_status_words(device);
+  if (!w) return NEEDLE_OK;
+  std::string names;
+  for (int k = 0; k < kWaitKinds; k++) {
+    volatile uint32_t* v = w + k;
+    if (*v) {
+      names += (names.empty() ? "" : ", ") + std::string(kWaitKindNames[k]);
+      *v = 0;
+    }
+  }
+  if (names.empty()) return NEEDLE_OK;
+  return op_fail(NEEDLE_BACKEND_UNAVAILABLE, "a bounded device wait ran out on device " + std::to_string(device) +
+                                                 " (" + names + "); that call's outputs are NaN");
+}
+
 uint32_t* needle::wait_status_words(int device) {
   if (device < 0 || device >= kStatusDevices) return nullptr;
   std::lock_guard<std::mutex> lock(g_status_mu);
   if (!g_status_host && !g_status_failed) {
     void* p = nullptr;
-    if (cudaHostAlloc(&p, sizeof(uint32_t) * kWaitKinds * kStatusDevices, cudaHostAllocMapped | cudaHostAllocPortable) ==
-        cudaSuccess) {
+    // a first call may come while a stream of this thread is being captured
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    const cudaError_t e = cudaHostAlloc(&p, sizeof(uint32_t) * kWaitKinds * kStatusDevices,
+                                        cudaHostAllocMapped | cudaHostAllocPortable);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) {
       std::memset(p, 0, sizeof(uint32_t) * kWaitKinds * kStatusDevices);
       g_status_host = static_cast<uint32_t*>(p);
     } else {
