@@ -18,8 +18,8 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libneedle_cuda.so")
 SOURCES = ["engine.cu", "cq.cu", "layer.cu", "ops.cu", "attn_fast.cu", "cq_fast.cu", "cq_gemm_tc.cu", "rope.cu",
-           "prefix_attn.cu", "logits.cu", "grammar.cpp"]
-HEADERS = ["common.cuh", "cq.cuh", "engine.cuh", "serving.cuh"]
+           "prefix_attn.cu", "prefix_attn_tc.cu", "logits.cu", "grammar.cpp"]
+HEADERS = ["common.cuh", "cq.cuh", "engine.cuh", "serving.cuh", "prefix_attn.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "--fmad=false", "-std=c++17", "--extended-lambda", "-Xcompiler", "-fPIC",
          "-Xcompiler", "-Wall", "-I", os.path.join(ROOT, "include")]

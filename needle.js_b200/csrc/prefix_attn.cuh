@@ -1,0 +1,89 @@
+// prefix_attn.cuh -- what the two kernels of prefix_attention share: the workspace's parts, fp16 operand
+// conversion, bounded barrier waits.
+#pragma once
+
+#include "serving.cuh"
+
+namespace needle {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// The reference maximum of a head covers the value scales too: a weight is 2^(s - M) vs, s and M base 2.  M is
+// raised, and what was summed rescaled, only when a block could bring weights of 2^15 (fp16 ends at 65504);
+// a raised M leaves them below 2^7.
+constexpr float kRaise = 7.0f;
+
+// Parts of the softmax: M and l of every (part, row, head), and the weighted values.  A part is 2^M times
+// its l and values; an empty one has M = -inf and its values are not read.
+struct Parts {
+  float2* ml;
+  float* o;
+  int64_t per_part;  // rows * heads
+};
+
+// The prefix on the tensor cores (prefix_attn_tc.cu): parts 0 .. parts - 1 of `out`, `part_len` positions each.
+// part_len is a multiple of prefix_tile(type).
+int prefix_tile(int32_t type);
+int prefix_rows();  // packed rows (rows * heads of a KV head) a CTA takes
+cudaError_t launch_attend_prefix(const needle_prefix_attention& a, const Parts& out, int parts, int part_len, float scale,
+                                 uint32_t* wait_words, cudaStream_t s);
+
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// Two codes of `w` (biased by 128 with w ^ 0x80808080) as fp16: 0x6400 | byte is 1024 + byte.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t selector) {
+  const uint32_t h = __byte_perm(w, 0x64646464u, selector);
+  return half2_bits(__hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480))));
+}
+
+// fp16 head and tail of two binary32 values.
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& head, uint32_t& tail) {
+  const __half2 h = __floats2half2_rn(a, b);
+  head = half2_bits(h);
+  tail = half2_bits(__floats2half2_rn(a - __low2float(h), b - __high2float(h)));
+}
+
+// 2^e for -126 <= e <= 127.
+__device__ __forceinline__ float power2(int e) { return __int_as_float((e + 127) << 23); }
+// Exponent of |v| (0 and subnormals -127, infinities and NaN 128).
+__device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255u) - 127; }
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void barrier_init(uint64_t* b, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(b)) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(shared_address(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+constexpr uint64_t kAttendWaitNs = 2000000000ull;
+// Waits for the phase of the given parity; false once kAttendWaitNs has passed without it.
+__device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
+  if (barrier_try(b, parity)) return true;
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+  for (;;) {
+    for (int i = 0; i < 64; i++)
+      if (barrier_try(b, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (now - start > kAttendWaitNs) return false;
+  }
+}
+
+__device__ __forceinline__ float power2f(float v) {  // 2^v, relative error 2^-22, 0 below 2^-126
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+}  // namespace needle

@@ -1,0 +1,529 @@
+// prefix_attn_tc.cu -- the shared prefix of a batch on the tensor cores (tcgen05).
+//
+// k_attend_prefix.  With many rows the prefix is a dense product: the heads of a KV head of all rows are
+// packed into M (packed row i = row i / group, head i % group), 256 to a CTA as two tiles of 128, and
+// the CTA walks its part of the prefix in tiles of kNT positions:
+//   loader warps    read int8 codes, turn them into fp16 (exact) and write K and V tiles, in the same
+//                   layout [position][64 dimensions, 128-byte swizzle], into rings in shared memory; V is
+//                   the B operand with its N dimension contiguous, so nothing is transposed
+//   MMA warp        S_t = Q_t K^T (tcgen05.mma, both from shared memory) and O_t += P_t V (P from
+//                   tensor memory), for the two tiles t in turn, so that one tile's products run while
+//                   the other's softmax does
+//   softmax warps   two warpgroups, one thread per packed row: a tile's S into registers, maximum,
+//                   exponentials, P back to tensor memory as fp16; O stays in tensor memory and is only
+//                   rescaled when a tile exceeds the reference maximum by 2^7
+// The reference M of a row covers the value scale too: a weight is 2^(s - M) vs <= 2^15, inside fp16, and
+// sums and outputs share the factor, which cancels.  16-bit queries are exact in fp16 after their row's
+// power of two (the score scale comes after the product), and their weights are rounded to fp16 once (2^-12 each, averaged over the positions; the
+// output's own rounding is 2^-12 or more).  Binary32 queries (kSplit) and their weights are split into fp16
+// heads and tails, two MMAs each, in tiles of 64 positions (tensor memory holds the tails).
+// What bounds it: 128 x 128 exponentials of a tile take 1024 cycles of the SM's 16 a cycle, its two
+// products at D = 128 another 1024 on the tensor pipe.
+// Every wait is bounded (2 s): a wait that runs out is reported through the wait-status words, and the
+// rows' parts become NaN.
+#include "prefix_attn.cuh"
+
+namespace needle {
+
+namespace {
+
+constexpr int kPrefixSoftmaxWarps = 8, kPrefixLoaderWarps = 3;
+constexpr int kPrefixMmaWarp = kPrefixSoftmaxWarps + kPrefixLoaderWarps;
+constexpr int kPrefixThreads = (kPrefixMmaWarp + 1) * 32;
+constexpr int kPrefixRows = 256;  // packed rows of a CTA
+
+template <int D, bool SPLIT>
+struct PrefixShape {
+  static constexpr int kNT = SPLIT ? 64 : 128;       // positions of a tile
+  static constexpr int kHalves = D / 64;
+  static constexpr int kParts = SPLIT ? 2 : 1;       // fp16 parts of a query or weight
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr uint32_t kQHalf = 128 * 128;                       // bytes of 128 rows x 64 dimensions
+  static constexpr uint32_t kQTile = kQHalf * kHalves * kParts;       // [part][half]
+  static constexpr uint32_t kKvHalf = kNT * 128;
+  static constexpr uint32_t kKvTile = kKvHalf * kHalves;
+  static constexpr uint32_t kK = 2 * kQTile, kV = kK + kStages * kKvTile;
+  static constexpr uint32_t kScales = kV + kStages * kKvTile;         // per stage: kNT key, kNT value scales
+  static constexpr uint32_t kSmem = kScales + kStages * kNT * 8 + 1024;
+  // tensor memory columns
+  static constexpr uint32_t kS = 0;                                    // two tiles of kNT
+  static constexpr bool kOverlay = D == 128 && !SPLIT;                 // P takes the place of S
+  static constexpr uint32_t kP = kOverlay ? 0 : (SPLIT ? 128 : 384);
+  static constexpr uint32_t kPStep = kOverlay ? kNT : 64;              // from one tile's P to the other's
+  static constexpr uint32_t kO = 256;
+};
+
+// Byte offset of 16-byte unit `unit` (0..7) of row `row` in a [rows][64 x fp16] tile, 128-byte swizzle.
+__device__ __forceinline__ uint32_t swizzled(int row, int unit) {
+  return (uint32_t)(row * 128 + ((unit ^ (row & 7)) << 4));
+}
+// Shared-memory matrix descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart.  K contiguous: the rows
+// are M or N.  N contiguous: the rows are K, and 64-wide blocks of N lie `block` bytes apart.
+__device__ __forceinline__ uint64_t descriptor(uint32_t address, uint32_t block) {
+  return (uint64_t)((address >> 4) & 0x3FFF) | ((uint64_t)((block >> 4) & 0x3FFF) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// fp16 x fp16 -> fp32, M = 128, N = n; B with N contiguous when `b_n`.
+__device__ __forceinline__ uint32_t instruction(int n, bool b_n) {
+  return (1u << 4) | (b_n ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+// Arrives on `b` once every MMA this thread has issued is complete.
+__device__ __forceinline__ void mma_commit_to(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(b))
+               : "memory");
+}
+
+// 32 (16) consecutive columns of this thread's lane of tensor memory.
+__device__ __forceinline__ void tensor_load32(uint32_t at, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(at));
+}
+__device__ __forceinline__ void tensor_load16(uint32_t at, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(at));
+}
+__device__ __forceinline__ void tensor_store16(uint32_t at, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(at),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tensor_wait_loads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tensor_wait_stores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Shared-memory writes of this thread before reads of the tensor cores.
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Two binary32 values at once.
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void apart(Two t, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v)); }
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Scores from position `valid` on become -inf.
+template <int N>
+__device__ __forceinline__ void hide(uint32_t* x, int valid) {
+#pragma unroll
+  for (int j = 0; j < N; j++)
+    if (j >= valid) x[j] = 0xff800000u;
+}
+
+template <class T, int D, bool SPLIT>
+__global__ void __launch_bounds__(kPrefixThreads, 1)
+    k_attend_prefix(const __grid_constant__ needle_prefix_attention a, const Parts parts, int part_len, float scale,
+                    uint32_t* wait_words) {
+  using P = PrefixShape<D, SPLIT>;
+  constexpr int NT = P::kNT;
+  extern __shared__ __align__(16) unsigned char raw[];
+  __shared__ __align__(8) uint64_t q_full, s_full[2], p_full[2], o_full;
+  __shared__ __align__(8) uint64_t k_full[P::kStages], k_empty[P::kStages], v_full[P::kStages], v_empty[P::kStages];
+  __shared__ uint32_t tensor_base;
+  __shared__ int failed;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.y, group = a.heads / a.kv_heads;
+  const int64_t packed = (int64_t)a.rows * group, first = (int64_t)blockIdx.x * kPrefixRows;
+  const int tiles_m = packed - first > 128 ? 2 : 1;
+  const int begin = blockIdx.z * part_len, end = min(begin + part_len, a.prefix_length);
+  const int n = (end - begin + NT - 1) / NT;
+  const uint32_t sm = (shared_address(raw) + 1023u) & ~1023u;
+  unsigned char* smem = raw + (sm - shared_address(raw));
+
+  if (tid == 0) {
+    barrier_init(&q_full, 4 * tiles_m);
+    for (int t = 0; t < 2; t++) {
+      barrier_init(&s_full[t], 1);
+      barrier_init(&p_full[t], 4);
+    }
+    barrier_init(&o_full, 1);
+    for (int i = 0; i < P::kStages; i++) {
+      barrier_init(&k_full[i], kPrefixLoaderWarps);
+      barrier_init(&v_full[i], kPrefixLoaderWarps);
+      barrier_init(&k_empty[i], 1);
+      barrier_init(&v_empty[i], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    failed = 0;
+  }
+  if (warp == kPrefixMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_address(&tensor_base)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tensor_fence_before();
+  __syncthreads();
+  tensor_fence_after();
+  const uint32_t tm = tensor_base;
+
+  if (warp == kPrefixMmaWarp) {
+    const uint32_t qk = instruction(NT, false), pv = instruction(D, true);
+    bool ok = true;
+    auto wait = [&](uint64_t* b, uint32_t parity) {  // one lane polls, the warp stays together
+      ok = ok && __all_sync(0xffffffffu, lane != 0 || barrier_wait(b, parity));
+      __syncwarp();
+    };
+    auto scores = [&](int t, int i) {  // S_t = Q_t K_i^T
+      const uint32_t q = sm + t * P::kQTile, k = sm + P::kK + (i % P::kStages) * P::kKvTile;
+#pragma unroll
+      for (int part = 0; part < P::kParts; part++)
+#pragma unroll
+        for (int half = 0; half < P::kHalves; half++)
+#pragma unroll
+          for (int s = 0; s < 4; s++)
+            mma_shared(tm + P::kS + t * NT, descriptor(q + (part * P::kHalves + half) * P::kQHalf + s * 32, 16),
+                       descriptor(k + half * P::kKvHalf + s * 32, 16), qk, part + half + s > 0);
+      mma_commit_to(&s_full[t]);
+    };
+    auto values = [&](int t, int i) {  // O_t += P_t V_i
+      const uint32_t v = sm + P::kV + (i % P::kStages) * P::kKvTile;
+#pragma unroll
+      for (int part = 0; part < P::kParts; part++)
+#pragma unroll
+        for (int s = 0; s < NT / 16; s++)
+          mma_tensor(tm + P::kO + t * D, tm + P::kP + t * P::kPStep + part * (NT / 2) + s * 8,
+                     descriptor(v + s * 2048, P::kKvHalf), pv, i > 0 || part + s > 0);
+    };
+    wait(&q_full, 0);
+    wait(&k_full[0], 0);
+    if (ok && lane == 0) {
+      tensor_fence_after();
+      for (int t = 0; t < tiles_m; t++) scores(t, 0);
+      mma_commit_to(&k_empty[0]);
+    }
+    __syncwarp();
+    for (int i = 0; i < n && ok; i++) {
+      for (int t = 0; t < tiles_m && ok; t++) {
+        if (t == 0) wait(&v_full[i % P::kStages], (i / P::kStages) & 1);
+        wait(&p_full[t], i & 1);
+        if (ok && lane == 0) {
+          tensor_fence_after();
+          values(t, i);
+          if (t == tiles_m - 1) mma_commit_to(&v_empty[i % P::kStages]);
+        }
+        __syncwarp();
+        if (i + 1 < n) {
+          const int st = (i + 1) % P::kStages;
+          if (t == 0) wait(&k_full[st], ((i + 1) / P::kStages) & 1);
+          if (ok && lane == 0) {
+            tensor_fence_after();
+            scores(t, i + 1);
+            if (t == tiles_m - 1) mma_commit_to(&k_empty[st]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) {
+      if (!ok) atomicExch(&failed, 1);
+      mma_commit_to(&o_full);
+    }
+    __syncwarp();
+  } else if (warp >= kPrefixSoftmaxWarps) {
+    // ---- loaders: K and V tiles in turn, the next tile's codes in registers while this one is written
+    constexpr int kLoaders = kPrefixLoaderWarps * 32, kRowUnits = D / 16, kAll = NT * kRowUnits;
+    constexpr int kUnits = (kAll + kLoaders - 1) / kLoaders;  // 16-code units of a thread
+    constexpr int kScalesEach = (NT + kLoaders - 1) / kLoaders;
+    const int lt = tid - kPrefixSoftmaxWarps * 32;
+    const int64_t base = (int64_t)h * a.prefix_capacity;
+    uint4 code[kUnits];
+    float key_scale[kScalesEach], value_scale[kScalesEach];
+    auto fetch = [&](int item) {  // item 2 i: K of tile i, 2 i + 1: V
+      const int8_t* src = (item & 1) ? a.prefix_value_codes : a.prefix_key_codes;
+      const int j = begin + (item >> 1) * NT;
+#pragma unroll
+      for (int u = 0; u < kUnits; u++) {
+        const int unit = u * kLoaders + lt, p = j + unit / kRowUnits;
+        code[u] = unit < kAll && p < end ? __ldg(reinterpret_cast<const uint4*>(src + (base + p) * D) + unit % kRowUnits) : make_uint4(0, 0, 0, 0);
+      }
+      if (item & 1) {
+#pragma unroll
+        for (int u = 0; u < kScalesEach; u++) {
+          const int p = j + u * kLoaders + lt;
+          key_scale[u] = p < end ? __ldg(a.prefix_key_scales + base + p) : 1.0f;  // -inf stays -inf
+          value_scale[u] = p < end ? __ldg(a.prefix_value_scales + base + p) : 0.0f;
+        }
+      }
+    };
+    bool ok = true;
+    fetch(0);
+    for (int item = 0; item < 2 * n; item++) {
+      const int i = item >> 1, st = i % P::kStages;
+      const bool value = item & 1;
+      if (i >= P::kStages) {
+        ok = __all_sync(0xffffffffu, lane != 0 || barrier_wait(value ? &v_empty[st] : &k_empty[st], (i / P::kStages - 1) & 1));
+        if (!ok) break;
+      }
+      unsigned char* to = smem + (value ? P::kV : P::kK) + st * P::kKvTile;
+#pragma unroll
+      for (int u = 0; u < kUnits; u++) {
+        const int unit = u * kLoaders + lt, row = unit / kRowUnits, cc = unit % kRowUnits;
+        if (unit >= kAll) break;
+        const uint32_t w[4] = {code[u].x ^ 0x80808080u, code[u].y ^ 0x80808080u, code[u].z ^ 0x80808080u, code[u].w ^ 0x80808080u};
+        const uint4 lo = make_uint4(codes_f16(w[0], 0x4140), codes_f16(w[0], 0x4342), codes_f16(w[1], 0x4140), codes_f16(w[1], 0x4342));
+        const uint4 hi = make_uint4(codes_f16(w[2], 0x4140), codes_f16(w[2], 0x4342), codes_f16(w[3], 0x4140), codes_f16(w[3], 0x4342));
+        unsigned char* tile = to + (cc >> 2) * P::kKvHalf;
+        // the two 64-dimension halves of a row share banks: they write their two units in opposite order
+        const int flip = (cc >> 2) & 1, at = (cc & 3) * 2;
+        *reinterpret_cast<uint4*>(tile + swizzled(row, at + flip)) = flip ? hi : lo;
+        *reinterpret_cast<uint4*>(tile + swizzled(row, at + 1 - flip)) = flip ? lo : hi;
+      }
+      if (value) {
+        float* s = reinterpret_cast<float*>(smem + P::kScales + st * NT * 8);
+#pragma unroll
+        for (int u = 0; u < kScalesEach; u++)
+          if (u * kLoaders + lt < NT) {
+            s[u * kLoaders + lt] = key_scale[u];
+            s[NT + u * kLoaders + lt] = value_scale[u];
+          }
+      }
+      if (item + 1 < 2 * n) fetch(item + 1);
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) barrier_arrive(value ? &v_full[st] : &k_full[st]);
+    }
+    if (!ok) atomicExch(&failed, 1);
+  } else {
+    // ---- softmax: thread = packed row
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    if (t < tiles_m) {
+      const int64_t i = first + t * 128 + r;
+      const int64_t row = i / group, head = (int64_t)h * group + i % group;
+      const int slot = i < packed ? (a.slots ? a.slots[row] : (int)min(row, (int64_t)0x7fffffff)) : -1;
+      const bool live = slot >= 0 && slot < a.slot_count;
+      // the row's query, scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared memory
+      const T* q = static_cast<const T*>(a.q) + (live ? row * a.q_stride + head * D : 0);
+      constexpr int V = 16 / sizeof(T);
+      const bool vec = live && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+      auto query = [&](int d, float* x) {  // 8 dimensions from d on
+#pragma unroll
+        for (int k = 0; k < 8 / V; k++) {
+          if (vec) {
+            const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(q + d + k * V);
+#pragma unroll
+            for (int e = 0; e < V; e++) x[k * V + e] = to_f32(v.v[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) x[k * V + e] = live ? to_f32(q[d + k * V + e]) : 0.0f;
+          }
+        }
+      };
+      float top = 0.0f;
+#pragma unroll 4
+      for (int d = 0; d < D; d += 8) {
+        float x[8];
+        query(d, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
+      }
+      const int e10 = min(max(exponent_of(top), -110), 110);
+      const float up = power2(10 - e10), inverse = power2(e10 - 10) * (scale * kLog2e);
+#pragma unroll 2
+      for (int d = 0; d < D; d += 8) {
+        float x[8];
+        uint32_t head4[4], tail4[4];
+        query(d, x);
+#pragma unroll
+        for (int e = 0; e < 4; e++) split_f16(x[2 * e] * up, x[2 * e + 1] * up, head4[e], tail4[e]);
+        unsigned char* to = smem + t * P::kQTile + (d >> 6) * P::kQHalf + swizzled(r, (d & 63) >> 3);
+        *reinterpret_cast<uint4*>(to) = make_uint4(head4[0], head4[1], head4[2], head4[3]);
+        if constexpr (SPLIT)
+          *reinterpret_cast<uint4*>(to + P::kHalves * P::kQHalf) = make_uint4(tail4[0], tail4[1], tail4[2], tail4[3]);
+      }
+      fence_async_proxy();
+      __syncwarp();
+      if (lane == 0) barrier_arrive(&q_full);
+
+      const uint32_t mine = tm + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t s_at = mine + P::kS + t * NT, p_at = mine + P::kP + t * P::kPStep, o_at = mine + P::kO + t * D;
+      float M = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int k = 0; k < n; k++) {
+        const int st = k % P::kStages;
+        ok = __all_sync(0xffffffffu, lane != 0 || (barrier_wait(&v_full[st], (k / P::kStages) & 1) && barrier_wait(&s_full[t], k & 1)));
+        if (!ok) break;
+        __syncwarp();
+        tensor_fence_after();
+        const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(smem + P::kScales + st * NT * 8);
+        const ulonglong2* vs = ks + NT / 4;
+        const int valid = min(NT, end - (begin + k * NT));
+        // the row's scores, once from tensor memory, and their maximum
+        uint32_t x[NT];
+#pragma unroll
+        for (int c = 0; c < NT; c += 32) tensor_load32(s_at + c, x + c);
+        tensor_wait_loads();
+        if (valid < NT) hide<NT>(x, valid);
+        float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < NT; j += 4) {
+          const ulonglong2 s2 = ks[j / 4];
+          float v[4];
+          apart(mul2(two(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), Two{s2.x}), v[0], v[1]);
+          apart(mul2(two(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), Two{s2.y}), v[2], v[3]);
+#pragma unroll
+          for (int o = 0; o < 4; o++) x[j + o] = __float_as_uint(v[o]);
+          most4[(j / 4) & 1] = max3(most4[(j / 4) & 1], v[0], v[1]);
+          most4[2 + ((j / 4) & 1)] = max3(most4[2 + ((j / 4) & 1)], v[2], v[3]);
+        }
+        const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
+        const float* v1 = reinterpret_cast<const float*>(vs);
+        uint32_t vtop = 0;
+#pragma unroll
+        for (int c = 0; c < NT; c += 32) vtop = max(vtop, __float_as_uint(v1[c + lane]) & 0x7fffffffu);
+        vtop = __reduce_max_sync(0xffffffffu, vtop);
+        const int ev = min(max(exponent_of(__uint_as_float(vtop)), -100), 100) - 6;
+        const float reach = most * inverse + (float)ev;  // weights are below 2^(reach - M + 7)
+        const bool raise = reach > M + kRaise;
+        if (__any_sync(0xffffffffu, raise)) {
+          const float Mn = raise ? reach + 1.0f : M;
+          const float f = M == -INFINITY ? 0.0f : power2f(M - Mn);
+          l *= f;
+          M = Mn;
+          if (k > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t y[16];
+              tensor_load16(o_at + c, y);
+              tensor_wait_loads();
+#pragma unroll
+              for (int j = 0; j < 16; j++) y[j] = __float_as_uint(__uint_as_float(y[j]) * f);
+              tensor_store16(o_at + c, y);
+            }
+          }
+        }
+        const Two inverse2 = two(inverse, inverse), minus = two(-M, -M);
+        Two sum = two(0.0f, 0.0f);
+#pragma unroll
+        for (int c = 0; c < NT; c += 32) {
+          uint32_t head16[16], tail16[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const ulonglong2 v2 = vs[(c + j) / 4];
+#pragma unroll
+            for (int o = 0; o < 4; o += 2) {
+              float e0, e1;
+              apart(fma2(two(__uint_as_float(x[c + j + o]), __uint_as_float(x[c + j + o + 1])), inverse2, minus), e0, e1);
+              e0 = power2f(e0);
+              e1 = power2f(e1);
+              const Two p2 = two(e0, e1);
+              sum = add2(sum, p2);
+              float w0, w1;
+              apart(mul2(p2, Two{o ? v2.y : v2.x}), w0, w1);
+              if constexpr (SPLIT) split_f16(w0, w1, head16[(j + o) / 2], tail16[(j + o) / 2]);
+              else head16[(j + o) / 2] = half2_bits(__floats2half2_rn(w0, w1));
+            }
+          }
+          tensor_store16(p_at + c / 2, head16);
+          if constexpr (SPLIT) tensor_store16(p_at + NT / 2 + c / 2, tail16);
+        }
+        float s0, s1;
+        apart(sum, s0, s1);
+        l += s0 + s1;
+        tensor_wait_stores();
+        tensor_fence_before();
+        __syncwarp();
+        if (lane == 0) barrier_arrive(&p_full[t]);
+      }
+      if (!ok) atomicExch(&failed, 1);
+      const bool done = __all_sync(0xffffffffu, lane != 0 || barrier_wait(&o_full, 0));
+      tensor_fence_after();
+      const bool bad = !ok || !done || *(volatile int*)&failed != 0;
+      if (bad && lane == 0) report_wait_timeout(wait_words, kWaitAttention);
+      const int64_t part = blockIdx.z * parts.per_part + row * a.heads + head;
+      if (live) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l);
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t x[32];
+        tensor_load32(o_at + c, x);
+        tensor_wait_loads();
+        if (live) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint4*>(parts.o + part * D + c + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        }
+      }
+    }
+  }
+  tensor_fence_before();
+  __syncthreads();
+  if (warp == kPrefixMmaWarp) {
+    tensor_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u) : "memory");
+  }
+}
+
+}  // namespace
+
+int prefix_tile(int32_t type) { return type == NEEDLE_TYPE_F32 ? PrefixShape<64, true>::kNT : PrefixShape<64, false>::kNT; }
+int prefix_rows() { return kPrefixRows; }
+
+cudaError_t launch_attend_prefix(const needle_prefix_attention& a, const Parts& out, int parts, int part_len, float scale,
+                                 uint32_t* wait_words, cudaStream_t s) {
+  return with_type(a.type, [&](auto zero) {
+    using T = decltype(zero);
+    constexpr bool kSplit = sizeof(T) == 4;
+    const int64_t packed = int64_t(a.rows) * (a.heads / a.kv_heads);
+    const dim3 grid((unsigned)((packed + kPrefixRows - 1) / kPrefixRows), a.kv_heads, parts);
+    auto go = [&](auto kernel, size_t smem) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return e;
+      kernel<<<grid, kPrefixThreads, smem, s>>>(a, out, part_len, scale, wait_words);
+      return cudaGetLastError();
+    };
+    return a.head_dim == 64 ? go(k_attend_prefix<T, 64, kSplit>, PrefixShape<64, kSplit>::kSmem)
+                            : go(k_attend_prefix<T, 128, kSplit>, PrefixShape<128, kSplit>::kSmem);
+  });
+}
+
+}  // namespace needle
