@@ -17,8 +17,8 @@
 //   K: lane (n, c) = (lane / 4, lane % 4) reads D / 4 codes of position n; k-step t takes 4 of them;
 //   V: the lane reads D / 8 codes of the positions 2c, 2c + 1, 2c + 8, 2c + 9, which are the ones whose
 //      weights the score product left in its registers; output tile j takes code j of each.
-// `warps` warps share a unit (row, KV head, 8 heads, split of the positions) and are merged in shared
-// memory; splits and the prefix's parts are merged from the workspace.
+// A CTA is one unit (row, KV head, 8 heads, split of the positions): 1 to 8 warps, merged in shared memory;
+// with many units a single warp, since caches of different ages would leave the others of a CTA idle; splits and the prefix's parts are merged from the workspace.
 #include <algorithm>
 #include <cmath>
 
@@ -238,118 +238,108 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
   __shared__ __align__(8) uint64_t full[kStreamWarps][kStreamStages];
   __shared__ float merge_m[kStreamWarps][kGroupHeads], merge_l[kStreamWarps][kGroupHeads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-  const int share = plan.warps, member = warp & (share - 1);
-  const int64_t units = (int64_t)a.rows * a.kv_heads * plan.groups;
-  const int64_t unit = (int64_t)blockIdx.x * (kStreamWarps / share) + warp / share;
-  const int split = blockIdx.y, group = a.heads / a.kv_heads;
-  bool live = unit < units;
-  const int row = live ? (int)(unit / (a.kv_heads * plan.groups)) : 0;
-  const int rest = live ? (int)(unit - (int64_t)row * (a.kv_heads * plan.groups)) : 0;
+  const int share = plan.warps, member = warp;
+  const int split = blockIdx.y, group = a.heads / a.kv_heads, of_row = a.kv_heads * plan.groups;
+  const int row = (int)(blockIdx.x / of_row), rest = (int)(blockIdx.x - row * of_row);
   const int h = rest / plan.groups, g0 = (rest - h * plan.groups) * kGroupHeads;
   const int heads = min(kGroupHeads, group - g0);
-  const int slot = live ? (a.slots ? a.slots[row] : row) : -1;
-  live = live && slot >= 0 && slot < a.slot_count;
+  const int slot = a.slots ? a.slots[row] : row;
+  if (slot < 0 || slot >= a.slot_count) return;
   const int64_t head = (int64_t)h * group + g0;  // the unit's first query head
   Rows<D> r;
   bool ok = true;
-  if (live) {
-    Stage<D>* ring = reinterpret_cast<Stage<D>*>(raw) + warp * kStreamStages;
-    uint64_t* bars = full[warp];
-    if (lane == 0) {
-      for (int s = 0; s < kStreamStages; s++) barrier_init(&bars[s], 33);  // each lane's scale copies, and the codes
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
-    const int count = min(max(a.counts[row], 0), a.capacity);
-    const int64_t own = ((int64_t)slot * a.kv_heads + h) * a.capacity, shared = (int64_t)h * a.prefix_capacity;
-    const int prefix = plan.parts ? 0 : a.prefix_length;
-    // positions [from, to) of prefix ++ own cache, in blocks that do not straddle the two
-    const int64_t from = (int64_t)split * plan.split_len, to = min(from + plan.split_len, (int64_t)prefix + count);
-    const int begin0 = (int)min(from, (int64_t)prefix), end0 = (int)min(max(to, (int64_t)0), (int64_t)prefix);
-    const int begin1 = (int)max(from - prefix, (int64_t)0), end1 = (int)max(to - prefix, (int64_t)begin1);
-    const int blocks0 = max(end0 - begin0 + kBlock - 1, 0) / kBlock, blocks1 = (end1 - begin1 + kBlock - 1) / kBlock;
-    const int mine = (blocks0 + blocks1 - member + share - 1) / share;  // blocks member, member + share, ...
-    auto length = [&](int i) {
-      const int b = member + i * share;
-      return min(kBlock, b < blocks0 ? end0 - begin0 - b * kBlock : end1 - begin1 - (b - blocks0) * kBlock);
-    };
-    auto issue = [&](int i) {
-      const int b = member + i * share, n = length(i);
-      const bool pre = b < blocks0;
-      const int64_t at = pre ? shared + begin0 + b * kBlock : own + begin1 + (b - blocks0) * kBlock;
-      Stage<D>& s = ring[i % kStreamStages];
-      uint64_t* bar = &bars[i % kStreamStages];
-      if (lane == 0) {
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(bar)), "r"((uint32_t)(2 * n * D))
-                     : "memory");
-        copy_bulk(s.k, (pre ? a.prefix_key_codes : a.key_codes) + at * D, n * D, bar);
-        copy_bulk(s.v, (pre ? a.prefix_value_codes : a.value_codes) + at * D, n * D, bar);
-      }
-      const int p = min(lane, n - 1), bytes = lane < n ? 4 : 0;  // zeros behind the last position
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(&s.ks[lane])),
-                   "l"((pre ? a.prefix_key_scales : a.key_scales) + at + p), "r"(bytes)
-                   : "memory");
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(&s.vs[lane])),
-                   "l"((pre ? a.prefix_value_scales : a.value_scales) + at + p), "r"(bytes)
-                   : "memory");
-      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
-    };
-#pragma unroll
-    for (int i = 0; i < kStreamStages - 1; i++)
-      if (i < mine) issue(i);
-    load_queries<T, D>(r, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, scale, lane);
-    int i = 0;
-#pragma unroll 1
-    for (; i < mine; i++) {
-      ok = __all_sync(0xffffffffu, barrier_wait(&bars[i % kStreamStages], (uint32_t)(i / kStreamStages) & 1));
-      if (!ok) break;
-      // the stage of block i - 1 has been read by every lane that came here
-      if (i + kStreamStages - 1 < mine) issue(i + kStreamStages - 1);
-      attend_block<D>(r, ring[i % kStreamStages], length(i), lane);
-    }
-    if (!ok) {  // copies may still be landing: give them their time before the memory is let go
-      for (int k = i; k < min(mine, i + kStreamStages - 1); k++) barrier_wait(&bars[k % kStreamStages], (uint32_t)(k / kStreamStages) & 1);
-      if (lane == 0) report_wait_timeout(wait_words, kWaitAttention);
-      r.M = 0.0f;
-      r.l = NAN;
-    }
-    r.l += __shfl_xor_sync(0xffffffffu, r.l, 1);
-    r.l += __shfl_xor_sync(0xffffffffu, r.l, 2);
+  Stage<D>* ring = reinterpret_cast<Stage<D>*>(raw) + warp * kStreamStages;
+  uint64_t* bars = full[warp];
+  if (lane == 0) {
+    for (int s = 0; s < kStreamStages; s++) barrier_init(&bars[s], 33);  // each lane's scale copies, and the codes
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  __syncwarp();
+  const int count = min(max(a.counts[row], 0), a.capacity);
+  const int64_t own = ((int64_t)slot * a.kv_heads + h) * a.capacity, shared = (int64_t)h * a.prefix_capacity;
+  const int prefix = plan.parts ? 0 : a.prefix_length;
+  // positions [from, to) of prefix ++ own cache, in blocks that do not straddle the two
+  const int64_t from = (int64_t)split * plan.split_len, to = min(from + plan.split_len, (int64_t)prefix + count);
+  const int begin0 = (int)min(from, (int64_t)prefix), end0 = (int)min(max(to, (int64_t)0), (int64_t)prefix);
+  const int begin1 = (int)max(from - prefix, (int64_t)0), end1 = (int)max(to - prefix, (int64_t)begin1);
+  const int blocks0 = max(end0 - begin0 + kBlock - 1, 0) / kBlock, blocks1 = (end1 - begin1 + kBlock - 1) / kBlock;
+  const int mine = (blocks0 + blocks1 - member + share - 1) / share;  // blocks member, member + share, ...
+  auto length = [&](int i) {
+    const int b = member + i * share;
+    return min(kBlock, b < blocks0 ? end0 - begin0 - b * kBlock : end1 - begin1 - (b - blocks0) * kBlock);
+  };
+  auto issue = [&](int i) {
+    const int b = member + i * share, n = length(i);
+    const bool pre = b < blocks0;
+    const int64_t at = pre ? shared + begin0 + b * kBlock : own + begin1 + (b - blocks0) * kBlock;
+    Stage<D>& s = ring[i % kStreamStages];
+    uint64_t* bar = &bars[i % kStreamStages];
+    if (lane == 0) {
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(bar)), "r"((uint32_t)(2 * n * D))
+                   : "memory");
+      copy_bulk(s.k, (pre ? a.prefix_key_codes : a.key_codes) + at * D, n * D, bar);
+      copy_bulk(s.v, (pre ? a.prefix_value_codes : a.value_codes) + at * D, n * D, bar);
+    }
+    const int p = min(lane, n - 1), bytes = lane < n ? 4 : 0;  // zeros behind the last position
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(&s.ks[lane])),
+                 "l"((pre ? a.prefix_key_scales : a.key_scales) + at + p), "r"(bytes)
+                 : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(&s.vs[lane])),
+                 "l"((pre ? a.prefix_value_scales : a.value_scales) + at + p), "r"(bytes)
+                 : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStreamStages - 1; i++)
+    if (i < mine) issue(i);
+  load_queries<T, D>(r, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, scale, lane);
+  int i = 0;
+#pragma unroll 1
+  for (; i < mine; i++) {
+    ok = __all_sync(0xffffffffu, barrier_wait(&bars[i % kStreamStages], (uint32_t)(i / kStreamStages) & 1));
+    if (!ok) break;
+    // the stage of block i - 1 has been read by every lane that came here
+    if (i + kStreamStages - 1 < mine) issue(i + kStreamStages - 1);
+    attend_block<D>(r, ring[i % kStreamStages], length(i), lane);
+  }
+  if (!ok) {  // copies may still be landing: give them their time before the memory is let go
+    for (int k = i; k < min(mine, i + kStreamStages - 1); k++) barrier_wait(&bars[k % kStreamStages], (uint32_t)(k / kStreamStages) & 1);
+    if (lane == 0) report_wait_timeout(wait_words, kWaitAttention);
+    r.M = 0.0f;
+    r.l = NAN;
+  }
+  r.l += __shfl_xor_sync(0xffffffffu, r.l, 1);
+  r.l += __shfl_xor_sync(0xffffffffu, r.l, 2);
   // the lane's output dimensions in order, the two row halves of the accumulators added
   float o[N];
-  if (live) {
 #pragma unroll
-    for (int t = 0; t < Rows<D>::kTiles; t++) {
-      o[t] = r.o[t][0] + r.o[t][2];
-      o[N / 2 + t] = r.o[t][1] + r.o[t][3];
-    }
+  for (int t = 0; t < Rows<D>::kTiles; t++) {
+    o[t] = r.o[t][0] + r.o[t][2];
+    o[N / 2 + t] = r.o[t][1] + r.o[t][3];
   }
   if (share > 1) {
     float* merge_o = reinterpret_cast<float*>(raw);  // [warps][8][D], where the rings were
     __syncthreads();
-    if (live) {
-      if (c == 0) {
-        merge_m[warp][g] = r.M;
-        merge_l[warp][g] = r.l;
-      }
-#pragma unroll
-      for (int i = 0; i < N; i += 4)
-        *reinterpret_cast<float4*>(&merge_o[(warp * kGroupHeads + g) * D + c * N + i]) =
-            make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+    if (c == 0) {
+      merge_m[warp][g] = r.M;
+      merge_l[warp][g] = r.l;
     }
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(&merge_o[(warp * kGroupHeads + g) * D + c * N + i]) =
+          make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
     __syncthreads();
-    if (!live || member != 0) return;
+    if (member != 0) return;
     float M = -INFINITY, L = 0.0f;
-    for (int w = 0; w < share; w++) M = fmaxf(M, merge_m[warp + w][g]);
+    for (int w = 0; w < share; w++) M = fmaxf(M, merge_m[w][g]);
 #pragma unroll
     for (int i = 0; i < N; i++) o[i] = 0.0f;
     for (int w = 0; w < share; w++) {
-      const float m = merge_m[warp + w][g], f = m == -INFINITY ? 0.0f : power2f(m - M);
-      L = fmaf(merge_l[warp + w][g], f, L);
+      const float m = merge_m[w][g], f = m == -INFINITY ? 0.0f : power2f(m - M);
+      L = fmaf(merge_l[w][g], f, L);
 #pragma unroll
       for (int i = 0; i < N; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(&merge_o[((warp + w) * kGroupHeads + g) * D + c * N + i]);
+        const float4 v = *reinterpret_cast<const float4*>(&merge_o[(w * kGroupHeads + g) * D + c * N + i]);
         o[i] = fmaf(v.x, f, o[i]);
         o[i + 1] = fmaf(v.y, f, o[i + 1]);
         o[i + 2] = fmaf(v.z, f, o[i + 2]);
@@ -359,7 +349,7 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
     r.M = M;
     r.l = L;
   }
-  if (!live || g >= heads) return;
+  if (g >= heads) return;
   const int64_t at = (int64_t)row * a.heads + head + g;
   if (plan.splits > 1) {
     const int64_t part = (int64_t)(plan.parts + split) * parts.per_part + at;
@@ -490,12 +480,12 @@ cudaError_t launch_attention(const needle_prefix_attention& a, const StreamPlan&
     if (e != cudaSuccess) return e;
   }
   const int64_t units = int64_t(a.rows) * a.kv_heads * p.groups;
-  const int per_cta = kStreamWarps / p.warps;
-  constexpr size_t smem = sizeof(Stage<D>) * kStreamStages * kStreamWarps;
-  static_assert(smem >= size_t(kStreamWarps) * kGroupHeads * D * 4, "the merge takes the rings' place");
-  cudaError_t e = cudaFuncSetAttribute(k_attend_stream<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const size_t smem = sizeof(Stage<D>) * kStreamStages * p.warps;
+  static_assert(sizeof(Stage<D>) * kStreamStages >= size_t(kGroupHeads) * D * 4, "the merge takes the rings' place");
+  cudaError_t e = cudaFuncSetAttribute(k_attend_stream<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       int(sizeof(Stage<D>) * kStreamStages * kStreamWarps));
   if (e != cudaSuccess) return e;
-  k_attend_stream<T, D><<<dim3((unsigned)((units + per_cta - 1) / per_cta), p.splits), kStreamThreads, smem, s>>>(a, p, parts, scale, wait_words);
+  k_attend_stream<T, D><<<dim3((unsigned)units, p.splits), p.warps * 32, smem, s>>>(a, p, parts, scale, wait_words);
   e = cudaGetLastError();
   if (e != cudaSuccess || p.splits == 1) return e;
   k_attend_merge<T, D><<<(unsigned)((parts.per_part + kStreamWarps - 1) / kStreamWarps), kStreamThreads, 0, s>>>(a, part_count(p), parts);
@@ -508,6 +498,7 @@ int check_attention(const needle_prefix_attention* a) {
   if (a->head_dim != 64 && a->head_dim != 128) return refuse("head dimensions of 64 and 128 only");
   if (a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads != 0 || a->heads > 4096)
     return refuse("heads must be a multiple of kv_heads, at most 4096");
+  if (int64_t(a->rows) * a->heads > 0x7fffffff) return refuse("rows times heads must stay below 2^31");
   if (a->rows < 0 || a->prefix_length < 0 || a->slot_count < 0 || a->capacity < 0)
     return refuse("bad row, position or slot count");
   if (a->prefix_length > a->prefix_capacity) return refuse("the prefix is longer than its capacity");

@@ -31,6 +31,7 @@ constexpr int kPrefixSoftmaxWarps = 8, kPrefixLoaderWarps = 3;
 constexpr int kPrefixMmaWarp = kPrefixSoftmaxWarps + kPrefixLoaderWarps;
 constexpr int kPrefixThreads = (kPrefixMmaWarp + 1) * 32;
 constexpr int kPrefixRows = 256;  // packed rows of a CTA
+constexpr int kTurnRow = 36;      // floats of a row in the epilogue's transposition
 
 template <int D, bool SPLIT>
 struct PrefixShape {
@@ -44,6 +45,7 @@ struct PrefixShape {
   static constexpr uint32_t kKvTile = kKvHalf * kHalves;
   static constexpr uint32_t kK = 2 * kQTile, kV = kK + kStages * kKvTile;
   static constexpr uint32_t kScales = kV + kStages * kKvTile;         // per stage: kNT key, kNT value scales
+  static_assert(2 * kStages * kKvTile >= kPrefixSoftmaxWarps * 32 * kTurnRow * 4, "the epilogue takes the rings' place");
   static constexpr uint32_t kSmem = kScales + kStages * kNT * 8 + 1024;
   // tensor memory columns
   static constexpr uint32_t kS = 0;                                    // two tiles of kNT
@@ -88,15 +90,10 @@ __device__ __forceinline__ void mma_commit_to(uint64_t* b) {
 }
 
 // 32 (16) consecutive columns of this thread's lane of tensor memory.
-__device__ __forceinline__ void tensor_load32(uint32_t at, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(at));
+__device__ __forceinline__ void tensor_load32(uint32_t at, float2* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : "=f"(v[0].x), "=f"(v[0].y), "=f"(v[1].x), "=f"(v[1].y), "=f"(v[2].x), "=f"(v[2].y), "=f"(v[3].x), "=f"(v[3].y), "=f"(v[4].x), "=f"(v[4].y), "=f"(v[5].x), "=f"(v[5].y), "=f"(v[6].x), "=f"(v[6].y), "=f"(v[7].x), "=f"(v[7].y), "=f"(v[8].x), "=f"(v[8].y), "=f"(v[9].x), "=f"(v[9].y), "=f"(v[10].x), "=f"(v[10].y), "=f"(v[11].x), "=f"(v[11].y), "=f"(v[12].x), "=f"(v[12].y), "=f"(v[13].x), "=f"(v[13].y), "=f"(v[14].x), "=f"(v[14].y), "=f"(v[15].x), "=f"(v[15].y)
+               : "r"(at));
 }
 __device__ __forceinline__ void tensor_load16(uint32_t at, uint32_t* v) {
   asm volatile(
@@ -121,31 +118,6 @@ __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fen
 // Shared-memory writes of this thread before reads of the tensor cores.
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Two binary32 values at once.
-struct Two {
-  uint64_t v;
-};
-__device__ __forceinline__ Two two(float a, float b) {
-  Two r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void apart(Two t, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(t.v)); }
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-  Two r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-  Two r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-  Two r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -154,10 +126,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // Scores from position `valid` on become -inf.
 template <int N>
-__device__ __forceinline__ void hide(uint32_t* x, int valid) {
+__device__ __forceinline__ void hide(float2* x, int valid) {
 #pragma unroll
-  for (int j = 0; j < N; j++)
-    if (j >= valid) x[j] = 0xff800000u;
+  for (int j = 0; j < N / 2; j++) {
+    if (2 * j >= valid) x[j].x = -INFINITY;
+    if (2 * j + 1 >= valid) x[j].y = -INFINITY;
+  }
 }
 
 template <class T, int D, bool SPLIT>
@@ -340,46 +314,51 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     if (t < tiles_m) {
       const int64_t i = first + t * 128 + r;
       const int64_t row = i / group, head = (int64_t)h * group + i % group;
-      const int slot = i < packed ? (a.slots ? a.slots[row] : (int)min(row, (int64_t)0x7fffffff)) : -1;
+      const int slot = i < packed ? (a.slots ? a.slots[row] : (int)row) : -1;
       const bool live = slot >= 0 && slot < a.slot_count;
-      // the row's query, scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared memory
-      const T* q = static_cast<const T*>(a.q) + (live ? row * a.q_stride + head * D : 0);
-      constexpr int V = 16 / sizeof(T);
-      const bool vec = live && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-      auto query = [&](int d, float* x) {  // 8 dimensions from d on
+      // the warp's 32 queries, each scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared
+      // memory: kLanes lanes take a row, 16 bytes each
+      constexpr int V = 16 / sizeof(T), kLanes = D / V, kAtOnce = 32 / kLanes, kBatch = 8;
+      const int64_t offset = live ? row * a.q_stride + head * D : -1;
+      const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_stride * (int64_t)sizeof(T) & 15) == 0;
+      const int d0 = lane % kLanes * V;
+      float inverse = 0.0f;
+#pragma unroll 1
+      for (int b = 0; b < kLanes; b += kBatch) {
+        Vec<T, V> in[kBatch];
 #pragma unroll
-        for (int k = 0; k < 8 / V; k++) {
-          if (vec) {
-            const Vec<T, V> v = *reinterpret_cast<const Vec<T, V>*>(q + d + k * V);
-#pragma unroll
-            for (int e = 0; e < V; e++) x[k * V + e] = to_f32(v.v[e]);
+        for (int k = 0; k < kBatch; k++) {
+          const int64_t at = __shfl_sync(0xffffffffu, offset, (b + k) * kAtOnce + lane / kLanes);
+          const T* q = static_cast<const T*>(a.q) + at + d0;
+          if (at < 0) {
+            in[k] = Vec<T, V>{};
+          } else if (vec) {
+            in[k] = *reinterpret_cast<const Vec<T, V>*>(q);
           } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) x[k * V + e] = live ? to_f32(q[d + k * V + e]) : 0.0f;
+            for (int e = 0; e < V; e++) in[k].v[e] = q[e];
           }
         }
-      };
-      float top = 0.0f;
-#pragma unroll 4
-      for (int d = 0; d < D; d += 8) {
-        float x[8];
-        query(d, x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
-      }
-      const int e10 = min(max(exponent_of(top), -110), 110);
-      const float up = power2(10 - e10), inverse = power2(e10 - 10) * (scale * kLog2e);
-#pragma unroll 2
-      for (int d = 0; d < D; d += 8) {
-        float x[8];
-        uint32_t head4[4], tail4[4];
-        query(d, x);
+        for (int k = 0; k < kBatch; k++) {
+          float top = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) split_f16(x[2 * e] * up, x[2 * e + 1] * up, head4[e], tail4[e]);
-        unsigned char* to = smem + t * P::kQTile + (d >> 6) * P::kQHalf + swizzled(r, (d & 63) >> 3);
-        *reinterpret_cast<uint4*>(to) = make_uint4(head4[0], head4[1], head4[2], head4[3]);
-        if constexpr (SPLIT)
-          *reinterpret_cast<uint4*>(to + P::kHalves * P::kQHalf) = make_uint4(tail4[0], tail4[1], tail4[2], tail4[3]);
+          for (int e = 0; e < V; e++) top = fmaxf(top, fabsf(to_f32(in[k].v[e])));
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const int e10 = min(max(exponent_of(top), -110), 110), r0 = (b + k) * kAtOnce, rr = r0 + lane / kLanes;
+          const float up = power2(10 - e10);
+          alignas(16) uint32_t heads[V / 2], tails[V / 2];
+#pragma unroll
+          for (int e = 0; e < V / 2; e++) split_f16(to_f32(in[k].v[2 * e]) * up, to_f32(in[k].v[2 * e + 1]) * up, heads[e], tails[e]);
+          unsigned char* to = smem + t * P::kQTile + (d0 >> 6) * P::kQHalf + swizzled(quarter * 32 + rr, (d0 & 63) >> 3) + (d0 & 7) * 2;
+          *reinterpret_cast<Vec<uint32_t, V / 2>*>(to) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(heads);
+          if constexpr (SPLIT)
+            *reinterpret_cast<Vec<uint32_t, V / 2>*>(to + P::kHalves * P::kQHalf) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(tails);
+          // the row's own lane keeps what undoes the scaling
+          const float back = __shfl_sync(0xffffffffu, power2(e10 - 10) * (scale * kLog2e), (lane - r0) * kLanes & 31);
+          if (lane >= r0 && lane < r0 + kAtOnce) inverse = back;
+        }
       }
       fence_async_proxy();
       __syncwarp();
@@ -395,32 +374,29 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (!ok) break;
         __syncwarp();
         tensor_fence_after();
-        const ulonglong2* ks = reinterpret_cast<const ulonglong2*>(smem + P::kScales + st * NT * 8);
-        const ulonglong2* vs = ks + NT / 4;
+        const float4* ks = reinterpret_cast<const float4*>(smem + P::kScales + st * NT * 8);
+        const float4* vs = ks + NT / 4;
         const int valid = min(NT, end - (begin + k * NT));
         // the row's scores, once from tensor memory, and their maximum
-        uint32_t x[NT];
+        float2 x[NT / 2];
 #pragma unroll
-        for (int c = 0; c < NT; c += 32) tensor_load32(s_at + c, x + c);
+        for (int c = 0; c < NT; c += 32) tensor_load32(s_at + c, x + c / 2);
         tensor_wait_loads();
         if (valid < NT) hide<NT>(x, valid);
         float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < NT; j += 4) {
-          const ulonglong2 s2 = ks[j / 4];
-          float v[4];
-          apart(mul2(two(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), Two{s2.x}), v[0], v[1]);
-          apart(mul2(two(__uint_as_float(x[j + 2]), __uint_as_float(x[j + 3])), Two{s2.y}), v[2], v[3]);
-#pragma unroll
-          for (int o = 0; o < 4; o++) x[j + o] = __float_as_uint(v[o]);
-          most4[(j / 4) & 1] = max3(most4[(j / 4) & 1], v[0], v[1]);
-          most4[2 + ((j / 4) & 1)] = max3(most4[2 + ((j / 4) & 1)], v[2], v[3]);
+        for (int j = 0; j < NT / 2; j += 2) {
+          const float4 s4 = ks[j / 2];
+          x[j] = __fmul2_rn(x[j], make_float2(s4.x, s4.y));
+          x[j + 1] = __fmul2_rn(x[j + 1], make_float2(s4.z, s4.w));
+          most4[j & 2] = max3(most4[j & 2], x[j].x, x[j].y);
+          most4[1 + (j & 2)] = max3(most4[1 + (j & 2)], x[j + 1].x, x[j + 1].y);
         }
         const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
-        const float* v1 = reinterpret_cast<const float*>(vs);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(vs);
         uint32_t vtop = 0;
 #pragma unroll
-        for (int c = 0; c < NT; c += 32) vtop = max(vtop, __float_as_uint(v1[c + lane]) & 0x7fffffffu);
+        for (int c = 0; c < NT; c += 32) vtop = max(vtop, v1[c + lane] & 0x7fffffffu);
         vtop = __reduce_max_sync(0xffffffffu, vtop);
         const int ev = min(max(exponent_of(__uint_as_float(vtop)), -100), 100) - 6;
         const float reach = most * inverse + (float)ev;  // weights are below 2^(reach - M + 7)
@@ -442,34 +418,29 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             }
           }
         }
-        const Two inverse2 = two(inverse, inverse), minus = two(-M, -M);
-        Two sum = two(0.0f, 0.0f);
+        const float2 inverse2 = make_float2(inverse, inverse), minus = make_float2(-M, -M);
+        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int c = 0; c < NT; c += 32) {
-          uint32_t head16[16], tail16[16];
+          uint32_t heads[16], tails[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const ulonglong2 v2 = vs[(c + j) / 4];
+          for (int j = 0; j < 16; j += 2) {
+            const float4 v4 = vs[(c + 2 * j) / 4];
 #pragma unroll
-            for (int o = 0; o < 4; o += 2) {
-              float e0, e1;
-              apart(fma2(two(__uint_as_float(x[c + j + o]), __uint_as_float(x[c + j + o + 1])), inverse2, minus), e0, e1);
-              e0 = power2f(e0);
-              e1 = power2f(e1);
-              const Two p2 = two(e0, e1);
-              sum = add2(sum, p2);
-              float w0, w1;
-              apart(mul2(p2, Two{o ? v2.y : v2.x}), w0, w1);
-              if constexpr (SPLIT) split_f16(w0, w1, head16[(j + o) / 2], tail16[(j + o) / 2]);
-              else head16[(j + o) / 2] = half2_bits(__floats2half2_rn(w0, w1));
+            for (int o = 0; o < 2; o++) {
+              float2 p = __ffma2_rn(x[c / 2 + j + o], inverse2, minus);
+              p.x = power2f(p.x);
+              p.y = power2f(p.y);
+              sum = __fadd2_rn(sum, p);
+              const float2 w = __fmul2_rn(p, o ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
+              if constexpr (SPLIT) split_f16(w.x, w.y, heads[j + o], tails[j + o]);
+              else heads[j + o] = half2_bits(__floats2half2_rn(w.x, w.y));
             }
           }
-          tensor_store16(p_at + c / 2, head16);
-          if constexpr (SPLIT) tensor_store16(p_at + NT / 2 + c / 2, tail16);
+          tensor_store16(p_at + c / 2, heads);
+          if constexpr (SPLIT) tensor_store16(p_at + NT / 2 + c / 2, tails);
         }
-        float s0, s1;
-        apart(sum, s0, s1);
-        l += s0 + s1;
+        l += sum.x + sum.y;
         tensor_wait_stores();
         tensor_fence_before();
         __syncwarp();
@@ -482,16 +453,27 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       if (bad && lane == 0) report_wait_timeout(wait_words, kWaitAttention);
       const int64_t part = blockIdx.z * parts.per_part + row * a.heads + head;
       if (live) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l);
+      // 32 columns at a time through shared memory (the K and V rings are free), so that rows are written
+      // 128 bytes at once
+      float* turn = reinterpret_cast<float*>(smem + P::kK) + warp * 32 * kTurnRow;
+      const int64_t to = live ? part * D : -1;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
-        uint32_t x[32];
+        float2 x[16];
         tensor_load32(o_at + c, x);
         tensor_wait_loads();
-        if (live) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint4*>(parts.o + part * D + c + j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        for (int j = 0; j < 16; j += 2)
+          *reinterpret_cast<float4*>(turn + lane * kTurnRow + 2 * j) = make_float4(x[j].x, x[j].y, x[j + 1].x, x[j + 1].y);
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int rr = k * 4 + (lane >> 3);
+          const int64_t at = __shfl_sync(0xffffffffu, to, rr);
+          const float4 v = *reinterpret_cast<const float4*>(turn + rr * kTurnRow + (lane & 7) * 4);
+          if (at >= 0) *reinterpret_cast<float4*>(parts.o + at + c + (lane & 7) * 4) = v;
         }
+        __syncwarp();
       }
     }
   }
