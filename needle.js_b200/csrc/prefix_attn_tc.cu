@@ -9,8 +9,8 @@
 //   MMA warp        S_t = Q_t K^T (tcgen05.mma, both from shared memory) and O_t += P_t V (P from
 //                   tensor memory), for the two tiles t in turn, so that one tile's products run while
 //                   the other's softmax does
-//   softmax warps   two warpgroups, one thread per packed row: a tile's S into registers, maximum,
-//                   exponentials, P back to tensor memory as fp16; O stays in tensor memory and is only
+//   softmax warps   eight for each tile, two threads a packed row: half a tile's S into registers, maximum
+//                   (of both halves, through shared memory), exponentials, P back to tensor memory as fp16; O stays in tensor memory and is only
 //                   rescaled when a tile exceeds the reference maximum by 2^7
 // The reference M of a row covers the value scale too: a weight is 2^(s - M) vs <= 2^15, inside fp16, and
 // sums and outputs share the factor, which cancels.  16-bit queries are exact in fp16 after their row's
@@ -27,7 +27,8 @@ namespace needle {
 
 namespace {
 
-constexpr int kPrefixSoftmaxWarps = 8, kPrefixLoaderWarps = 3;
+constexpr int kPrefixSoftmaxWarps = 16, kPrefixLoaderWarps = 3;
+constexpr int kTileWarps = kPrefixSoftmaxWarps / 2;  // softmax warps of a tile: two for each 32 rows
 constexpr int kPrefixMmaWarp = kPrefixSoftmaxWarps + kPrefixLoaderWarps;
 constexpr int kPrefixThreads = (kPrefixMmaWarp + 1) * 32;
 constexpr int kPrefixRows = 256;  // packed rows of a CTA
@@ -45,7 +46,7 @@ struct PrefixShape {
   static constexpr uint32_t kKvTile = kKvHalf * kHalves;
   static constexpr uint32_t kK = 2 * kQTile, kV = kK + kStages * kKvTile;
   static constexpr uint32_t kScales = kV + kStages * kKvTile;         // per stage: kNT key, kNT value scales
-  static_assert(2 * kStages * kKvTile >= kPrefixSoftmaxWarps * 32 * kTurnRow * 4, "the epilogue takes the rings' place");
+  static_assert(kScales >= kPrefixSoftmaxWarps * 32 * kTurnRow * 4, "the epilogue takes the operands' place");
   static constexpr uint32_t kSmem = kScales + kStages * kNT * 8 + 1024;
   // tensor memory columns
   static constexpr uint32_t kS = 0;                                    // two tiles of kNT
@@ -145,6 +146,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   __shared__ __align__(8) uint64_t k_full[P::kStages], k_empty[P::kStages], v_full[P::kStages], v_empty[P::kStages];
   __shared__ uint32_t tensor_base;
   __shared__ int failed;
+  __shared__ float row_inverse[kPrefixRows], exchange[2][2][128];  // [tile][column half][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int h = blockIdx.y, group = a.heads / a.kv_heads;
   const int64_t packed = (int64_t)a.rows * group, first = (int64_t)blockIdx.x * kPrefixRows;
@@ -155,10 +157,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   unsigned char* smem = raw + (sm - shared_address(raw));
 
   if (tid == 0) {
-    barrier_init(&q_full, 4 * tiles_m);
+    barrier_init(&q_full, kTileWarps * tiles_m);
     for (int t = 0; t < 2; t++) {
       barrier_init(&s_full[t], 1);
-      barrier_init(&p_full[t], 4);
+      barrier_init(&p_full[t], kTileWarps);
     }
     barrier_init(&o_full, 1);
     for (int i = 0; i < P::kStages; i++) {
@@ -309,26 +311,37 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     }
     if (!ok) atomicExch(&failed, 1);
   } else {
-    // ---- softmax: thread = packed row
-    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    // ---- softmax: two threads a packed row, each with half of a tile's positions
+    const int t = warp / kTileWarps, half = (warp >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
+    constexpr int NH = NT / 2, DH = D / 2;  // columns of S and of O a thread takes
+    // barrier of the tile's warps; whether `good` holds for all of them
+    auto tile_sync = [&](bool good) {
+      int all;
+      asm volatile(
+          "{\n .reg .pred p, q;\n setp.ne.b32 p, %3, 0;\n bar.red.and.pred q, %1, %2, p;\n selp.b32 %0, 1, 0, q;\n}\n"
+          : "=r"(all)
+          : "r"(1 + t), "r"(kTileWarps * 32), "r"((int)good)
+          : "memory");
+      return all != 0;
+    };
     if (t < tiles_m) {
       const int64_t i = first + t * 128 + r;
       const int64_t row = i / group, head = (int64_t)h * group + i % group;
       const int slot = i < packed ? (a.slots ? a.slots[row] : (int)row) : -1;
       const bool live = slot >= 0 && slot < a.slot_count;
-      // the warp's 32 queries, each scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared
+      // 16 of the quarter's 32 queries, each scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared
       // memory: kLanes lanes take a row, 16 bytes each
-      constexpr int V = 16 / sizeof(T), kLanes = D / V, kAtOnce = 32 / kLanes, kBatch = 8;
+      constexpr int V = 16 / sizeof(T), kLanes = D / V, kAtOnce = 32 / kLanes;
+      constexpr int kSteps = 16 / kAtOnce, kBatch = kSteps < 8 ? kSteps : 8;
       const int64_t offset = live ? row * a.q_stride + head * D : -1;
       const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_stride * (int64_t)sizeof(T) & 15) == 0;
       const int d0 = lane % kLanes * V;
-      float inverse = 0.0f;
 #pragma unroll 1
-      for (int b = 0; b < kLanes; b += kBatch) {
+      for (int b = 0; b < kSteps; b += kBatch) {
         Vec<T, V> in[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
-          const int64_t at = __shfl_sync(0xffffffffu, offset, (b + k) * kAtOnce + lane / kLanes);
+          const int64_t at = __shfl_sync(0xffffffffu, offset, half * 16 + (b + k) * kAtOnce + lane / kLanes);
           const T* q = static_cast<const T*>(a.q) + at + d0;
           if (at < 0) {
             in[k] = Vec<T, V>{};
@@ -346,58 +359,63 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           for (int e = 0; e < V; e++) top = fmaxf(top, fabsf(to_f32(in[k].v[e])));
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e10 = min(max(exponent_of(top), -110), 110), r0 = (b + k) * kAtOnce, rr = r0 + lane / kLanes;
+          const int e10 = min(max(exponent_of(top), -110), 110), rr = quarter * 32 + half * 16 + (b + k) * kAtOnce + lane / kLanes;
           const float up = power2(10 - e10);
           alignas(16) uint32_t heads[V / 2], tails[V / 2];
 #pragma unroll
           for (int e = 0; e < V / 2; e++) split_f16(to_f32(in[k].v[2 * e]) * up, to_f32(in[k].v[2 * e + 1]) * up, heads[e], tails[e]);
-          unsigned char* to = smem + t * P::kQTile + (d0 >> 6) * P::kQHalf + swizzled(quarter * 32 + rr, (d0 & 63) >> 3) + (d0 & 7) * 2;
+          unsigned char* to = smem + t * P::kQTile + (d0 >> 6) * P::kQHalf + swizzled(rr, (d0 & 63) >> 3) + (d0 & 7) * 2;
           *reinterpret_cast<Vec<uint32_t, V / 2>*>(to) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(heads);
           if constexpr (SPLIT)
             *reinterpret_cast<Vec<uint32_t, V / 2>*>(to + P::kHalves * P::kQHalf) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(tails);
-          // the row's own lane keeps what undoes the scaling
-          const float back = __shfl_sync(0xffffffffu, power2(e10 - 10) * (scale * kLog2e), (lane - r0) * kLanes & 31);
-          if (lane >= r0 && lane < r0 + kAtOnce) inverse = back;
+          if (lane % kLanes == 0) row_inverse[t * 128 + rr] = power2(e10 - 10) * (scale * kLog2e);  // undoes the scaling
         }
       }
       fence_async_proxy();
       __syncwarp();
       if (lane == 0) barrier_arrive(&q_full);
+      tile_sync(true);
+      const float inverse = row_inverse[t * 128 + r];
 
       const uint32_t mine = tm + ((uint32_t)(quarter * 32) << 16);
-      const uint32_t s_at = mine + P::kS + t * NT, p_at = mine + P::kP + t * P::kPStep, o_at = mine + P::kO + t * D;
+      const uint32_t s_at = mine + P::kS + t * NT + half * NH, p_at = mine + P::kP + t * P::kPStep + half * (NH / 2),
+                     o_at = mine + P::kO + t * D + half * DH;
       float M = -INFINITY, l = 0.0f;
       bool ok = true;
       for (int k = 0; k < n; k++) {
         const int st = k % P::kStages;
         ok = __all_sync(0xffffffffu, lane != 0 || (barrier_wait(&v_full[st], (k / P::kStages) & 1) && barrier_wait(&s_full[t], k & 1)));
-        if (!ok) break;
         __syncwarp();
         tensor_fence_after();
         const float4* ks = reinterpret_cast<const float4*>(smem + P::kScales + st * NT * 8);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(ks + NT / 4);  // value scales of the tile
+        ks += half * (NH / 4);
         const float4* vs = ks + NT / 4;
-        const int valid = min(NT, end - (begin + k * NT));
+        const int valid = end - (begin + k * NT) - half * NH;
         // the row's scores, once from tensor memory, and their maximum
-        float2 x[NT / 2];
+        float2 x[NH / 2];
 #pragma unroll
-        for (int c = 0; c < NT; c += 32) tensor_load32(s_at + c, x + c / 2);
+        for (int c = 0; c < NH; c += 32) tensor_load32(s_at + c, x + c / 2);
         tensor_wait_loads();
-        if (valid < NT) hide<NT>(x, valid);
+        if (valid < NH) hide<NH>(x, valid);
         float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < NT / 2; j += 2) {
+        for (int j = 0; j < NH / 2; j += 2) {
           const float4 s4 = ks[j / 2];
           x[j] = __fmul2_rn(x[j], make_float2(s4.x, s4.y));
           x[j + 1] = __fmul2_rn(x[j + 1], make_float2(s4.z, s4.w));
           most4[j & 2] = max3(most4[j & 2], x[j].x, x[j].y);
           most4[1 + (j & 2)] = max3(most4[1 + (j & 2)], x[j + 1].x, x[j + 1].y);
         }
-        const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
-        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(vs);
+        float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
+        exchange[t][half][r] = most;
         uint32_t vtop = 0;
 #pragma unroll
         for (int c = 0; c < NT; c += 32) vtop = max(vtop, v1[c + lane] & 0x7fffffffu);
         vtop = __reduce_max_sync(0xffffffffu, vtop);
+        ok = tile_sync(ok);  // the warps of a tile go on, or stop, together
+        if (!ok) break;
+        most = fmaxf(most, exchange[t][half ^ 1][r]);
         const int ev = min(max(exponent_of(__uint_as_float(vtop)), -100), 100) - 6;
         const float reach = most * inverse + (float)ev;  // weights are below 2^(reach - M + 7)
         const bool raise = reach > M + kRaise;
@@ -408,7 +426,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           M = Mn;
           if (k > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = 0; c < DH; c += 16) {
               uint32_t y[16];
               tensor_load16(o_at + c, y);
               tensor_wait_loads();
@@ -421,7 +439,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         const float2 inverse2 = make_float2(inverse, inverse), minus = make_float2(-M, -M);
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int c = 0; c < NT; c += 32) {
+        for (int c = 0; c < NH; c += 32) {
           uint32_t heads[16], tails[16];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
@@ -451,14 +469,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       tensor_fence_after();
       const bool bad = !ok || !done || *(volatile int*)&failed != 0;
       if (bad && lane == 0) report_wait_timeout(wait_words, kWaitAttention);
+      exchange[t][half][r] = l;  // each thread's sum covers its own positions
+      tile_sync(true);
       const int64_t part = blockIdx.z * parts.per_part + row * a.heads + head;
-      if (live) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l);
-      // 32 columns at a time through shared memory (the K and V rings are free), so that rows are written
+      if (live && half == 0) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l + exchange[t][1][r]);
+      // 32 columns at a time through shared memory (the operands are done with), so that rows are written
       // 128 bytes at once
-      float* turn = reinterpret_cast<float*>(smem + P::kK) + warp * 32 * kTurnRow;
-      const int64_t to = live ? part * D : -1;
+      float* turn = reinterpret_cast<float*>(smem) + warp * 32 * kTurnRow;
+      const int64_t to = live ? part * D + half * DH : -1;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
+      for (int c = 0; c < DH; c += 32) {
         float2 x[16];
         tensor_load32(o_at + c, x);
         tensor_wait_loads();
