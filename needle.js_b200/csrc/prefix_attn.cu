@@ -431,14 +431,14 @@ StreamPlan plan_for(const needle_prefix_attention& a) {
   p.groups = (group + kGroupHeads - 1) / kGroupHeads;
   const int64_t packed = int64_t(a.rows) * group;
   if (packed >= kPrefixLeastRows && a.prefix_length >= kPrefixLeastPositions) {
-    // parts of the prefix: as many as keep the waves of CTAs short, each costing about 3 tiles on top
-    const int nt = prefix_tile(a.type);
+    // parts of the prefix: as many as keep the waves of CTAs short, each costing about 6 tiles on top
+    const int nt = prefix_tile();
     const int tiles = (a.prefix_length + nt - 1) / nt;
     const int64_t units = (packed + prefix_rows() - 1) / prefix_rows() * a.kv_heads;
     int64_t best = 0;
     int parts = 1;
     for (int c = 1; c <= std::min(tiles, 64); c++) {
-      const int64_t cost = (units * c + 147) / 148 * ((tiles + c - 1) / c + 3);
+      const int64_t cost = (units * c + 147) / 148 * ((tiles + c - 1) / c + 6);
       if (c == 1 || cost < best) {
         best = cost;
         parts = c;

@@ -22,8 +22,8 @@ struct Parts {
 };
 
 // The prefix on the tensor cores (prefix_attn_tc.cu): parts 0 .. parts - 1 of `out`, `part_len` positions each.
-// part_len is a multiple of prefix_tile(type).
-int prefix_tile(int32_t type);
+// part_len is a multiple of prefix_tile().
+int prefix_tile();
 int prefix_rows();  // packed rows (rows * heads of a KV head) a CTA takes
 cudaError_t launch_attend_prefix(const needle_prefix_attention& a, const Parts& out, int parts, int part_len, float scale,
                                  uint32_t* wait_words, cudaStream_t s);
@@ -77,6 +77,20 @@ __device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
       if (barrier_try(b, parity)) return true;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
     if (now - start > kAttendWaitNs) return false;
+  }
+}
+
+// The same for a converged warp, all lanes polling: a branch that one lane takes, and coming back from it,
+// costs a waiting warp about 200 cycles.
+__device__ __forceinline__ bool barrier_wait_warp(uint64_t* b, uint32_t parity) {
+  if (__all_sync(0xffffffffu, barrier_try(b, parity))) return true;
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+  for (;;) {
+    for (int i = 0; i < 64; i++)
+      if (__all_sync(0xffffffffu, barrier_try(b, parity))) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (__any_sync(0xffffffffu, now - start > kAttendWaitNs)) return false;
   }
 }
 

@@ -2,23 +2,23 @@
 //
 // k_attend_prefix.  With many rows the prefix is a dense product: the heads of a KV head of all rows are
 // packed into M (packed row i = row i / group, head i % group), 256 to a CTA as two tiles of 128, and
-// the CTA walks its part of the prefix in tiles of kNT positions:
+// the CTA walks its part of the prefix in tiles of 64 positions:
 //   loader warps    read int8 codes, turn them into fp16 (exact) and write K and V tiles, in the same
 //                   layout [position][64 dimensions, 128-byte swizzle], into rings in shared memory; V is
 //                   the B operand with its N dimension contiguous, so nothing is transposed
-//   MMA warp        S_t = Q_t K^T (tcgen05.mma, both from shared memory) and O_t += P_t V (P from
-//                   tensor memory), for the two tiles t in turn, so that one tile's products run while
-//                   the other's softmax does
-//   softmax warps   eight for each tile, two threads a packed row: half a tile's S into registers, maximum
-//                   (of both halves, through shared memory), exponentials, P back to tensor memory as fp16; O stays in tensor memory and is only
-//                   rescaled when a tile exceeds the reference maximum by 2^7
+//   MMA warp        S_t = Q_t K^T (tcgen05.mma, both from shared memory), two tiles of positions ahead, and
+//                   O_t += P_t V (P from tensor memory, where S was), for the two tiles t in turn
+//   softmax warps   four for each tile, one thread a packed row: 64 scores into registers, maximum,
+//                   exponentials, P back to tensor memory as fp16; O stays in tensor memory and is only
+//                   rescaled when a tile could bring weights past 2^15
+// S is double-buffered, so the softmax warps never wait for the products of their own scores: with one buffer
+// of 128 positions a tile went through softmax (3700 cycles) and products (1900) in turn, 91 us for
+// 333 rows x 32 heads x 8191 positions of 128 dimensions.
 // The reference M of a row covers the value scale too: a weight is 2^(s - M) vs <= 2^15, inside fp16, and
 // sums and outputs share the factor, which cancels.  16-bit queries are exact in fp16 after their row's
-// power of two (the score scale comes after the product), and their weights are rounded to fp16 once (2^-12 each, averaged over the positions; the
-// output's own rounding is 2^-12 or more).  Binary32 queries (kSplit) and their weights are split into fp16
-// heads and tails, two MMAs each, in tiles of 64 positions (tensor memory holds the tails).
-// What bounds it: 128 x 128 exponentials of a tile take 1024 cycles of the SM's 16 a cycle, its two
-// products at D = 128 another 1024 on the tensor pipe.
+// power of two (the score scale comes after the product), and their weights are rounded to fp16 once (2^-12
+// each, averaged over the positions; the output's own rounding is 2^-12 or more).  Binary32 queries (SPLIT)
+// and their weights are split into fp16 heads and tails, two MMAs each.
 // Every wait is bounded (2 s): a wait that runs out is reported through the wait-status words, and the
 // rows' parts become NaN.
 #include "prefix_attn.cuh"
@@ -27,34 +27,32 @@ namespace needle {
 
 namespace {
 
-constexpr int kPrefixSoftmaxWarps = 16, kPrefixLoaderWarps = 3;
-constexpr int kTileWarps = kPrefixSoftmaxWarps / 2;  // softmax warps of a tile: two for each 32 rows
+constexpr int kTileWarps = 4;  // softmax warps of a tile
+constexpr int kPrefixSoftmaxWarps = 2 * kTileWarps, kPrefixLoaderWarps = 3;
 constexpr int kPrefixMmaWarp = kPrefixSoftmaxWarps + kPrefixLoaderWarps;
 constexpr int kPrefixThreads = (kPrefixMmaWarp + 1) * 32;
 constexpr int kPrefixRows = 256;  // packed rows of a CTA
+constexpr int kNT = 64;           // positions of a tile
 constexpr int kTurnRow = 36;      // floats of a row in the epilogue's transposition
 
 template <int D, bool SPLIT>
 struct PrefixShape {
-  static constexpr int kNT = SPLIT ? 64 : 128;       // positions of a tile
   static constexpr int kHalves = D / 64;
   static constexpr int kParts = SPLIT ? 2 : 1;       // fp16 parts of a query or weight
-  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kStages = D == 128 && SPLIT ? 3 : 4;  // of K and V tiles: two ahead in scores, one in values
   static constexpr uint32_t kQHalf = 128 * 128;                       // bytes of 128 rows x 64 dimensions
   static constexpr uint32_t kQTile = kQHalf * kHalves * kParts;       // [part][half]
   static constexpr uint32_t kKvHalf = kNT * 128;
   static constexpr uint32_t kKvTile = kKvHalf * kHalves;
   static constexpr uint32_t kK = 2 * kQTile, kV = kK + kStages * kKvTile;
-  static constexpr uint32_t kScales = kV + kStages * kKvTile;         // per stage: kNT key, kNT value scales
+  static constexpr uint32_t kScales = kV + kStages * kKvTile;
+  static constexpr uint32_t kScaleStage = kNT * 8 + 16;  // key scales, value scales, the largest value scales
   static_assert(kScales >= kPrefixSoftmaxWarps * 32 * kTurnRow * 4, "the epilogue takes the operands' place");
-  static constexpr uint32_t kSmem = kScales + kStages * kNT * 8 + 1024;
-  // tensor memory columns
-  static constexpr uint32_t kS = 0;                                    // two tiles of kNT
-  static constexpr bool kOverlay = D == 128 && !SPLIT;                 // P takes the place of S
-  static constexpr uint32_t kP = kOverlay ? 0 : (SPLIT ? 128 : 384);
-  static constexpr uint32_t kPStep = kOverlay ? kNT : 64;              // from one tile's P to the other's
-  static constexpr uint32_t kO = 256;
+  static constexpr uint32_t kSmem = kScales + kStages * kScaleStage + 1024;
 };
+// Tensor memory columns: S of tile t, buffer b, and P in its place (heads, then tails); O of tile t.
+__device__ __forceinline__ uint32_t s_column(int t, int b) { return t * 128 + b * kNT; }
+__device__ __forceinline__ uint32_t o_column(int t, int d) { return 256 + t * d; }
 
 // Byte offset of 16-byte unit `unit` (0..7) of row `row` in a [rows][64 x fp16] tile, 128-byte swizzle.
 __device__ __forceinline__ uint32_t swizzled(int row, int unit) {
@@ -70,24 +68,31 @@ __device__ __forceinline__ uint64_t descriptor(uint32_t address, uint32_t block)
 __device__ __forceinline__ uint32_t instruction(int n, bool b_n) {
   return (1u << 4) | (b_n ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// The whole (converged) warp calls these and one lane, the leader, issues: the descriptors stay in uniform
+// registers.  Issued from a branch that one lane takes, an MMA cost about 110 cycles, twice what it runs for.
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
+                                           uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
+                                           uint32_t leader) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(leader)
       : "memory");
 }
-// Arrives on `b` once every MMA this thread has issued is complete.
-__device__ __forceinline__ void mma_commit_to(uint64_t* b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(b))
-               : "memory");
+// Arrives on `b` once every MMA the leader has issued is complete.
+__device__ __forceinline__ void mma_commit_to(uint64_t* b, uint32_t leader) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(shared_address(b)),
+      "r"(leader)
+      : "memory");
 }
 
 // 32 (16) consecutive columns of this thread's lane of tensor memory.
@@ -140,34 +145,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     k_attend_prefix(const __grid_constant__ needle_prefix_attention a, const Parts parts, int part_len, float scale,
                     uint32_t* wait_words) {
   using P = PrefixShape<D, SPLIT>;
-  constexpr int NT = P::kNT;
   extern __shared__ __align__(16) unsigned char raw[];
-  __shared__ __align__(8) uint64_t q_full, s_full[2], p_full[2], o_full;
-  __shared__ __align__(8) uint64_t k_full[P::kStages], k_empty[P::kStages], v_full[P::kStages], v_empty[P::kStages];
+  __shared__ __align__(8) uint64_t q_full, s_full[2][2], p_full[2][2], rest[2], o_full;
+  __shared__ __align__(8) uint64_t full[P::kStages], empty[P::kStages];
   __shared__ uint32_t tensor_base;
   __shared__ int failed;
-  __shared__ float row_inverse[kPrefixRows], exchange[2][2][128];  // [tile][column half][row]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int h = blockIdx.y, group = a.heads / a.kv_heads;
   const int64_t packed = (int64_t)a.rows * group, first = (int64_t)blockIdx.x * kPrefixRows;
   const int tiles_m = packed - first > 128 ? 2 : 1;
   const int begin = blockIdx.z * part_len, end = min(begin + part_len, a.prefix_length);
-  const int n = (end - begin + NT - 1) / NT;
+  const int n = (end - begin + kNT - 1) / kNT;
   const uint32_t sm = (shared_address(raw) + 1023u) & ~1023u;
   unsigned char* smem = raw + (sm - shared_address(raw));
 
   if (tid == 0) {
     barrier_init(&q_full, kTileWarps * tiles_m);
     for (int t = 0; t < 2; t++) {
-      barrier_init(&s_full[t], 1);
-      barrier_init(&p_full[t], kTileWarps);
+      for (int b = 0; b < 2; b++) {
+        barrier_init(&s_full[t][b], 1);
+        barrier_init(&p_full[t][b], kTileWarps);
+      }
+      barrier_init(&rest[t], 1);
     }
     barrier_init(&o_full, 1);
     for (int i = 0; i < P::kStages; i++) {
-      barrier_init(&k_full[i], kPrefixLoaderWarps);
-      barrier_init(&v_full[i], kPrefixLoaderWarps);
-      barrier_init(&k_empty[i], 1);
-      barrier_init(&v_empty[i], 1);
+      barrier_init(&full[i], kPrefixLoaderWarps);
+      barrier_init(&empty[i], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
@@ -181,167 +185,147 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   tensor_fence_before();
   __syncthreads();
   tensor_fence_after();
-  const uint32_t tm = tensor_base;
+  const uint32_t tm = __shfl_sync(0xffffffffu, tensor_base, 0);
 
   if (warp == kPrefixMmaWarp) {
-    const uint32_t qk = instruction(NT, false), pv = instruction(D, true);
+    const uint32_t qk = instruction(kNT, false), pv = instruction(D, true), leader = lane == 0;
     bool ok = true;
-    auto wait = [&](uint64_t* b, uint32_t parity) {  // one lane polls, the warp stays together
-      ok = ok && __all_sync(0xffffffffu, lane != 0 || barrier_wait(b, parity));
-      __syncwarp();
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+      ok = ok && barrier_wait_warp(b, parity);
+      tensor_fence_after();
     };
     auto scores = [&](int t, int i) {  // S_t = Q_t K_i^T
-      const uint32_t q = sm + t * P::kQTile, k = sm + P::kK + (i % P::kStages) * P::kKvTile;
+      const uint64_t q = descriptor(sm + t * P::kQTile, 16), k = descriptor(sm + P::kK + (i % P::kStages) * P::kKvTile, 16);
 #pragma unroll
       for (int part = 0; part < P::kParts; part++)
 #pragma unroll
         for (int half = 0; half < P::kHalves; half++)
 #pragma unroll
           for (int s = 0; s < 4; s++)
-            mma_shared(tm + P::kS + t * NT, descriptor(q + (part * P::kHalves + half) * P::kQHalf + s * 32, 16),
-                       descriptor(k + half * P::kKvHalf + s * 32, 16), qk, part + half + s > 0);
-      mma_commit_to(&s_full[t]);
+            mma_shared(tm + s_column(t, i & 1), q + (((part * P::kHalves + half) * P::kQHalf + s * 32) >> 4),
+                       k + ((half * P::kKvHalf + s * 32) >> 4), qk, part + half + s > 0, leader);
+      mma_commit_to(&s_full[t][i & 1], leader);
     };
     auto values = [&](int t, int i) {  // O_t += P_t V_i
-      const uint32_t v = sm + P::kV + (i % P::kStages) * P::kKvTile;
+      const uint64_t v = descriptor(sm + P::kV + (i % P::kStages) * P::kKvTile, P::kKvHalf);
 #pragma unroll
       for (int part = 0; part < P::kParts; part++)
 #pragma unroll
-        for (int s = 0; s < NT / 16; s++)
-          mma_tensor(tm + P::kO + t * D, tm + P::kP + t * P::kPStep + part * (NT / 2) + s * 8,
-                     descriptor(v + s * 2048, P::kKvHalf), pv, i > 0 || part + s > 0);
+        for (int s = 0; s < kNT / 16; s++)
+          mma_tensor(tm + o_column(t, D), tm + s_column(t, i & 1) + part * (kNT / 2) + s * 8, v + ((s * 2048) >> 4), pv,
+                     i > 0 || part + s > 0, leader);
     };
     wait(&q_full, 0);
-    wait(&k_full[0], 0);
-    if (ok && lane == 0) {
-      tensor_fence_after();
-      for (int t = 0; t < tiles_m; t++) scores(t, 0);
-      mma_commit_to(&k_empty[0]);
+    for (int i = 0; i < min(n, 2) && ok; i++) {
+      wait(&full[i], 0);
+      if (!ok) break;
+      for (int t = 0; t < tiles_m; t++) scores(t, i);
     }
-    __syncwarp();
     for (int i = 0; i < n && ok; i++) {
-      for (int t = 0; t < tiles_m && ok; t++) {
-        if (t == 0) wait(&v_full[i % P::kStages], (i / P::kStages) & 1);
-        wait(&p_full[t], i & 1);
-        if (ok && lane == 0) {
-          tensor_fence_after();
-          values(t, i);
-          if (t == tiles_m - 1) mma_commit_to(&v_empty[i % P::kStages]);
-        }
-        __syncwarp();
-        if (i + 1 < n) {
-          const int st = (i + 1) % P::kStages;
-          if (t == 0) wait(&k_full[st], ((i + 1) / P::kStages) & 1);
-          if (ok && lane == 0) {
-            tensor_fence_after();
-            scores(t, i + 1);
-            if (t == tiles_m - 1) mma_commit_to(&k_empty[st]);
-          }
-          __syncwarp();
-        }
+      const bool more = i + 2 < n;
+      if (more) wait(&full[(i + 2) % P::kStages], ((i + 2) / P::kStages) & 1);
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        if (t >= tiles_m) break;
+        wait(&p_full[t][i & 1], (i >> 1) & 1);
+        if (!ok) break;
+        values(t, i);
+        if (t == tiles_m - 1) mma_commit_to(&empty[i % P::kStages], leader);
+        if (i == n - 2) mma_commit_to(&rest[t], leader);
+        if (more) scores(t, i + 2);  // behind P_t V_i in the tensor pipe, which reads P from where S goes
       }
     }
-    if (lane == 0) {
-      if (!ok) atomicExch(&failed, 1);
-      mma_commit_to(&o_full);
-    }
+    if (leader && !ok) atomicExch(&failed, 1);
     __syncwarp();
+    mma_commit_to(&o_full, leader);
   } else if (warp >= kPrefixSoftmaxWarps) {
-    // ---- loaders: K and V tiles in turn, the next tile's codes in registers while this one is written
-    constexpr int kLoaders = kPrefixLoaderWarps * 32, kRowUnits = D / 16, kAll = NT * kRowUnits;
-    constexpr int kUnits = (kAll + kLoaders - 1) / kLoaders;  // 16-code units of a thread
-    constexpr int kScalesEach = (NT + kLoaders - 1) / kLoaders;
+    // ---- loaders: K and V tiles in turn, the next two tiles' codes in registers while one is written.  Eight
+    // neighbouring threads write two rows of one 64-dimension half: every bank once.
+    constexpr int kLoaders = kPrefixLoaderWarps * 32, kRowUnits = D / 16;  // 16-code units of a row
+    constexpr int kStep = kLoaders / kRowUnits;                            // rows that all loaders take at once
+    constexpr int kUnits = (kNT + kStep - 1) / kStep;
     const int lt = tid - kPrefixSoftmaxWarps * 32;
-    const int64_t base = (int64_t)h * a.prefix_capacity;
-    uint4 code[kUnits];
-    float key_scale[kScalesEach], value_scale[kScalesEach];
-    auto fetch = [&](int item) {  // item 2 i: K of tile i, 2 i + 1: V
-      const int8_t* src = (item & 1) ? a.prefix_value_codes : a.prefix_key_codes;
-      const int j = begin + (item >> 1) * NT;
+    const int half = D == 128 ? (lt >> 3) & 1 : 0, cc = lt & 3;
+    const int row0 = D == 128 ? (lt >> 4) * 2 + ((lt >> 2) & 1) : lt >> 2;
+    const uint32_t at = half * P::kKvHalf + swizzled(row0, 2 * cc);
+    const int64_t base = (int64_t)h * a.prefix_capacity + begin;
+    const int64_t code_at = (base + row0) * D + half * 64 + cc * 16;
+    uint4 codes[2][kUnits];  // of K, of V
+    float key_scale = 1.0f, value_scale = 0.0f;
+    auto fetch = [&](int i, bool value) {
+      if (i >= n) return;
+      uint4(&code)[kUnits] = codes[value];
+      const int j = i * kNT, left = end - begin - j;
+      const int8_t* src = (value ? a.prefix_value_codes : a.prefix_key_codes) + code_at + (int64_t)j * D;
 #pragma unroll
-      for (int u = 0; u < kUnits; u++) {
-        const int unit = u * kLoaders + lt, p = j + unit / kRowUnits;
-        code[u] = unit < kAll && p < end ? __ldg(reinterpret_cast<const uint4*>(src + (base + p) * D) + unit % kRowUnits) : make_uint4(0, 0, 0, 0);
-      }
-      if (item & 1) {
-#pragma unroll
-        for (int u = 0; u < kScalesEach; u++) {
-          const int p = j + u * kLoaders + lt;
-          key_scale[u] = p < end ? __ldg(a.prefix_key_scales + base + p) : 1.0f;  // -inf stays -inf
-          value_scale[u] = p < end ? __ldg(a.prefix_value_scales + base + p) : 0.0f;
-        }
+      for (int u = 0; u < kUnits; u++)
+        code[u] = row0 + u * kStep < min(left, kNT) ? __ldg(reinterpret_cast<const uint4*>(src + u * kStep * D)) : make_uint4(0, 0, 0, 0);
+      if (value && lt < kNT) {
+        key_scale = lt < left ? __ldg(a.prefix_key_scales + base + j + lt) : 1.0f;  // -inf stays -inf
+        value_scale = lt < left ? __ldg(a.prefix_value_scales + base + j + lt) : 0.0f;
       }
     };
-    bool ok = true;
-    fetch(0);
-    for (int item = 0; item < 2 * n; item++) {
-      const int i = item >> 1, st = i % P::kStages;
-      const bool value = item & 1;
-      if (i >= P::kStages) {
-        ok = __all_sync(0xffffffffu, lane != 0 || barrier_wait(value ? &v_empty[st] : &k_empty[st], (i / P::kStages - 1) & 1));
-        if (!ok) break;
-      }
+    auto write = [&](int i, bool value) {
+      const uint4(&code)[kUnits] = codes[value];
+      const int st = i % P::kStages;
       unsigned char* to = smem + (value ? P::kV : P::kK) + st * P::kKvTile;
 #pragma unroll
       for (int u = 0; u < kUnits; u++) {
-        const int unit = u * kLoaders + lt, row = unit / kRowUnits, cc = unit % kRowUnits;
-        if (unit >= kAll) break;
+        if (row0 + u * kStep >= kNT) break;
         const uint32_t w[4] = {code[u].x ^ 0x80808080u, code[u].y ^ 0x80808080u, code[u].z ^ 0x80808080u, code[u].w ^ 0x80808080u};
-        const uint4 lo = make_uint4(codes_f16(w[0], 0x4140), codes_f16(w[0], 0x4342), codes_f16(w[1], 0x4140), codes_f16(w[1], 0x4342));
-        const uint4 hi = make_uint4(codes_f16(w[2], 0x4140), codes_f16(w[2], 0x4342), codes_f16(w[3], 0x4140), codes_f16(w[3], 0x4342));
-        unsigned char* tile = to + (cc >> 2) * P::kKvHalf;
-        // the two 64-dimension halves of a row share banks: they write their two units in opposite order
-        const int flip = (cc >> 2) & 1, at = (cc & 3) * 2;
-        *reinterpret_cast<uint4*>(tile + swizzled(row, at + flip)) = flip ? hi : lo;
-        *reinterpret_cast<uint4*>(tile + swizzled(row, at + 1 - flip)) = flip ? lo : hi;
+        // kStep is 12 or 24: four rows on, bit 2 of the swizzle flips
+        const uint32_t o = (at ^ ((u * kStep & 4) << 4)) + u * kStep * 128;
+        *reinterpret_cast<uint4*>(to + o) =
+            make_uint4(codes_f16(w[0], 0x4140), codes_f16(w[0], 0x4342), codes_f16(w[1], 0x4140), codes_f16(w[1], 0x4342));
+        *reinterpret_cast<uint4*>(to + (o ^ 16)) =
+            make_uint4(codes_f16(w[2], 0x4140), codes_f16(w[2], 0x4342), codes_f16(w[3], 0x4140), codes_f16(w[3], 0x4342));
       }
-      if (value) {
-        float* s = reinterpret_cast<float*>(smem + P::kScales + st * NT * 8);
-#pragma unroll
-        for (int u = 0; u < kScalesEach; u++)
-          if (u * kLoaders + lt < NT) {
-            s[u * kLoaders + lt] = key_scale[u];
-            s[NT + u * kLoaders + lt] = value_scale[u];
-          }
+      if (value && lt < kNT) {
+        float* s = reinterpret_cast<float*>(smem + P::kScales + st * P::kScaleStage);
+        s[lt] = key_scale;
+        s[kNT + lt] = value_scale;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(value_scale) & 0x7fffffffu);
+        if (lane == 0) s[2 * kNT + (lt >> 5)] = __uint_as_float(top);
       }
-      if (item + 1 < 2 * n) fetch(item + 1);
-      fence_async_proxy();
+    };
+    bool ok = true;
+    fetch(0, false);
+    fetch(0, true);
+#pragma unroll 1
+    for (int i = 0; i < n; i++) {
+      const int st = i % P::kStages;
+      ok = i < P::kStages || barrier_wait_warp(&empty[st], (i / P::kStages - 1) & 1);
+      if (!ok) break;
+      write(i, false);
+      write(i, true);
+      fence_async_proxy();  // before the next loads: it waits for every access in flight
       __syncwarp();
-      if (lane == 0) barrier_arrive(value ? &v_full[st] : &k_full[st]);
+      if (lane == 0) barrier_arrive(&full[st]);
+      fetch(i + 1, false);
+      fetch(i + 1, true);
     }
     if (!ok) atomicExch(&failed, 1);
   } else {
-    // ---- softmax: two threads a packed row, each with half of a tile's positions
-    const int t = warp / kTileWarps, half = (warp >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
-    constexpr int NH = NT / 2, DH = D / 2;  // columns of S and of O a thread takes
-    // barrier of the tile's warps; whether `good` holds for all of them
-    auto tile_sync = [&](bool good) {
-      int all;
-      asm volatile(
-          "{\n .reg .pred p, q;\n setp.ne.b32 p, %3, 0;\n bar.red.and.pred q, %1, %2, p;\n selp.b32 %0, 1, 0, q;\n}\n"
-          : "=r"(all)
-          : "r"(1 + t), "r"(kTileWarps * 32), "r"((int)good)
-          : "memory");
-      return all != 0;
-    };
+    // ---- softmax: thread = packed row
+    const int t = warp / kTileWarps, quarter = warp & 3, r = quarter * 32 + lane;
     if (t < tiles_m) {
       const int64_t i = first + t * 128 + r;
       const int64_t row = i / group, head = (int64_t)h * group + i % group;
       const int slot = i < packed ? (a.slots ? a.slots[row] : (int)row) : -1;
       const bool live = slot >= 0 && slot < a.slot_count;
-      // 16 of the quarter's 32 queries, each scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared
+      // the warp's 32 queries, each scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared
       // memory: kLanes lanes take a row, 16 bytes each
-      constexpr int V = 16 / sizeof(T), kLanes = D / V, kAtOnce = 32 / kLanes;
-      constexpr int kSteps = 16 / kAtOnce, kBatch = kSteps < 8 ? kSteps : 8;
+      constexpr int V = 16 / sizeof(T), kLanes = D / V, kAtOnce = 32 / kLanes, kBatch = 8;
       const int64_t offset = live ? row * a.q_stride + head * D : -1;
       const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_stride * (int64_t)sizeof(T) & 15) == 0;
       const int d0 = lane % kLanes * V;
+      float inverse = 0.0f;
 #pragma unroll 1
-      for (int b = 0; b < kSteps; b += kBatch) {
+      for (int b = 0; b < kLanes; b += kBatch) {
         Vec<T, V> in[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
-          const int64_t at = __shfl_sync(0xffffffffu, offset, half * 16 + (b + k) * kAtOnce + lane / kLanes);
+          const int64_t at = __shfl_sync(0xffffffffu, offset, (b + k) * kAtOnce + lane / kLanes);
           const T* q = static_cast<const T*>(a.q) + at + d0;
           if (at < 0) {
             in[k] = Vec<T, V>{};
@@ -359,64 +343,55 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           for (int e = 0; e < V; e++) top = fmaxf(top, fabsf(to_f32(in[k].v[e])));
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e10 = min(max(exponent_of(top), -110), 110), rr = quarter * 32 + half * 16 + (b + k) * kAtOnce + lane / kLanes;
+          const int e10 = min(max(exponent_of(top), -110), 110), r0 = (b + k) * kAtOnce, rr = r0 + lane / kLanes;
           const float up = power2(10 - e10);
           alignas(16) uint32_t heads[V / 2], tails[V / 2];
 #pragma unroll
           for (int e = 0; e < V / 2; e++) split_f16(to_f32(in[k].v[2 * e]) * up, to_f32(in[k].v[2 * e + 1]) * up, heads[e], tails[e]);
-          unsigned char* to = smem + t * P::kQTile + (d0 >> 6) * P::kQHalf + swizzled(rr, (d0 & 63) >> 3) + (d0 & 7) * 2;
+          unsigned char* to = smem + t * P::kQTile + (d0 >> 6) * P::kQHalf + swizzled(quarter * 32 + rr, (d0 & 63) >> 3) + (d0 & 7) * 2;
           *reinterpret_cast<Vec<uint32_t, V / 2>*>(to) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(heads);
           if constexpr (SPLIT)
             *reinterpret_cast<Vec<uint32_t, V / 2>*>(to + P::kHalves * P::kQHalf) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(tails);
-          if (lane % kLanes == 0) row_inverse[t * 128 + rr] = power2(e10 - 10) * (scale * kLog2e);  // undoes the scaling
+          // the row's own lane keeps what undoes the scaling
+          const float back = __shfl_sync(0xffffffffu, power2(e10 - 10) * (scale * kLog2e), (lane - r0) * kLanes & 31);
+          if (lane >= r0 && lane < r0 + kAtOnce) inverse = back;
         }
       }
       fence_async_proxy();
       __syncwarp();
       if (lane == 0) barrier_arrive(&q_full);
-      tile_sync(true);
-      const float inverse = row_inverse[t * 128 + r];
 
-      const uint32_t mine = tm + ((uint32_t)(quarter * 32) << 16);
-      const uint32_t s_at = mine + P::kS + t * NT + half * NH, p_at = mine + P::kP + t * P::kPStep + half * (NH / 2),
-                     o_at = mine + P::kO + t * D + half * DH;
+      const uint32_t mine = tm + ((uint32_t)(quarter * 32) << 16), o_at = mine + o_column(t, D);
       float M = -INFINITY, l = 0.0f;
       bool ok = true;
+#pragma unroll 1
       for (int k = 0; k < n; k++) {
         const int st = k % P::kStages;
-        ok = __all_sync(0xffffffffu, lane != 0 || (barrier_wait(&v_full[st], (k / P::kStages) & 1) && barrier_wait(&s_full[t], k & 1)));
-        __syncwarp();
+        const uint32_t s_at = mine + s_column(t, k & 1);
+        ok = barrier_wait_warp(&full[st], (k / P::kStages) & 1) && barrier_wait_warp(&s_full[t][k & 1], (k >> 1) & 1);
+        if (!ok) break;
         tensor_fence_after();
-        const float4* ks = reinterpret_cast<const float4*>(smem + P::kScales + st * NT * 8);
-        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(ks + NT / 4);  // value scales of the tile
-        ks += half * (NH / 4);
-        const float4* vs = ks + NT / 4;
-        const int valid = end - (begin + k * NT) - half * NH;
+        const float4* ks = reinterpret_cast<const float4*>(smem + P::kScales + st * P::kScaleStage);
+        const float4* vs = ks + kNT / 4;
+        const float2 vtop = *reinterpret_cast<const float2*>(vs + kNT / 4);
+        const int valid = end - (begin + k * kNT);
         // the row's scores, once from tensor memory, and their maximum
-        float2 x[NH / 2];
+        float2 x[kNT / 2];
 #pragma unroll
-        for (int c = 0; c < NH; c += 32) tensor_load32(s_at + c, x + c / 2);
+        for (int c = 0; c < kNT; c += 32) tensor_load32(s_at + c, x + c / 2);
         tensor_wait_loads();
-        if (valid < NH) hide<NH>(x, valid);
+        if (valid < kNT) hide<kNT>(x, valid);
         float most4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < NH / 2; j += 2) {
+        for (int j = 0; j < kNT / 2; j += 2) {
           const float4 s4 = ks[j / 2];
           x[j] = __fmul2_rn(x[j], make_float2(s4.x, s4.y));
           x[j + 1] = __fmul2_rn(x[j + 1], make_float2(s4.z, s4.w));
           most4[j & 2] = max3(most4[j & 2], x[j].x, x[j].y);
           most4[1 + (j & 2)] = max3(most4[1 + (j & 2)], x[j + 1].x, x[j + 1].y);
         }
-        float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
-        exchange[t][half][r] = most;
-        uint32_t vtop = 0;
-#pragma unroll
-        for (int c = 0; c < NT; c += 32) vtop = max(vtop, v1[c + lane] & 0x7fffffffu);
-        vtop = __reduce_max_sync(0xffffffffu, vtop);
-        ok = tile_sync(ok);  // the warps of a tile go on, or stop, together
-        if (!ok) break;
-        most = fmaxf(most, exchange[t][half ^ 1][r]);
-        const int ev = min(max(exponent_of(__uint_as_float(vtop)), -100), 100) - 6;
+        const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
+        const int ev = min(max(exponent_of(fmaxf(vtop.x, vtop.y)), -100), 100) - 6;
         const float reach = most * inverse + (float)ev;  // weights are below 2^(reach - M + 7)
         const bool raise = reach > M + kRaise;
         if (__any_sync(0xffffffffu, raise)) {
@@ -425,8 +400,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           l *= f;
           M = Mn;
           if (k > 0) {
+            // O must be at rest: this tile's products have not begun, and those of the tile before are done when
+            // the next tile's scores, issued behind them, are there
+            ok = k + 1 < n ? barrier_wait_warp(&s_full[t][(k + 1) & 1], ((k + 1) >> 1) & 1) : barrier_wait_warp(&rest[t], 0);
+            if (!ok) break;
+            tensor_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < DH; c += 16) {
+            for (int c = 0; c < D; c += 16) {
               uint32_t y[16];
               tensor_load16(o_at + c, y);
               tensor_wait_loads();
@@ -439,7 +419,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         const float2 inverse2 = make_float2(inverse, inverse), minus = make_float2(-M, -M);
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int c = 0; c < NH; c += 32) {
+        for (int c = 0; c < kNT; c += 32) {
           uint32_t heads[16], tails[16];
 #pragma unroll
           for (int j = 0; j < 16; j += 2) {
@@ -455,30 +435,28 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
               else heads[j + o] = half2_bits(__floats2half2_rn(w.x, w.y));
             }
           }
-          tensor_store16(p_at + c / 2, heads);
-          if constexpr (SPLIT) tensor_store16(p_at + NT / 2 + c / 2, tails);
+          tensor_store16(s_at + c / 2, heads);
+          if constexpr (SPLIT) tensor_store16(s_at + kNT / 2 + c / 2, tails);
         }
         l += sum.x + sum.y;
         tensor_wait_stores();
         tensor_fence_before();
         __syncwarp();
-        if (lane == 0) barrier_arrive(&p_full[t]);
+        if (lane == 0) barrier_arrive(&p_full[t][k & 1]);
       }
       if (!ok) atomicExch(&failed, 1);
-      const bool done = __all_sync(0xffffffffu, lane != 0 || barrier_wait(&o_full, 0));
+      const bool done = barrier_wait_warp(&o_full, 0);
       tensor_fence_after();
       const bool bad = !ok || !done || *(volatile int*)&failed != 0;
       if (bad && lane == 0) report_wait_timeout(wait_words, kWaitAttention);
-      exchange[t][half][r] = l;  // each thread's sum covers its own positions
-      tile_sync(true);
       const int64_t part = blockIdx.z * parts.per_part + row * a.heads + head;
-      if (live && half == 0) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l + exchange[t][1][r]);
+      if (live) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l);
       // 32 columns at a time through shared memory (the operands are done with), so that rows are written
       // 128 bytes at once
       float* turn = reinterpret_cast<float*>(smem) + warp * 32 * kTurnRow;
-      const int64_t to = live ? part * D + half * DH : -1;
+      const int64_t to = live ? part * D : -1;
 #pragma unroll 1
-      for (int c = 0; c < DH; c += 32) {
+      for (int c = 0; c < D; c += 32) {
         float2 x[16];
         tensor_load32(o_at + c, x);
         tensor_wait_loads();
@@ -507,7 +485,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 
 }  // namespace
 
-int prefix_tile(int32_t type) { return type == NEEDLE_TYPE_F32 ? PrefixShape<64, true>::kNT : PrefixShape<64, false>::kNT; }
+int prefix_tile() { return kNT; }
 int prefix_rows() { return kPrefixRows; }
 
 cudaError_t launch_attend_prefix(const needle_prefix_attention& a, const Parts& out, int parts, int part_len, float scale,
