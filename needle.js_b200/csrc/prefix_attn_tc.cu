@@ -68,31 +68,31 @@ __device__ __forceinline__ uint64_t descriptor(uint32_t address, uint32_t block)
 __device__ __forceinline__ uint32_t instruction(int n, bool b_n) {
   return (1u << 4) | (b_n ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// The whole (converged) warp calls these and one lane, the leader, issues: the descriptors stay in uniform
-// registers.  Issued from a branch that one lane takes, an MMA cost about 110 cycles, twice what it runs for.
-__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
-                                           uint32_t leader) {
+// True in one lane of the converged warp.  A whole group of MMAs is issued inside one such branch: per MMA of
+// 128 x 64 x 16 that measured 57 cycles, a predicate of each MMA's own (lane == 0) 105.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e != 0;
+}
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(leader)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
-                                           uint32_t leader) {
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %6, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(leader)
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrives on `b` once every MMA the leader has issued is complete.
-__device__ __forceinline__ void mma_commit_to(uint64_t* b, uint32_t leader) {
-  asm volatile(
-      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
-      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(shared_address(b)),
-      "r"(leader)
-      : "memory");
+// Arrives on `b` once every MMA this lane has issued is complete.
+__device__ __forceinline__ void mma_commit_to(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(b))
+               : "memory");
 }
 
 // 32 (16) consecutive columns of this thread's lane of tensor memory.
@@ -185,10 +185,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   tensor_fence_before();
   __syncthreads();
   tensor_fence_after();
-  const uint32_t tm = __shfl_sync(0xffffffffu, tensor_base, 0);
+  // All 512 columns are this CTA's, so they begin at address 0; as a constant it leaves the MMAs' operands in
+  // uniform registers.
+  constexpr uint32_t tm = 0;
+  if (tensor_base != tm && tid == 0) failed = 1;
 
   if (warp == kPrefixMmaWarp) {
-    const uint32_t qk = instruction(kNT, false), pv = instruction(D, true), leader = lane == 0;
+    const uint32_t qk = instruction(kNT, false), pv = instruction(D, true);
     bool ok = true;
     auto wait = [&](uint64_t* b, uint32_t parity) {
       ok = ok && barrier_wait_warp(b, parity);
@@ -203,8 +206,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 #pragma unroll
           for (int s = 0; s < 4; s++)
             mma_shared(tm + s_column(t, i & 1), q + (((part * P::kHalves + half) * P::kQHalf + s * 32) >> 4),
-                       k + ((half * P::kKvHalf + s * 32) >> 4), qk, part + half + s > 0, leader);
-      mma_commit_to(&s_full[t][i & 1], leader);
+                       k + ((half * P::kKvHalf + s * 32) >> 4), qk, part + half + s > 0);
+      mma_commit_to(&s_full[t][i & 1]);
     };
     auto values = [&](int t, int i) {  // O_t += P_t V_i
       const uint64_t v = descriptor(sm + P::kV + (i % P::kStages) * P::kKvTile, P::kKvHalf);
@@ -213,13 +216,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 #pragma unroll
         for (int s = 0; s < kNT / 16; s++)
           mma_tensor(tm + o_column(t, D), tm + s_column(t, i & 1) + part * (kNT / 2) + s * 8, v + ((s * 2048) >> 4), pv,
-                     i > 0 || part + s > 0, leader);
+                     i > 0 || part + s > 0);
     };
     wait(&q_full, 0);
     for (int i = 0; i < min(n, 2) && ok; i++) {
       wait(&full[i], 0);
       if (!ok) break;
-      for (int t = 0; t < tiles_m; t++) scores(t, i);
+      if (elect_one())
+        for (int t = 0; t < tiles_m; t++) scores(t, i);
+      __syncwarp();
     }
     for (int i = 0; i < n && ok; i++) {
       const bool more = i + 2 < n;
@@ -229,15 +234,20 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (t >= tiles_m) break;
         wait(&p_full[t][i & 1], (i >> 1) & 1);
         if (!ok) break;
-        values(t, i);
-        if (t == tiles_m - 1) mma_commit_to(&empty[i % P::kStages], leader);
-        if (i == n - 2) mma_commit_to(&rest[t], leader);
-        if (more) scores(t, i + 2);  // behind P_t V_i in the tensor pipe, which reads P from where S goes
+        if (elect_one()) {
+          values(t, i);
+          if (t == tiles_m - 1) mma_commit_to(&empty[i % P::kStages]);
+          if (i == n - 2) mma_commit_to(&rest[t]);
+          if (more) scores(t, i + 2);  // behind P_t V_i in the tensor pipe, which reads P from where S goes
+        }
+        __syncwarp();
       }
     }
-    if (leader && !ok) atomicExch(&failed, 1);
+    if (elect_one()) {
+      if (!ok) atomicExch(&failed, 1);
+      mma_commit_to(&o_full);
+    }
     __syncwarp();
-    mma_commit_to(&o_full, leader);
   } else if (warp >= kPrefixSoftmaxWarps) {
     // ---- loaders: K and V tiles in turn, the next two tiles' codes in registers while one is written.  Eight
     // neighbouring threads write two rows of one 64-dimension half: every bank once.
@@ -479,7 +489,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   __syncthreads();
   if (warp == kPrefixMmaWarp) {
     tensor_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tensor_base), "r"(512u) : "memory");
   }
 }
 
