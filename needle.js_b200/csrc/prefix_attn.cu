@@ -30,7 +30,7 @@ namespace {
 
 constexpr int kStreamWarps = 8;
 constexpr int kStreamThreads = kStreamWarps * 32;
-constexpr int kStreamStages = 3;
+constexpr int kStreamStages = 2;
 constexpr int kGroupHeads = 8;  // query heads of one KV head taken together
 constexpr int kBlock = 32;      // positions of a step
 
@@ -230,7 +230,7 @@ __device__ __forceinline__ void store_out(T* p, const float* x, bool vec) {
 }
 
 template <class T, int D>
-__global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
+__global__ void __maxnreg__(D == 64 ? 80 : 152)
     k_attend_stream(const __grid_constant__ needle_prefix_attention a, const StreamPlan plan, const Parts parts, float scale,
                     uint32_t* wait_words) {
   constexpr int N = D / 4;  // output dimensions of a lane
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
   const int row = (int)(blockIdx.x / of_row), rest = (int)(blockIdx.x - row * of_row);
   const int h = rest / plan.groups, g0 = (rest - h * plan.groups) * kGroupHeads;
   const int heads = min(kGroupHeads, group - g0);
-  const int slot = a.slots ? a.slots[row] : row;
+  const int slot = a.slots ? __ldg(a.slots + row) : row, count = min(max(__ldg(a.counts + row), 0), a.capacity);
   if (slot < 0 || slot >= a.slot_count) return;
   const int64_t head = (int64_t)h * group + g0;  // the unit's first query head
   Rows<D> r;
@@ -255,7 +255,6 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
-  const int count = min(max(a.counts[row], 0), a.capacity);
   const int64_t own = ((int64_t)slot * a.kv_heads + h) * a.capacity, shared = (int64_t)h * a.prefix_capacity;
   const int prefix = plan.parts ? 0 : a.prefix_length;
   // positions [from, to) of prefix ++ own cache, in blocks that do not straddle the two
@@ -290,7 +289,7 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
   };
 #pragma unroll
-  for (int i = 0; i < kStreamStages - 1; i++)
+  for (int i = 0; i < kStreamStages; i++)
     if (i < mine) issue(i);
   load_queries<T, D>(r, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, scale, lane);
   int i = 0;
@@ -298,12 +297,12 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
   for (; i < mine; i++) {
     ok = __all_sync(0xffffffffu, barrier_wait(&bars[i % kStreamStages], (uint32_t)(i / kStreamStages) & 1));
     if (!ok) break;
-    // the stage of block i - 1 has been read by every lane that came here
-    if (i + kStreamStages - 1 < mine) issue(i + kStreamStages - 1);
     attend_block<D>(r, ring[i % kStreamStages], length(i), lane);
+    __syncwarp();  // every lane has read the stage
+    if (i + kStreamStages < mine) issue(i + kStreamStages);
   }
   if (!ok) {  // copies may still be landing: give them their time before the memory is let go
-    for (int k = i; k < min(mine, i + kStreamStages - 1); k++) barrier_wait(&bars[k % kStreamStages], (uint32_t)(k / kStreamStages) & 1);
+    for (int k = i; k < min(mine, i + kStreamStages); k++) barrier_wait(&bars[k % kStreamStages], (uint32_t)(k / kStreamStages) & 1);
     if (lane == 0) report_wait_timeout(wait_words, kWaitAttention);
     r.M = 0.0f;
     r.l = NAN;
@@ -316,6 +315,25 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
   for (int t = 0; t < Rows<D>::kTiles; t++) {
     o[t] = r.o[t][0] + r.o[t][2];
     o[N / 2 + t] = r.o[t][1] + r.o[t][3];
+  }
+  // the prefix's parts, where no split waits for the merge kernel: each warp of the unit takes some
+  const int64_t at = (int64_t)row * a.heads + head + g;
+#pragma unroll 2
+  for (int p = plan.splits == 1 && g < heads ? member : plan.parts; p < plan.parts; p += share) {
+    const int64_t part = p * parts.per_part + at;
+    const float2 ml = parts.ml[part];
+    if (ml.x == -INFINITY) continue;
+    const float M = fmaxf(r.M, ml.x), f0 = r.M == -INFINITY ? 0.0f : power2f(r.M - M), f1 = power2f(ml.x - M);
+    r.l = fmaf(r.l, f0, ml.y * f1);
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(parts.o + part * D + c * N + i);
+      o[i] = fmaf(o[i], f0, v.x * f1);
+      o[i + 1] = fmaf(o[i + 1], f0, v.y * f1);
+      o[i + 2] = fmaf(o[i + 2], f0, v.z * f1);
+      o[i + 3] = fmaf(o[i + 3], f0, v.w * f1);
+    }
+    r.M = M;
   }
   if (share > 1) {
     float* merge_o = reinterpret_cast<float*>(raw);  // [warps][8][D], where the rings were
@@ -350,7 +368,6 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
     r.l = L;
   }
   if (g >= heads) return;
-  const int64_t at = (int64_t)row * a.heads + head + g;
   if (plan.splits > 1) {
     const int64_t part = (int64_t)(plan.parts + split) * parts.per_part + at;
     if (c == 0) parts.ml[part] = make_float2(r.M, r.l);
@@ -359,22 +376,6 @@ __global__ void __launch_bounds__(kStreamThreads, D == 64 ? 2 : 1)
     for (int i = 0; i < N; i += 4)
       *reinterpret_cast<float4*>(parts.o + part * D + c * N + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
     return;
-  }
-  for (int p = 0; p < plan.parts; p++) {
-    const int64_t part = p * parts.per_part + at;
-    const float2 ml = parts.ml[part];
-    if (ml.x == -INFINITY) continue;
-    const float M = fmaxf(r.M, ml.x), f0 = r.M == -INFINITY ? 0.0f : power2f(r.M - M), f1 = power2f(ml.x - M);
-    r.l = fmaf(r.l, f0, ml.y * f1);
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(parts.o + part * D + c * N + i);
-      o[i] = fmaf(o[i], f0, v.x * f1);
-      o[i + 1] = fmaf(o[i + 1], f0, v.y * f1);
-      o[i + 2] = fmaf(o[i + 2], f0, v.z * f1);
-      o[i + 3] = fmaf(o[i + 3], f0, v.w * f1);
-    }
-    r.M = M;
   }
   const float over = r.l > 0.0f ? 1.0f / r.l : r.l == 0.0f ? 0.0f : r.l;
 #pragma unroll
