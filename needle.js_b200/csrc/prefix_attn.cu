@@ -7,16 +7,20 @@
 //   j over the prefix and the row's own positions;  lse = m + log sum_j e^(s_j - m)
 //
 // k_attend_stream.  The query heads of one KV head (up to 8) meet 32 positions at a time on the tensor
-// cores (mma.sync m16n8k16, fp16 x fp16 -> fp32).  M is only the heads of one row, so the products are thin
-// and the kernel lives on its loads: a position costs 2 D + 8 bytes.  Every warp streams its positions
-// through a ring of its own in shared memory, filled by bulk copies, so no warp waits for another.
-// Codes are exact in fp16; queries and weights, binary32, are split into an fp16 head (MMA rows 0-7) and
-// tail (rows 8-15), which the accumulator's two row halves add up again, so results have binary32 accuracy
-// for every element type.  The order of k inside a product is free, so lanes read K and V from the ring
-// straight into operand order, 16 (8) consecutive codes at a time, and no byte is transposed through memory:
-//   K: lane (n, c) = (lane / 4, lane % 4) reads D / 4 codes of position n; k-step t takes 4 of them;
-//   V: the lane reads D / 8 codes of the positions 2c, 2c + 1, 2c + 8, 2c + 9, which are the ones whose
-//      weights the score product left in its registers; output tile j takes code j of each.
+// cores (mma.sync m16n8k16, fp16 x fp16 -> fp32).  One row has few heads, so the products are thin and the
+// kernel lives on its loads, 2 D + 8 bytes a position, and on its instruction count.  Every warp streams
+// its positions through a ring of its own in shared memory, filled by bulk copies, so no warp waits for
+// another.  Codes are exact in fp16; queries and weights, binary32, are split into fp16 heads and tails
+// that sit in neighbouring columns of N (4 query heads fill its 8), whose products a lane adds up again:
+// results have binary32 accuracy for every element type.  Positions and output dimensions are the M side:
+//   S^T (positions x heads) = K Q^T: lane (g, c) = (lane / 4, lane % 4) reads codes of the positions g and
+//     g + 8 straight into operand order (the order of k inside a product is free) and gets their scores of
+//     head c;
+//   O^T (dimensions x heads) = V^T P^T: the lane reads D / 8 codes of the positions 2c, 2c + 1, 2c + 8,
+//     2c + 9 and pairs them byte by byte; the weights, packed as (head, tail), are brought to the lanes that
+//     need them by one 8 x 8 transposition (movmatrix) for 8 positions.
+// Groups of more than 4 heads (NG 2) use every converted code twice.  With heads on the M side, where 2 of
+// 16 rows were of use for 2 heads, the kernel took 1.6 times the instructions.
 // A CTA is one unit (row, KV head, 8 heads, split of the positions): 1 to 8 warps, merged in shared memory;
 // with many units a single warp, since caches of different ages would leave the others of a CTA idle; splits and the prefix's parts are merged from the workspace.
 #include <algorithm>
@@ -67,81 +71,107 @@ __device__ __forceinline__ void copy_bulk(void* to, const void* from, uint32_t b
       : "memory");
 }
 
-// A warp's state of up to 8 heads: lane (g, c) keeps head g's reference maximum, its own share of the sum,
-// and D / 4 consecutive output dimensions from c * D / 4 on.
-template <int D>
+// A warp's state of up to 4 NG heads: lane (g, c) keeps the heads c, 4 + c: their reference maximum, the sum of
+// its own weights, and the output dimensions g * D / 8 .. + D / 8 - 1.
+template <int D, int NG>
 struct Rows {
-  static constexpr int kTiles = D / 8;
-  uint32_t q[D / 16][4];  // A operand of each k-step: head and tail of the scaled query
-  float inverse;          // undoes the query's power of two
-  float M, l;             // reference maximum (base 2), sum of the lane's weights
-  float o[kTiles][4];
+  uint32_t q[NG][D / 16][2];  // B operand of each k-step: column g is head g / 2, its head or tail by g % 2
+  float inverse[NG];          // undoes the query's power of two
+  float M[NG], l[NG];         // reference maximum (base 2), sum of the lane's weights
+  float o[NG][D / 16][4];
 };
 
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {  // 8 x 8 of 16 bits, a row's pair per lane
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // The n positions of a stage.
-template <int D>
-__device__ __forceinline__ void attend_block(Rows<D>& r, const Stage<D>& b, int n, int lane) {
+template <int D, int NG>
+__device__ __forceinline__ void attend_block(Rows<D, NG>& r, const Stage<D>& b, int n, int lane) {
   const int g = lane >> 2, c = lane & 3;
-  float s[8], vs[8];  // [16-position half][position 2c, 2c + 1, 2c + 8, 2c + 9]
-  float top = -INFINITY, vtop = 0.0f;
+  float s[NG][4], vs[4];  // positions g, g + 8, g + 16, g + 24
+  float vtop = 0.0f;
 #pragma unroll
-  for (int t = 0; t < 4; t++) {
-    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int u = 0; u < 2; u++) {
+    float d[NG][4];
+#pragma unroll
+    for (int q = 0; q < NG; q++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) d[q][i] = 0.0f;
 #pragma unroll
     for (int h = 0; h < D / 64; h++) {
-      const uint4 k4 = *reinterpret_cast<const uint4*>(b.k + (t * 8 + g) * D + h * 64 + c * 16);
-      const uint32_t w[4] = {k4.x, k4.y, k4.z, k4.w};
+      const uint4 k0 = *reinterpret_cast<const uint4*>(b.k + (u * 16 + g) * D + h * 64 + c * 16);
+      const uint4 k1 = *reinterpret_cast<const uint4*>(b.k + (u * 16 + 8 + g) * D + h * 64 + c * 16);
+      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const uint32_t u = w[k] ^ 0x80808080u;
-        mma_f16(d, r.q[h * 4 + k], codes_f16(u, 0x4140), codes_f16(u, 0x4342));
+        const uint32_t x0 = w0[k] ^ 0x80808080u, x1 = w1[k] ^ 0x80808080u;
+        const uint32_t a[4] = {codes_f16(x0, 0x4140), codes_f16(x1, 0x4140), codes_f16(x0, 0x4342), codes_f16(x1, 0x4342)};
+#pragma unroll
+        for (int q = 0; q < NG; q++) mma_f16(d[q], a, r.q[q][h * 4 + k][0], r.q[q][h * 4 + k][1]);
       }
     }
-    const float2 ks2 = *reinterpret_cast<const float2*>(b.ks + t * 8 + 2 * c);
-    const float2 vs2 = *reinterpret_cast<const float2*>(b.vs + t * 8 + 2 * c);
-    s[2 * t] = (d[0] + d[2]) * (ks2.x * r.inverse);
-    s[2 * t + 1] = (d[1] + d[3]) * (ks2.y * r.inverse);
-    vs[2 * t] = vs2.x;
-    vs[2 * t + 1] = vs2.y;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float ks = b.ks[u * 16 + i * 8 + g];
+      vs[2 * u + i] = b.vs[u * 16 + i * 8 + g];
+      vtop = fmaxf(vtop, fabsf(vs[2 * u + i]));
+#pragma unroll
+      for (int q = 0; q < NG; q++) s[q][2 * u + i] = (d[q][2 * i] + d[q][2 * i + 1]) * (ks * r.inverse[q]);
+    }
   }
   if (n < kBlock) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if ((i >> 1) * 8 + 2 * c + (i & 1) >= n) s[i] = -INFINITY;
-  }
+    for (int i = 0; i < 4; i++)
+      if (i * 8 + g >= n) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    top = fmaxf(top, s[i]);
-    vtop = fmaxf(vtop, fabsf(vs[i]));
+        for (int q = 0; q < NG; q++) s[q][i] = -INFINITY;
+      }
   }
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
   vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)));
-  const float reach = top + (float)(min(max(exponent_of(vtop), -100), 100) - 6);
-  if (__any_sync(0xffffffffu, reach > r.M + kRaise)) {
-    const float Mn = reach > r.M + kRaise ? reach + 1.0f : r.M;
-    const float f = r.M == -INFINITY ? 0.0f : power2f(r.M - Mn);
-    r.l *= f;
+  const float ev = (float)(min(max(exponent_of(vtop), -100), 100) - 6);
+  float reach[NG];
+  bool raise = false;
 #pragma unroll
-    for (int t = 0; t < Rows<D>::kTiles; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) r.o[t][i] *= f;
-    r.M = Mn;
+  for (int q = 0; q < NG; q++) {
+    float top = fmaxf(fmaxf(s[q][0], s[q][1]), fmaxf(s[q][2], s[q][3]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    reach[q] = top + ev;
+    raise = raise || reach[q] > r.M[q] + kRaise;
   }
-  const float base = r.M == -INFINITY ? 0.0f : r.M;
+  if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-  for (int half = 0; half < 2; half++) {
-    float w[4];
+    for (int q = 0; q < NG; q++) {
+      const float Mn = reach[q] > r.M[q] + kRaise ? reach[q] + 1.0f : r.M[q];
+      const float f = r.M[q] == -INFINITY ? 0.0f : power2f(r.M[q] - Mn);
+      r.l[q] *= f;
+#pragma unroll
+      for (int t = 0; t < D / 16; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.o[q][t][i] *= f;
+      r.M[q] = Mn;
+    }
+  }
+  uint32_t p[NG][4];  // weights of 8 positions each, as B operand
+#pragma unroll
+  for (int q = 0; q < NG; q++) {
+    const float base = r.M[q] == -INFINITY ? 0.0f : r.M[q];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float p = power2f(s[half * 4 + i] - base);
-      r.l += p;
-      w[i] = p * vs[half * 4 + i];
+      const float e = power2f(s[q][i] - base);
+      r.l[q] += e;
+      const float w = e * vs[i];
+      const float head = __half2float(__float2half_rn(w));
+      p[q][i] = transpose8(half2_bits(__floats2half2_rn(head, w - head)));
     }
-    uint32_t a[4];  // rows 0-7: heads of the weights, rows 8-15: tails
-    split_f16(w[0], w[1], a[0], a[1]);
-    split_f16(w[2], w[3], a[2], a[3]);
-    const int8_t* v = b.v + (half * 16 + 2 * c) * D + g * (D / 8);
+  }
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    const int8_t* v = b.v + (u * 16 + 2 * c) * D + g * (D / 8);
 #pragma unroll
     for (int h = 0; h < D / 64; h++) {
       uint2 v2[4];
@@ -149,67 +179,74 @@ __device__ __forceinline__ void attend_block(Rows<D>& r, const Stage<D>& b, int 
       for (int i = 0; i < 4; i++) v2[i] = *reinterpret_cast<const uint2*>(v + ((i & 1) + (i >> 1) * 8) * D + h * 8);
 #pragma unroll
       for (int word = 0; word < 2; word++) {
-        uint32_t u[4];
+        uint32_t x[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] = (word ? v2[i].y : v2[i].x) ^ 0x80808080u;
+        for (int i = 0; i < 4; i++) x[i] = (word ? v2[i].y : v2[i].x) ^ 0x80808080u;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {  // codes 2k, 2k + 1 of the word
+        for (int k = 0; k < 2; k++) {  // codes 2k, 2k + 1 of the word: two neighbouring dimensions
           const uint32_t sel = k ? 0x7362 : 0x5140;
-          const uint32_t lo = __byte_perm(u[0], u[1], sel), hi = __byte_perm(u[2], u[3], sel);
-          const int t = h * 8 + word * 4 + 2 * k;
-          mma_f16(r.o[t], a, codes_f16(lo, 0x4140), codes_f16(hi, 0x4140));
-          mma_f16(r.o[t + 1], a, codes_f16(lo, 0x4342), codes_f16(hi, 0x4342));
+          const uint32_t lo = __byte_perm(x[0], x[1], sel), hi = __byte_perm(x[2], x[3], sel);
+          const uint32_t a[4] = {codes_f16(lo, 0x4140), codes_f16(lo, 0x4342), codes_f16(hi, 0x4140), codes_f16(hi, 0x4342)};
+#pragma unroll
+          for (int q = 0; q < NG; q++) mma_f16(r.o[q][h * 4 + word * 2 + k], a, p[q][2 * u], p[q][2 * u + 1]);
         }
       }
     }
   }
 }
 
-// Reads the unit's queries into MMA operand order, scaled by `scale` * log2(e) and, per head, to a
-// largest magnitude in [2^10, 2^11).
-template <class T, int D>
-__device__ __forceinline__ void load_queries(Rows<D>& r, const T* q, int heads, float scale, int lane) {
+// Reads the unit's queries into operand order, scaled by `scale` * log2(e) and, per head, to a largest
+// magnitude in [2^10, 2^11).
+template <class T, int D, int NG>
+__device__ __forceinline__ void load_queries(Rows<D, NG>& r, const T* q, int heads, float scale, int lane) {
   constexpr int V = 16 / sizeof(T);
   const int g = lane >> 2, c = lane & 3;
-  float x[D / 4];
-  float top = 0.0f;
   const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
 #pragma unroll
-  for (int h = 0; h < D / 64; h++)
+  for (int n = 0; n < NG; n++) {
+    const int head = 4 * n + (g >> 1);
+    float x[D / 4];
+    float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; i += V) {
-      const T* p = q + g * D + h * 64 + c * 16 + i;
-      Vec<T, V> v{};
-      if (g < heads) {
-        if (vec) {
-          v = *reinterpret_cast<const Vec<T, V>*>(p);
-        } else {
+    for (int h = 0; h < D / 64; h++)
 #pragma unroll
-          for (int e = 0; e < V; e++) v.v[e] = p[e];
+      for (int i = 0; i < 16; i += V) {
+        const T* p = q + head * D + h * 64 + c * 16 + i;
+        Vec<T, V> v{};
+        if (head < heads) {
+          if (vec) {
+            v = *reinterpret_cast<const Vec<T, V>*>(p);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) v.v[e] = p[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          x[h * 16 + i + e] = to_f32(v.v[e]) * (scale * kLog2e);
+          top = fmaxf(top, fabsf(x[h * 16 + i + e]));
         }
       }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = min(max(exponent_of(top), -110), 110);
+    const float f = power2(10 - e);
+    r.inverse[n] = __shfl_sync(0xffffffffu, power2(e - 10), 8 * c);  // of head c, whose columns are 2c and 2c + 1
 #pragma unroll
-      for (int e = 0; e < V; e++) {
-        x[h * 16 + i + e] = to_f32(v.v[e]) * (scale * kLog2e);
-        top = fmaxf(top, fabsf(x[h * 16 + i + e]));
+    for (int k = 0; k < D / 16; k++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        uint32_t head2, tail2;
+        split_f16(x[4 * k + 2 * i] * f, x[4 * k + 2 * i + 1] * f, head2, tail2);
+        r.q[n][k][i] = g & 1 ? tail2 : head2;
       }
-    }
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  const int e = min(max(exponent_of(top), -110), 110);
-  const float f = power2(10 - e);
-  r.inverse = power2(e - 10);
+    r.M[n] = -INFINITY;
+    r.l[n] = 0.0f;
 #pragma unroll
-  for (int k = 0; k < D / 16; k++) {
-    split_f16(x[4 * k] * f, x[4 * k + 1] * f, r.q[k][0], r.q[k][1]);
-    split_f16(x[4 * k + 2] * f, x[4 * k + 3] * f, r.q[k][2], r.q[k][3]);
+    for (int t = 0; t < D / 16; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) r.o[n][t][i] = 0.0f;
   }
-  r.M = -INFINITY;
-  r.l = 0.0f;
-#pragma unroll
-  for (int t = 0; t < Rows<D>::kTiles; t++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) r.o[t][i] = 0.0f;
 }
 
 template <class T, int N>
@@ -229,11 +266,49 @@ __device__ __forceinline__ void store_out(T* p, const float* x, bool vec) {
   }
 }
 
-template <class T, int D>
-__global__ void __maxnreg__(D == 64 ? 80 : 152)
+// What becomes of N output dimensions of a head, from g * N on, held by lane g of its eight.
+template <int N>
+__device__ __forceinline__ void store_part(const Parts& parts, int64_t part, float m, float l, const float* o, int g) {
+  if (g == 0) parts.ml[part] = make_float2(m, l);
+  if (m == -INFINITY) return;  // an empty part: its values are never read
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    *reinterpret_cast<float4*>(parts.o + part * (8 * N) + g * N + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+}
+
+template <int N>
+__device__ __forceinline__ void add_part(const Parts& parts, int64_t part, float& m, float& l, float* o, int g) {
+  const float2 ml = parts.ml[part];
+  if (ml.x == -INFINITY) return;
+  const float M = fmaxf(m, ml.x), f0 = m == -INFINITY ? 0.0f : power2f(m - M), f1 = power2f(ml.x - M);
+  l = fmaf(l, f0, ml.y * f1);
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(parts.o + part * (8 * N) + g * N + i);
+    o[i] = fmaf(o[i], f0, v.x * f1);
+    o[i + 1] = fmaf(o[i + 1], f0, v.y * f1);
+    o[i + 2] = fmaf(o[i + 2], f0, v.z * f1);
+    o[i + 3] = fmaf(o[i + 3], f0, v.w * f1);
+  }
+  m = M;
+}
+
+template <class T, int N>
+__device__ __forceinline__ void finish(const needle_prefix_attention& a, int row, int64_t head, int64_t at, float m, float l,
+                                       float* o, int g) {
+  const float over = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+#pragma unroll
+  for (int i = 0; i < N; i++) o[i] *= over;
+  T* out = static_cast<T*>(a.out) + row * a.out_stride + head * (8 * N) + g * N;
+  store_out<T, N>(out, o, (reinterpret_cast<uintptr_t>(out) & 15) == 0);
+  if (g == 0 && a.lse) a.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <class T, int D, int NG>
+__global__ void __maxnreg__(D * NG == 64 ? 72 : D * NG == 128 ? 96 : 152)
     k_attend_stream(const __grid_constant__ needle_prefix_attention a, const StreamPlan plan, const Parts parts, float scale,
                     uint32_t* wait_words) {
-  constexpr int N = D / 4;  // output dimensions of a lane
+  constexpr int N = D / 8;  // output dimensions of a lane
   extern __shared__ __align__(16) unsigned char raw[];
   __shared__ __align__(8) uint64_t full[kStreamWarps][kStreamStages];
   __shared__ float merge_m[kStreamWarps][kGroupHeads], merge_l[kStreamWarps][kGroupHeads];
@@ -241,12 +316,12 @@ __global__ void __maxnreg__(D == 64 ? 80 : 152)
   const int share = plan.warps, member = warp;
   const int split = blockIdx.y, group = a.heads / a.kv_heads, of_row = a.kv_heads * plan.groups;
   const int row = (int)(blockIdx.x / of_row), rest = (int)(blockIdx.x - row * of_row);
-  const int h = rest / plan.groups, g0 = (rest - h * plan.groups) * kGroupHeads;
-  const int heads = min(kGroupHeads, group - g0);
+  const int h = rest / plan.groups, g0 = (rest - h * plan.groups) * 4 * NG;
+  const int heads = min(4 * NG, group - g0);
   const int slot = a.slots ? __ldg(a.slots + row) : row, count = min(max(__ldg(a.counts + row), 0), a.capacity);
   if (slot < 0 || slot >= a.slot_count) return;
   const int64_t head = (int64_t)h * group + g0;  // the unit's first query head
-  Rows<D> r;
+  Rows<D, NG> r;
   bool ok = true;
   Stage<D>* ring = reinterpret_cast<Stage<D>*>(raw) + warp * kStreamStages;
   uint64_t* bars = full[warp];
@@ -291,98 +366,85 @@ __global__ void __maxnreg__(D == 64 ? 80 : 152)
 #pragma unroll
   for (int i = 0; i < kStreamStages; i++)
     if (i < mine) issue(i);
-  load_queries<T, D>(r, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, scale, lane);
+  load_queries<T, D, NG>(r, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, scale, lane);
   int i = 0;
 #pragma unroll 1
   for (; i < mine; i++) {
     ok = __all_sync(0xffffffffu, barrier_wait(&bars[i % kStreamStages], (uint32_t)(i / kStreamStages) & 1));
     if (!ok) break;
-    attend_block<D>(r, ring[i % kStreamStages], length(i), lane);
+    attend_block<D, NG>(r, ring[i % kStreamStages], length(i), lane);
     __syncwarp();  // every lane has read the stage
     if (i + kStreamStages < mine) issue(i + kStreamStages);
   }
   if (!ok) {  // copies may still be landing: give them their time before the memory is let go
     for (int k = i; k < min(mine, i + kStreamStages); k++) barrier_wait(&bars[k % kStreamStages], (uint32_t)(k / kStreamStages) & 1);
     if (lane == 0) report_wait_timeout(wait_words, kWaitAttention);
-    r.M = 0.0f;
-    r.l = NAN;
   }
-  r.l += __shfl_xor_sync(0xffffffffu, r.l, 1);
-  r.l += __shfl_xor_sync(0xffffffffu, r.l, 2);
-  // the lane's output dimensions in order, the two row halves of the accumulators added
-  float o[N];
+  float* merge_o = reinterpret_cast<float*>(raw);  // [warps][4 NG][D], where the rings were
+  const int64_t first = (int64_t)row * a.heads + head;
+  if (share > 1) __syncthreads();
 #pragma unroll
-  for (int t = 0; t < Rows<D>::kTiles; t++) {
-    o[t] = r.o[t][0] + r.o[t][2];
-    o[N / 2 + t] = r.o[t][1] + r.o[t][3];
-  }
-  // the prefix's parts, where no split waits for the merge kernel: each warp of the unit takes some
-  const int64_t at = (int64_t)row * a.heads + head + g;
+  for (int q = 0; q < NG; q++) {
+    const int hh = 4 * q + c;  // the lane's head
+    const int64_t at = first + hh;
+    float m = ok ? r.M[q] : 0.0f, l = ok ? r.l[q] : NAN;
+    l += __shfl_xor_sync(0xffffffffu, l, 4);
+    l += __shfl_xor_sync(0xffffffffu, l, 8);
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+    // the products of heads and tails added
+    float o[N];
+#pragma unroll
+    for (int t = 0; t < D / 16; t++) {
+      o[2 * t] = r.o[q][t][0] + r.o[q][t][1];
+      o[2 * t + 1] = r.o[q][t][2] + r.o[q][t][3];
+    }
+    if (plan.splits > 1 && share == 1) {
+      if (hh < heads) store_part<N>(parts, (int64_t)(plan.parts + split) * parts.per_part + at, m, l, o, g);
+      continue;
+    }
+    // the prefix's parts, where no split waits for the merge kernel: each warp of the unit takes some
 #pragma unroll 2
-  for (int p = plan.splits == 1 && g < heads ? member : plan.parts; p < plan.parts; p += share) {
-    const int64_t part = p * parts.per_part + at;
-    const float2 ml = parts.ml[part];
-    if (ml.x == -INFINITY) continue;
-    const float M = fmaxf(r.M, ml.x), f0 = r.M == -INFINITY ? 0.0f : power2f(r.M - M), f1 = power2f(ml.x - M);
-    r.l = fmaf(r.l, f0, ml.y * f1);
+    for (int p = plan.splits == 1 && hh < heads ? warp : plan.parts; p < plan.parts; p += share)
+      add_part<N>(parts, p * parts.per_part + at, m, l, o, g);
+    if (share > 1) {
+      if (g == 0) {
+        merge_m[warp][hh] = m;
+        merge_l[warp][hh] = l;
+      }
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(parts.o + part * D + c * N + i);
-      o[i] = fmaf(o[i], f0, v.x * f1);
-      o[i + 1] = fmaf(o[i + 1], f0, v.y * f1);
-      o[i + 2] = fmaf(o[i + 2], f0, v.z * f1);
-      o[i + 3] = fmaf(o[i + 3], f0, v.w * f1);
+      for (int i = 0; i < N; i += 4)
+        *reinterpret_cast<float4*>(&merge_o[(warp * 4 * NG + hh) * D + g * N + i]) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+    } else if (hh < heads) {
+      finish<T, N>(a, row, head + hh, at, m, l, o, g);
     }
-    r.M = M;
   }
-  if (share > 1) {
-    float* merge_o = reinterpret_cast<float*>(raw);  // [warps][8][D], where the rings were
-    __syncthreads();
-    if (c == 0) {
-      merge_m[warp][g] = r.M;
-      merge_l[warp][g] = r.l;
-    }
+  if (share == 1) return;
+  __syncthreads();
+  if (warp != 0) return;
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      *reinterpret_cast<float4*>(&merge_o[(warp * kGroupHeads + g) * D + c * N + i]) =
-          make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-    __syncthreads();
-    if (member != 0) return;
-    float M = -INFINITY, L = 0.0f;
-    for (int w = 0; w < share; w++) M = fmaxf(M, merge_m[w][g]);
+  for (int q = 0; q < NG; q++) {
+    const int hh = 4 * q + c;
+    if (hh >= heads) continue;
+    const int64_t at = first + hh;
+    float M = -INFINITY, L = 0.0f, o[N];
+    for (int w = 0; w < share; w++) M = fmaxf(M, merge_m[w][hh]);
 #pragma unroll
     for (int i = 0; i < N; i++) o[i] = 0.0f;
     for (int w = 0; w < share; w++) {
-      const float m = merge_m[w][g], f = m == -INFINITY ? 0.0f : power2f(m - M);
-      L = fmaf(merge_l[w][g], f, L);
+      const float m = merge_m[w][hh], f = m == -INFINITY ? 0.0f : power2f(m - M);
+      L = fmaf(merge_l[w][hh], f, L);
 #pragma unroll
       for (int i = 0; i < N; i += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(&merge_o[(w * kGroupHeads + g) * D + c * N + i]);
+        const float4 v = *reinterpret_cast<const float4*>(&merge_o[(w * 4 * NG + hh) * D + g * N + i]);
         o[i] = fmaf(v.x, f, o[i]);
         o[i + 1] = fmaf(v.y, f, o[i + 1]);
         o[i + 2] = fmaf(v.z, f, o[i + 2]);
         o[i + 3] = fmaf(v.w, f, o[i + 3]);
       }
     }
-    r.M = M;
-    r.l = L;
+    if (plan.splits > 1) store_part<N>(parts, (int64_t)(plan.parts + split) * parts.per_part + at, M, L, o, g);
+    else finish<T, N>(a, row, head + hh, at, M, L, o, g);
   }
-  if (g >= heads) return;
-  if (plan.splits > 1) {
-    const int64_t part = (int64_t)(plan.parts + split) * parts.per_part + at;
-    if (c == 0) parts.ml[part] = make_float2(r.M, r.l);
-    if (r.M == -INFINITY) return;  // an empty split: its values are never read
-#pragma unroll
-    for (int i = 0; i < N; i += 4)
-      *reinterpret_cast<float4*>(parts.o + part * D + c * N + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-    return;
-  }
-  const float over = r.l > 0.0f ? 1.0f / r.l : r.l == 0.0f ? 0.0f : r.l;
-#pragma unroll
-  for (int i = 0; i < N; i++) o[i] *= over;
-  T* out = static_cast<T*>(a.out) + row * a.out_stride + (head + g) * D + c * N;
-  store_out<T, N>(out, o, (reinterpret_cast<uintptr_t>(out) & 15) == 0);
-  if (c == 0 && a.lse) a.lse[at] = r.l == 0.0f ? -INFINITY : (r.M + log2f(r.l)) * kLn2;
 }
 
 // Merges the parts of every (row, head): one warp each.
@@ -483,11 +545,14 @@ cudaError_t launch_attention(const needle_prefix_attention& a, const StreamPlan&
   const int64_t units = int64_t(a.rows) * a.kv_heads * p.groups;
   const size_t smem = sizeof(Stage<D>) * kStreamStages * p.warps;
   static_assert(sizeof(Stage<D>) * kStreamStages >= size_t(kGroupHeads) * D * 4, "the merge takes the rings' place");
-  cudaError_t e = cudaFuncSetAttribute(k_attend_stream<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       int(sizeof(Stage<D>) * kStreamStages * kStreamWarps));
-  if (e != cudaSuccess) return e;
-  k_attend_stream<T, D><<<dim3((unsigned)units, p.splits), p.warps * 32, smem, s>>>(a, p, parts, scale, wait_words);
-  e = cudaGetLastError();
+  auto go = [&](auto kernel) {
+    const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 int(sizeof(Stage<D>) * kStreamStages * kStreamWarps));
+    if (err != cudaSuccess) return err;
+    kernel<<<dim3((unsigned)units, p.splits), p.warps * 32, smem, s>>>(a, p, parts, scale, wait_words);
+    return cudaGetLastError();
+  };
+  cudaError_t e = a.heads / a.kv_heads <= 4 ? go(k_attend_stream<T, D, 1>) : go(k_attend_stream<T, D, 2>);
   if (e != cudaSuccess || p.splits == 1) return e;
   k_attend_merge<T, D><<<(unsigned)((parts.per_part + kStreamWarps - 1) / kStreamWarps), kStreamThreads, 0, s>>>(a, part_count(p), parts);
   return cudaGetLastError();
