@@ -21,8 +21,8 @@
 //     need them by one 8 x 8 transposition (movmatrix) for 8 positions.
 // Groups of more than 4 heads (NG 2) use every converted code twice.  With heads on the M side, where 2 of
 // 16 rows were of use for 2 heads, the kernel took 1.6 times the instructions.
-// A CTA is one unit (row, KV head, 8 heads, split of the positions): 1 to 8 warps, merged in shared memory;
-// with many units a single warp, since caches of different ages would leave the others of a CTA idle; splits and the prefix's parts are merged from the workspace.
+// A unit (row, KV head, 8 heads, split of the positions) has a CTA of 2 to 8 warps, merged in shared memory, or,
+// where units are many, one warp, beside those of the row's other KV heads: caches of one age end together; splits and the prefix's parts are merged from the workspace.
 #include <algorithm>
 #include <cmath>
 
@@ -41,7 +41,9 @@ constexpr int kBlock = 32;      // positions of a step
 // How a call is laid out (plan_for).
 struct StreamPlan {
   int groups;      // 8-head groups of a KV head
-  int warps;       // warps per unit: 1, 2, 4 or 8
+  int group;       // query heads of a KV head
+  int warps, warps_log2;  // warps per unit: 1, 2, 4 or 8
+  int together;    // units of a row in a CTA, where a unit is one warp
   int splits;      // splits of the positions
   int split_len;   // positions of a split
   int parts;       // prefix parts in the workspace, in front of the splits; 0: the stream reads the prefix
@@ -161,12 +163,13 @@ __device__ __forceinline__ void attend_block(Rows<D, NG>& r, const Stage<D>& b, 
   for (int q = 0; q < NG; q++) {
     const float base = r.M[q] == -INFINITY ? 0.0f : r.M[q];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float e = power2f(s[q][i] - base);
-      r.l[q] += e;
-      const float w = e * vs[i];
-      const float head = __half2float(__float2half_rn(w));
-      p[q][i] = transpose8(half2_bits(__floats2half2_rn(head, w - head)));
+    for (int i = 0; i < 4; i += 2) {
+      const float e0 = power2f(s[q][i] - base), e1 = power2f(s[q][i + 1] - base);
+      r.l[q] += e0 + e1;
+      uint32_t heads, tails;
+      split_f16(e0 * vs[i], e1 * vs[i + 1], heads, tails);
+      p[q][i] = transpose8(__byte_perm(heads, tails, 0x5410));
+      p[q][i + 1] = transpose8(__byte_perm(heads, tails, 0x7632));
     }
   }
 #pragma unroll
@@ -195,43 +198,59 @@ __device__ __forceinline__ void attend_block(Rows<D, NG>& r, const Stage<D>& b, 
   }
 }
 
-// Reads the unit's queries into operand order, scaled by `scale` * log2(e) and, per head, to a largest
-// magnitude in [2^10, 2^11).
+// The unit's queries as they are in memory: lane (g, c) takes its share of head g / 2 (and 4 + g / 2).
 template <class T, int D, int NG>
-__device__ __forceinline__ void load_queries(Rows<D, NG>& r, const T* q, int heads, float scale, int lane) {
+struct RawQueries {
+  Vec<T, 16 / sizeof(T)> v[NG][D / 64][sizeof(T)];
+};
+
+template <class T, int D, int NG>
+__device__ __forceinline__ void load_queries(RawQueries<T, D, NG>& raw, const T* q, int heads, int lane) {
   constexpr int V = 16 / sizeof(T);
   const int g = lane >> 2, c = lane & 3;
   const bool vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0;
 #pragma unroll
   for (int n = 0; n < NG; n++) {
     const int head = 4 * n + (g >> 1);
-    float x[D / 4];
-    float top = 0.0f;
 #pragma unroll
     for (int h = 0; h < D / 64; h++)
 #pragma unroll
-      for (int i = 0; i < 16; i += V) {
-        const T* p = q + head * D + h * 64 + c * 16 + i;
-        Vec<T, V> v{};
+      for (int i = 0; i < (int)sizeof(T); i++) {
+        const T* p = q + head * D + h * 64 + c * 16 + i * V;
+        raw.v[n][h][i] = Vec<T, V>{};
         if (head < heads) {
           if (vec) {
-            v = *reinterpret_cast<const Vec<T, V>*>(p);
+            raw.v[n][h][i] = *reinterpret_cast<const Vec<T, V>*>(p);
           } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) v.v[e] = p[e];
+            for (int e = 0; e < V; e++) raw.v[n][h][i].v[e] = p[e];
           }
         }
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-          x[h * 16 + i + e] = to_f32(v.v[e]) * (scale * kLog2e);
-          top = fmaxf(top, fabsf(x[h * 16 + i + e]));
-        }
       }
+  }
+}
+
+// The queries in operand order, scaled by `scale` * log2(e) and, per head, to a largest magnitude in
+// [2^10, 2^11); the rest of the warp's state at its beginning.
+template <class T, int D, int NG>
+__device__ __forceinline__ void begin_rows(Rows<D, NG>& r, const RawQueries<T, D, NG>& raw, float scale, int lane) {
+  constexpr int V = 16 / sizeof(T);
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int n = 0; n < NG; n++) {
+    float x[D / 4];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < D / 4; i++) {
+      x[i] = to_f32(raw.v[n][i / 16][i % 16 / V].v[i % V]);
+      top = fmaxf(top, fabsf(x[i]));
+    }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = min(max(exponent_of(top), -110), 110);
     const float f = power2(10 - e);
-    r.inverse[n] = __shfl_sync(0xffffffffu, power2(e - 10), 8 * c);  // of head c, whose columns are 2c and 2c + 1
+    // of head c, whose columns are 2c and 2c + 1
+    r.inverse[n] = __shfl_sync(0xffffffffu, power2(e - 10), 8 * c) * (scale * kLog2e);
 #pragma unroll
     for (int k = 0; k < D / 16; k++)
 #pragma unroll
@@ -305,7 +324,7 @@ __device__ __forceinline__ void finish(const needle_prefix_attention& a, int row
 }
 
 template <class T, int D, int NG>
-__global__ void __maxnreg__(D * NG == 64 ? 72 : D * NG == 128 ? 96 : 152)
+__global__ void __maxnreg__(D == 64 ? (NG == 1 ? 80 : 112) : (NG == 1 ? 144 : 168))
     k_attend_stream(const __grid_constant__ needle_prefix_attention a, const StreamPlan plan, const Parts parts, float scale,
                     uint32_t* wait_words) {
   constexpr int N = D / 8;  // output dimensions of a lane
@@ -313,14 +332,16 @@ __global__ void __maxnreg__(D * NG == 64 ? 72 : D * NG == 128 ? 96 : 152)
   __shared__ __align__(8) uint64_t full[kStreamWarps][kStreamStages];
   __shared__ float merge_m[kStreamWarps][kGroupHeads], merge_l[kStreamWarps][kGroupHeads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
-  const int share = plan.warps, member = warp;
-  const int split = blockIdx.y, group = a.heads / a.kv_heads, of_row = a.kv_heads * plan.groups;
-  const int row = (int)(blockIdx.x / of_row), rest = (int)(blockIdx.x - row * of_row);
-  const int h = rest / plan.groups, g0 = (rest - h * plan.groups) * 4 * NG;
+  const int share = plan.warps, member = share > 1 ? warp : 0;
+  const int row = blockIdx.x, split = blockIdx.z, group = plan.group;
+  const int unit = blockIdx.y * plan.together + (share > 1 ? 0 : warp);  // of the row: KV head, 8-head group of it
+  const int h = plan.groups == 1 ? unit : unit / plan.groups, g0 = (unit - h * plan.groups) * 4 * NG;
   const int heads = min(4 * NG, group - g0);
+  const int64_t head = (int64_t)h * group + g0;  // the unit's first query head
+  RawQueries<T, D, NG> queries;  // ahead of everything that waits for memory
+  load_queries<T, D, NG>(queries, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, lane);
   const int slot = a.slots ? __ldg(a.slots + row) : row, count = min(max(__ldg(a.counts + row), 0), a.capacity);
   if (slot < 0 || slot >= a.slot_count) return;
-  const int64_t head = (int64_t)h * group + g0;  // the unit's first query head
   Rows<D, NG> r;
   bool ok = true;
   Stage<D>* ring = reinterpret_cast<Stage<D>*>(raw) + warp * kStreamStages;
@@ -337,44 +358,66 @@ __global__ void __maxnreg__(D * NG == 64 ? 72 : D * NG == 128 ? 96 : 152)
   const int begin0 = (int)min(from, (int64_t)prefix), end0 = (int)min(max(to, (int64_t)0), (int64_t)prefix);
   const int begin1 = (int)max(from - prefix, (int64_t)0), end1 = (int)max(to - prefix, (int64_t)begin1);
   const int blocks0 = max(end0 - begin0 + kBlock - 1, 0) / kBlock, blocks1 = (end1 - begin1 + kBlock - 1) / kBlock;
-  const int mine = (blocks0 + blocks1 - member + share - 1) / share;  // blocks member, member + share, ...
-  auto length = [&](int i) {
-    const int b = member + i * share;
-    return min(kBlock, b < blocks0 ? end0 - begin0 - b * kBlock : end1 - begin1 - (b - blocks0) * kBlock);
+  const int mine = (blocks0 + blocks1 - member + share - 1) >> plan.warps_log2;  // blocks member, member + share, ...
+  // the next block to be issued: its number, what is left of its segment, and where it is
+  int next = member, left = 0;
+  const int8_t *kp = nullptr, *vp = nullptr;
+  const float *ksp = nullptr, *vsp = nullptr;
+  auto point = [&](bool pre) {
+    const int b = pre ? next : next - blocks0;
+    const int64_t at = (pre ? shared + begin0 : own + begin1) + b * kBlock;
+    left = (pre ? end0 - begin0 : end1 - begin1) - b * kBlock;
+    kp = (pre ? a.prefix_key_codes : a.key_codes) + at * D;
+    vp = (pre ? a.prefix_value_codes : a.value_codes) + at * D;
+    ksp = (pre ? a.prefix_key_scales : a.key_scales) + at + lane;
+    vsp = (pre ? a.prefix_value_scales : a.value_scales) + at + lane;
   };
-  auto issue = [&](int i) {
-    const int b = member + i * share, n = length(i);
-    const bool pre = b < blocks0;
-    const int64_t at = pre ? shared + begin0 + b * kBlock : own + begin1 + (b - blocks0) * kBlock;
-    Stage<D>& s = ring[i % kStreamStages];
-    uint64_t* bar = &bars[i % kStreamStages];
+  int lengths[kStreamStages];
+  auto issue = [&](int st) {
+    if (next == member || (next >= blocks0 && next - share < blocks0)) point(next < blocks0);
+    const int n = min(kBlock, left);
+    lengths[st] = n;
+    Stage<D>& s = ring[st];
+    uint64_t* bar = &bars[st];
     if (lane == 0) {
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(bar)), "r"((uint32_t)(2 * n * D))
                    : "memory");
-      copy_bulk(s.k, (pre ? a.prefix_key_codes : a.key_codes) + at * D, n * D, bar);
-      copy_bulk(s.v, (pre ? a.prefix_value_codes : a.value_codes) + at * D, n * D, bar);
+      copy_bulk(s.k, kp, n * D, bar);
+      copy_bulk(s.v, vp, n * D, bar);
     }
-    const int p = min(lane, n - 1), bytes = lane < n ? 4 : 0;  // zeros behind the last position
+    const bool in = lane < n;  // zeros behind the last position
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(&s.ks[lane])),
-                 "l"((pre ? a.prefix_key_scales : a.key_scales) + at + p), "r"(bytes)
+                 "l"(in ? ksp : ksp - lane), "r"(in ? 4 : 0)
                  : "memory");
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared_address(&s.vs[lane])),
-                 "l"((pre ? a.prefix_value_scales : a.value_scales) + at + p), "r"(bytes)
+                 "l"(in ? vsp : vsp - lane), "r"(in ? 4 : 0)
                  : "memory");
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(shared_address(bar)) : "memory");
+    next += share;
+    left -= share * kBlock;
+    kp += share * kBlock * D;
+    vp += share * kBlock * D;
+    ksp += share * kBlock;
+    vsp += share * kBlock;
   };
 #pragma unroll
-  for (int i = 0; i < kStreamStages; i++)
-    if (i < mine) issue(i);
-  load_queries<T, D, NG>(r, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, scale, lane);
+  for (int st = 0; st < kStreamStages; st++)
+    if (st < mine) issue(st);
+  begin_rows<T, D, NG>(r, queries, scale, lane);
   int i = 0;
 #pragma unroll 1
-  for (; i < mine; i++) {
-    ok = __all_sync(0xffffffffu, barrier_wait(&bars[i % kStreamStages], (uint32_t)(i / kStreamStages) & 1));
+  for (uint32_t parity = 0; i < mine; parity ^= 1) {
+#pragma unroll
+    for (int st = 0; st < kStreamStages; st++) {
+      if (i >= mine) break;
+      ok = barrier_wait_warp(&bars[st], parity);
+      if (!ok) break;
+      attend_block<D, NG>(r, ring[st], lengths[st], lane);
+      __syncwarp();  // every lane has read the stage
+      if (i + kStreamStages < mine) issue(st);
+      i++;
+    }
     if (!ok) break;
-    attend_block<D, NG>(r, ring[i % kStreamStages], length(i), lane);
-    __syncwarp();  // every lane has read the stage
-    if (i + kStreamStages < mine) issue(i + kStreamStages);
   }
   if (!ok) {  // copies may still be landing: give them their time before the memory is let go
     for (int k = i; k < min(mine, i + kStreamStages); k++) barrier_wait(&bars[k % kStreamStages], (uint32_t)(k / kStreamStages) & 1);
@@ -404,7 +447,7 @@ __global__ void __maxnreg__(D * NG == 64 ? 72 : D * NG == 128 ? 96 : 152)
     }
     // the prefix's parts, where no split waits for the merge kernel: each warp of the unit takes some
 #pragma unroll 2
-    for (int p = plan.splits == 1 && hh < heads ? warp : plan.parts; p < plan.parts; p += share)
+    for (int p = plan.splits == 1 && hh < heads ? member : plan.parts; p < plan.parts; p += share)
       add_part<N>(parts, p * parts.per_part + at, m, l, o, g);
     if (share > 1) {
       if (g == 0) {
@@ -420,7 +463,7 @@ __global__ void __maxnreg__(D * NG == 64 ? 72 : D * NG == 128 ? 96 : 152)
   }
   if (share == 1) return;
   __syncthreads();
-  if (warp != 0) return;
+  if (member != 0) return;
 #pragma unroll
   for (int q = 0; q < NG; q++) {
     const int hh = 4 * q + c;
@@ -512,8 +555,16 @@ StreamPlan plan_for(const needle_prefix_attention& a) {
   }
   const int64_t units = int64_t(a.rows) * a.kv_heads * p.groups;
   const int64_t positions = int64_t(p.parts ? 0 : a.prefix_length) + a.capacity;
+  p.group = group;
   p.warps = 1;
-  while (p.warps < kStreamWarps && units * p.warps < kFullWarps && positions > int64_t(p.warps) * kBlock) p.warps *= 2;
+  while (p.warps < kStreamWarps && units * p.warps < kFullWarps && positions > int64_t(p.warps) * kBlock) {
+    p.warps *= 2;
+    p.warps_log2++;
+  }
+  p.together = 1;
+  if (p.warps == 1)
+    for (int k = 2; k <= kStreamWarps; k++)
+      if (a.kv_heads * p.groups % k == 0 && units / k >= kFullWarps) p.together = k;
   // the longest splits that still give every SM its warps
   int64_t splits = 1;
   if (p.warps == kStreamWarps) splits = std::max<int64_t>(1, std::min(kFullWarps / (units * p.warps), positions / kLeastSplit));
@@ -542,14 +593,15 @@ cudaError_t launch_attention(const needle_prefix_attention& a, const StreamPlan&
     const cudaError_t e = launch_attend_prefix(a, parts, p.parts, p.part_len, scale, wait_words, s);
     if (e != cudaSuccess) return e;
   }
-  const int64_t units = int64_t(a.rows) * a.kv_heads * p.groups;
-  const size_t smem = sizeof(Stage<D>) * kStreamStages * p.warps;
+  const int warps = p.warps * p.together;
+  const size_t smem = sizeof(Stage<D>) * kStreamStages * warps;
+  const dim3 grid(a.rows, a.kv_heads * p.groups / p.together, p.splits);
   static_assert(sizeof(Stage<D>) * kStreamStages >= size_t(kGroupHeads) * D * 4, "the merge takes the rings' place");
   auto go = [&](auto kernel) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  int(sizeof(Stage<D>) * kStreamStages * kStreamWarps));
     if (err != cudaSuccess) return err;
-    kernel<<<dim3((unsigned)units, p.splits), p.warps * 32, smem, s>>>(a, p, parts, scale, wait_words);
+    kernel<<<grid, warps * 32, smem, s>>>(a, p, parts, scale, wait_words);
     return cudaGetLastError();
   };
   cudaError_t e = a.heads / a.kv_heads <= 4 ? go(k_attend_stream<T, D, 1>) : go(k_attend_stream<T, D, 2>);
