@@ -341,7 +341,10 @@ __global__ void __maxnreg__(D == 64 ? (NG == 1 ? 80 : 112) : (NG == 1 ? 144 : 16
   RawQueries<T, D, NG> queries;  // ahead of everything that waits for memory
   load_queries<T, D, NG>(queries, static_cast<const T*>(a.q) + row * a.q_stride + head * D, heads, lane);
   const int slot = a.slots ? __ldg(a.slots + row) : row, count = min(max(__ldg(a.counts + row), 0), a.capacity);
-  if (slot < 0 || slot >= a.slot_count) return;
+  if (slot < 0 || slot >= a.slot_count) {
+    if (plan.parts > 0) wait_for_prior();  // no CTA, so not this kernel either, ends before the prefix kernel
+    return;
+  }
   Rows<D, NG> r;
   bool ok = true;
   Stage<D>* ring = reinterpret_cast<Stage<D>*>(raw) + warp * kStreamStages;
@@ -423,6 +426,7 @@ __global__ void __maxnreg__(D == 64 ? (NG == 1 ? 80 : 112) : (NG == 1 ? 144 : 16
     for (int k = i; k < min(mine, i + kStreamStages); k++) barrier_wait(&bars[k % kStreamStages], (uint32_t)(k / kStreamStages) & 1);
     if (lane == 0) report_wait_timeout(wait_words, kWaitAttention);
   }
+  if (plan.parts > 0) wait_for_prior();  // k_attend_prefix, beside which this kernel was started
   float* merge_o = reinterpret_cast<float*>(raw);  // [warps][4 NG][D], where the rings were
   const int64_t first = (int64_t)row * a.heads + head;
   if (share > 1) __syncthreads();
@@ -601,8 +605,18 @@ cudaError_t launch_attention(const needle_prefix_attention& a, const StreamPlan&
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  int(sizeof(Stage<D>) * kStreamStages * kStreamWarps));
     if (err != cudaSuccess) return err;
-    kernel<<<grid, warps * 32, smem, s>>>(a, p, parts, scale, wait_words);
-    return cudaGetLastError();
+    // beside the prefix kernel, whose results are waited for at the end
+    cudaLaunchAttribute overlap{};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(warps * 32);
+    config.dynamicSmemBytes = smem;
+    config.stream = s;
+    config.attrs = &overlap;
+    config.numAttrs = p.parts > 0 ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, a, p, parts, scale, wait_words);
   };
   cudaError_t e = a.heads / a.kv_heads <= 4 ? go(k_attend_stream<T, D, 1>) : go(k_attend_stream<T, D, 2>);
   if (e != cudaSuccess || p.splits == 1) return e;

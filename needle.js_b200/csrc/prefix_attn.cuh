@@ -94,6 +94,11 @@ __device__ __forceinline__ bool barrier_wait_warp(uint64_t* b, uint32_t parity) 
   }
 }
 
+// The next kernel of the stream may be started (when it was launched to overlap) / the kernel before has ended
+// and its writes are visible.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ float power2f(float v) {  // 2^v, relative error 2^-22, 0 below 2^-126
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));

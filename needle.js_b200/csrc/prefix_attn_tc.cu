@@ -159,6 +159,45 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const uint32_t sm = (shared_address(raw) + 1023u) & ~1023u;
   unsigned char* smem = raw + (sm - shared_address(raw));
 
+  launch_dependents();
+  // the softmax warps' rows (thread = packed row) and, before anything is waited for, their queries: kLanes
+  // lanes take a row, 8 dimensions each
+  constexpr int V = 16 / sizeof(T), kLanes = D / 8, kAtOnce = 32 / kLanes, kSteps = 32 / kAtOnce, kBatch = 8;
+  const int t = warp / kTileWarps, quarter = warp & 3;
+  const uint32_t i_row = (uint32_t)first + t * 128 + quarter * 32 + lane;
+  const uint32_t row = i_row / (uint32_t)group, head = (uint32_t)(h * group) + (i_row - row * group);
+  const int d0 = lane % kLanes * 8;
+  bool live = false;
+  int64_t offset = -1;
+  Vec<T, V> in[kBatch][8 / V];
+  float inverse = 0.0f;
+  const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_stride * (int64_t)sizeof(T) & 15) == 0;
+  auto load = [&](int b) {
+#pragma unroll
+    for (int k = 0; k < kBatch; k++) {
+      const int64_t at = __shfl_sync(0xffffffffu, offset, (b + k) * kAtOnce + lane / kLanes);
+      const T* q = static_cast<const T*>(a.q) + at + d0;
+#pragma unroll
+      for (int p = 0; p < 8 / V; p++) {
+        in[k][p] = Vec<T, V>{};
+        if (at >= 0) {
+          if (vec) {
+            in[k][p] = *reinterpret_cast<const Vec<T, V>*>(q + p * V);
+          } else {
+#pragma unroll
+            for (int e = 0; e < V; e++) in[k][p].v[e] = q[p * V + e];
+          }
+        }
+      }
+    }
+  };
+  if (warp < kPrefixSoftmaxWarps && t < tiles_m) {
+    const int slot = i_row < (uint32_t)packed ? (a.slots ? __ldg(a.slots + row) : (int)row) : -1;
+    live = slot >= 0 && slot < a.slot_count;
+    // rows of other slots than the call's are read too (they are in the buffer), and left out at the end
+    offset = i_row < (uint32_t)packed ? row * a.q_stride + head * D : -1;
+    load(0);
+  }
   if (tid == 0) {
     barrier_init(&q_full, kTileWarps * tiles_m);
     for (int t = 0; t < 2; t++) {
@@ -317,51 +356,31 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     if (!ok) atomicExch(&failed, 1);
   } else {
     // ---- softmax: thread = packed row
-    const int t = warp / kTileWarps, quarter = warp & 3, r = quarter * 32 + lane;
     if (t < tiles_m) {
-      const int64_t i = first + t * 128 + r;
-      const int64_t row = i / group, head = (int64_t)h * group + i % group;
-      const int slot = i < packed ? (a.slots ? a.slots[row] : (int)row) : -1;
-      const bool live = slot >= 0 && slot < a.slot_count;
-      // the warp's 32 queries, each scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared
-      // memory: kLanes lanes take a row, 16 bytes each
-      constexpr int V = 16 / sizeof(T), kLanes = D / V, kAtOnce = 32 / kLanes, kBatch = 8;
-      const int64_t offset = live ? row * a.q_stride + head * D : -1;
-      const bool vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.q_stride * (int64_t)sizeof(T) & 15) == 0;
-      const int d0 = lane % kLanes * V;
-      float inverse = 0.0f;
-#pragma unroll 1
-      for (int b = 0; b < kLanes; b += kBatch) {
-        Vec<T, V> in[kBatch];
+      // the warp's 32 queries, each scaled to a largest magnitude in [2^10, 2^11), as fp16 part(s) in shared memory
+#pragma unroll
+      for (int b = 0; b < kSteps; b += kBatch) {
+        if (b > 0) load(b);
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
-          const int64_t at = __shfl_sync(0xffffffffu, offset, (b + k) * kAtOnce + lane / kLanes);
-          const T* q = static_cast<const T*>(a.q) + at + d0;
-          if (at < 0) {
-            in[k] = Vec<T, V>{};
-          } else if (vec) {
-            in[k] = *reinterpret_cast<const Vec<T, V>*>(q);
-          } else {
+          const int r0 = (b + k) * kAtOnce, rr = r0 + lane / kLanes;
+          float x[8], top = 0.0f;
 #pragma unroll
-            for (int e = 0; e < V; e++) in[k].v[e] = q[e];
+          for (int e = 0; e < 8; e++) {
+            x[e] = to_f32(in[k][e / V].v[e % V]);
+            top = fmaxf(top, fabsf(x[e]));
           }
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; k++) {
-          float top = 0.0f;
-#pragma unroll
-          for (int e = 0; e < V; e++) top = fmaxf(top, fabsf(to_f32(in[k].v[e])));
 #pragma unroll
           for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          const int e10 = min(max(exponent_of(top), -110), 110), r0 = (b + k) * kAtOnce, rr = r0 + lane / kLanes;
+          const int e10 = min(max(exponent_of(top), -110), 110);
           const float up = power2(10 - e10);
-          alignas(16) uint32_t heads[V / 2], tails[V / 2];
+          uint32_t heads[4], tails[4];
 #pragma unroll
-          for (int e = 0; e < V / 2; e++) split_f16(to_f32(in[k].v[2 * e]) * up, to_f32(in[k].v[2 * e + 1]) * up, heads[e], tails[e]);
-          unsigned char* to = smem + t * P::kQTile + (d0 >> 6) * P::kQHalf + swizzled(quarter * 32 + rr, (d0 & 63) >> 3) + (d0 & 7) * 2;
-          *reinterpret_cast<Vec<uint32_t, V / 2>*>(to) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(heads);
+          for (int e = 0; e < 4; e++) split_f16(x[2 * e] * up, x[2 * e + 1] * up, heads[e], tails[e]);
+          unsigned char* to = smem + t * P::kQTile + (d0 >> 6) * P::kQHalf + swizzled(quarter * 32 + rr, (d0 & 63) >> 3);
+          *reinterpret_cast<uint4*>(to) = make_uint4(heads[0], heads[1], heads[2], heads[3]);
           if constexpr (SPLIT)
-            *reinterpret_cast<Vec<uint32_t, V / 2>*>(to + P::kHalves * P::kQHalf) = *reinterpret_cast<const Vec<uint32_t, V / 2>*>(tails);
+            *reinterpret_cast<uint4*>(to + P::kHalves * P::kQHalf) = make_uint4(tails[0], tails[1], tails[2], tails[3]);
           // the row's own lane keeps what undoes the scaling
           const float back = __shfl_sync(0xffffffffu, power2(e10 - 10) * (scale * kLog2e), (lane - r0) * kLanes & 31);
           if (lane >= r0 && lane < r0 + kAtOnce) inverse = back;
@@ -459,7 +478,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       tensor_fence_after();
       const bool bad = !ok || !done || *(volatile int*)&failed != 0;
       if (bad && lane == 0) report_wait_timeout(wait_words, kWaitAttention);
-      const int64_t part = blockIdx.z * parts.per_part + row * a.heads + head;
+      const int64_t part = blockIdx.z * parts.per_part + (int64_t)row * a.heads + head;
       if (live) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l);
       // 32 columns at a time through shared memory (the operands are done with), so that rows are written
       // 128 bytes at once
