@@ -13,8 +13,17 @@
 // Queries in binary32 are computed the same way; 16-bit queries in binary32, whose error (2^-23) is far
 // below the rounding to 16 bits (2^-11, 2^-8).
 //
-// One CTA per token: its threads first compute the token's cosines and sines (binary64, shared by all
-// heads), then each warp takes whole head rows, lanes holding consecutive elements.
+// A warp reads kRows head rows at once, 16 bytes a lane, and works on one token (or a part of one, where there are
+// few): it computes the token's angles in binary64, leaves them in shared memory, and walks over the keys, the
+// values and the queries.  Bytes bound the operator (every row is read and written once), then instructions:
+// 88 for 256 query elements, about 250 for 256 key elements, of which the binary64 rotation and its conversions
+// are the larger part.  What paid, at 8191 tokens of 32 / 8 heads of 128 in bf16 (217 MB): 131 us with a CTA a
+// token and 8-byte accesses; 100 us with a warp a token; 64 us with the exact division only for quotients next to
+// a border, in a loop over them (it was inlined for every element and held registers), and accesses whose
+// width is known at compile time; 61.6 us = 3.5 TB/s, 54% of a copy's rate, with loads issued at the start of
+// each kind rather than all before the angles (fewer registers held).  4 resident CTAs of 64 registers: 3 take
+// 64 us, 5 take 72 us (spills).  4096 tokens of 8 / 4 heads of 64 in binary32 (36 MB): 13.4 us, 4 tokens: 3.3 us.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -25,187 +34,325 @@ namespace needle {
 namespace {
 
 constexpr int kRopeThreads = 256;
-constexpr int kMaxPairs = 64;  // rotated pairs of a head of 128
+constexpr int kRopeWarps = kRopeThreads / 32;
+constexpr int kMaxPairs = 64;        // rotated pairs of a head of 128
+constexpr int kRopeFill = 148 * 3;   // CTAs that keep the GPU busy (148 * 6: as fast; 148 * 12: 4096 tokens 14 -> 19 us)
+constexpr int kRopeResident = 4;     // CTAs of an SM
+constexpr int kQueriesAhead = 4;     // query loads of a lane in flight
+
+// What a kernel is built for, E being the elements of a lane: pairs (2i, 2i + 1), rotary_dim a multiple of E, and
+// 16-byte accesses; pairs (i, i + half), half a multiple of E (a lane's partners are then one lane), and 16-byte
+// accesses; or any pairs and any alignment.
+enum Form { kInterleaved, kHalves, kAny };
 
 struct RopeArgs {
   needle_rope_append a;
+  int32_t parts;  // warps that share a token: 1, 2, 4 or 8
   double inverse[kMaxPairs];
 };
 
-// code of x at binary64 scale s = top / 127: the quotient is first taken in binary32 (error below
-// 2^-15 of a code step at |code| <= 127), and only quotients that near a border are divided in binary64.
-__device__ __forceinline__ int quantise(float x, float inverse, double scale) {
-  const float t = x * inverse;
-  float r = rintf(t);
-  if (!(fabsf(t - r) < 0.4999f)) r = (float)rint((double)x / scale);
-  return r != r ? 0 : (int)fminf(fmaxf(r, -127.0f), 127.0f);
-}
+// a c - b s; binary64 rounds every step as the engine's JavaScript does.
+__device__ __forceinline__ float turned(double a, double c, double b, double s) { return (float)(a * c - b * s); }
+__device__ __forceinline__ float turned(float a, float c, float b, float s) { return fmaf(a, c, -b * s); }
 
-template <class T, int EPL>
-__device__ __forceinline__ void load_row(const T* p, int lane, bool vec, float* x) {
-  if (vec) {
-    const Vec<T, EPL> v = *reinterpret_cast<const Vec<T, EPL>*>(p + lane * EPL);
-#pragma unroll
-    for (int i = 0; i < EPL; i++) x[i] = to_f32(v.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < EPL; i++) x[i] = to_f32(p[lane * EPL + i]);
-  }
-}
+// Where pair i's (cosine, sine) lies: lanes whose pairs are 4 or 8 apart meet different banks.
+__device__ __forceinline__ int angle_at(int pair) { return pair ^ (pair >> 3 & 7); }
 
-template <class T, int EPL>
-__device__ __forceinline__ void store_row(T* p, int lane, bool vec, const float* x) {
-  if (vec) {
-    Vec<T, EPL> v;
-#pragma unroll
-    for (int i = 0; i < EPL; i++) v.v[i] = from_f32<T>(x[i]);
-    *reinterpret_cast<Vec<T, EPL>*>(p + lane * EPL) = v;
-  } else {
-#pragma unroll
-    for (int i = 0; i < EPL; i++) p[lane * EPL + i] = from_f32<T>(x[i]);
-  }
-}
+// The norm and rotation of rows of D elements, E of them in each of D / E lanes, in arithmetic A.  Angles and norm
+// factors (1 + s) in binary64 are read from shared memory for every row: in registers they would cost half the
+// resident warps.  Binary32 angles are kept.
+template <class A, int D, int E, int FORM>
+struct Turn {
+  using Angle = typename std::conditional<std::is_same<A, double>::value, double2, float2>::type;
+  static constexpr int kLanes = D / E, kAngles = FORM == kInterleaved ? E / 2 : E;
+  static constexpr bool kKept = std::is_same<A, float>::value && FORM != kAny;
+  const A* factors;     // of this lane
+  const Angle* angles;  // of the token
+  Angle kept[kKept ? kAngles : 1];
+  int sub, half, other, pair0;
+  bool normed, interleaved, first, turns;
 
-// Norm and rotation of one head row (EPL consecutive elements per lane) in arithmetic A.
-template <class A, int EPL>
-__device__ __forceinline__ void turn_row(float* x, const float* norm, const double2* cs, int lane, int rotary,
-                                         bool interleaved) {
-  if (norm) {
-    A sum = 0;
+  __device__ __forceinline__ Turn(bool normed, const A* factors, const Angle* angles, int sub, int rotary, bool interleaved)
+      : factors(factors + sub * E), angles(angles), sub(sub), half(rotary >> 1), normed(normed), interleaved(interleaved) {
+    const int e0 = sub * E;
+    turns = e0 < rotary;
+    first = e0 < half;
+    other = first ? sub + half / E : sub - half / E;
+    pair0 = FORM == kInterleaved ? e0 / 2 : first ? e0 : e0 - half;
+    if constexpr (kKept) {
 #pragma unroll
-    for (int i = 0; i < EPL; i++) sum = fma((A)x[i], (A)x[i], sum);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const A inverse = (A)1 / sqrt(sum / (A)(EPL * 32) + (A)1e-6);
-#pragma unroll
-    for (int i = 0; i < EPL; i++) x[i] = (float)(((A)1 + (A)__ldg(norm + lane * EPL + i)) * (A)x[i] * inverse);
+      for (int i = 0; i < kAngles; i++) kept[i] = turns ? angles[angle_at(pair0 + i)] : Angle{1.0f, 0.0f};
+    }
   }
-  if (interleaved) {
+  __device__ __forceinline__ Angle angle(int i) const {
+    if constexpr (kKept)
+      return kept[i];
+    else
+      return angles[angle_at(pair0 + i)];
+  }
+  static __device__ __forceinline__ void turn_pair(float& x, float& y, const Angle& t) {
+    const A a = (A)x, b = (A)y;
+    x = turned(a, t.x, b, t.y);
+    y = turned(b, t.x, -a, t.y);
+  }
+
+  __device__ __forceinline__ void operator()(float (&x)[E]) const {
+    if (normed) {
+      A sum = 0;
 #pragma unroll
-    for (int i = 0; i < EPL; i += 2) {
-      const int e = lane * EPL + i;
-      if (e < rotary) {
-        const A c = (A)cs[e >> 1].x, s = (A)cs[e >> 1].y, a = (A)x[i], b = (A)x[i + 1];
-        x[i] = (float)(a * c - b * s);
-        x[i + 1] = (float)(b * c + a * s);
+      for (int i = 0; i < E; i++) sum = fma((A)x[i], (A)x[i], sum);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const A inverse = rsqrt(sum * (A)(1.0 / D) + (A)1e-6);
+      constexpr int kPiece = 16 / sizeof(A);
+#pragma unroll
+      for (int i = 0; i < E; i += kPiece) {
+        const Vec<A, kPiece> f = *reinterpret_cast<const Vec<A, kPiece>*>(factors + i);
+#pragma unroll
+        for (int j = 0; j < kPiece; j++) x[i + j] = (float)(f.v[j] * (A)x[i + j] * inverse);
       }
     }
-    return;
-  }
-  // pairs (e, e + half): the partner of a lane's element i is register (i +- half) % EPL of another lane
-  const int half = rotary >> 1, shift = half % EPL;
-  float y[EPL];
+    if (FORM == kInterleaved) {
+      if (turns) {
 #pragma unroll
-  for (int i = 0; i < EPL; i++) {
-    const int e = lane * EPL + i;
-    const int up = ((e + half) / EPL) & 31, down = ((e - half + 32 * EPL) / EPL) & 31;
-    if (shift == 0) {
-      y[i] = __shfl_sync(0xffffffffu, x[i], e < half ? up : down);
-    } else {
-      float from_up = 0.0f, from_down = 0.0f;
-#pragma unroll
-      for (int j = 0; j < EPL; j++) {
-        if ((i + shift) % EPL == j) from_up = x[j];
-        if ((i + EPL - shift) % EPL == j) from_down = x[j];
+        for (int i = 0; i < E; i += 2) turn_pair(x[i], x[i + 1], angle(i / 2));
       }
-      from_up = __shfl_sync(0xffffffffu, from_up, up);
-      from_down = __shfl_sync(0xffffffffu, from_down, down);
-      y[i] = e < half ? from_up : from_down;
+    } else if (FORM == kHalves) {
+      float y[E];
+#pragma unroll
+      for (int i = 0; i < E; i++) y[i] = __shfl_sync(0xffffffffu, x[i], other, kLanes);
+      if (turns) {
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+          const Angle t = angle(i);
+          x[i] = turned((A)x[i], t.x, first ? (A)y[i] : -(A)y[i], t.y);
+        }
+      }
+    } else if (interleaved) {
+#pragma unroll
+      for (int i = 0; i < E; i += 2)
+        if (sub * E + i < 2 * half) turn_pair(x[i], x[i + 1], angles[angle_at((sub * E + i) / 2)]);
+    } else {  // the partner of element i is element (i +- half) % E of a lane that depends on i
+      const int shift = half % E;
+      float y[E];
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        float from_up = 0.0f, from_down = 0.0f;
+#pragma unroll
+        for (int j = 0; j < E; j++) {
+          if ((i + shift) % E == j) from_up = x[j];
+          if ((i + E - shift) % E == j) from_down = x[j];
+        }
+        from_up = __shfl_sync(0xffffffffu, from_up, sub + (i + half) / E, kLanes);
+        from_down = __shfl_sync(0xffffffffu, from_down, sub - (half - i + E - 1) / E, kLanes);
+        y[i] = sub * E + i < half ? from_up : from_down;
+      }
+#pragma unroll
+      for (int i = 0; i < E; i++) {
+        const int e = sub * E + i;
+        if (e < 2 * half) {
+          const Angle t = angles[angle_at(e < half ? e : e - half)];
+          x[i] = turned((A)x[i], t.x, e < half ? (A)y[i] : -(A)y[i], t.y);
+        }
+      }
     }
   }
+};
+
+template <class T, int E, int FORM>
+__device__ __forceinline__ Vec<T, E> load_piece(const T* p) {
+  if constexpr (FORM != kAny) {
+    return *reinterpret_cast<const Vec<T, E>*>(p);
+  } else {
+    Vec<T, E> v;
 #pragma unroll
-  for (int i = 0; i < EPL; i++) {
-    const int e = lane * EPL + i;
-    if (e < rotary) {
-      const bool first = e < half;
-      const double2 t = cs[first ? e : e - half];
-      const A c = (A)t.x, s = (A)t.y;
-      x[i] = (float)(first ? (A)x[i] * c - (A)y[i] * s : (A)x[i] * c + (A)y[i] * s);
-    }
+    for (int i = 0; i < E; i++) v.v[i] = p[i];
+    return v;
   }
 }
 
-template <class T, int EPL>
-__global__ void __launch_bounds__(kRopeThreads) k_rope_append(const __grid_constant__ RopeArgs args, bool q_vec,
-                                                               bool k_vec, bool v_vec, bool qo_vec, bool ko_vec,
-                                                               bool vo_vec) {
-  constexpr int kDimension = EPL * 32;
-  __shared__ double2 cs[kMaxPairs];
+template <class T, int E, int FORM>
+__device__ __forceinline__ void store_piece(T* p, const float (&x)[E]) {
+  Vec<T, E> v;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < E; i++) v.v[i] = x[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x[i], x[i + 1]);
+        v.v[i] = h.x, v.v[i + 1] = h.y;
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[i], x[i + 1]);
+        v.v[i] = h.x, v.v[i + 1] = h.y;
+      }
+    }
+  }
+  if constexpr (FORM != kAny) {
+    *reinterpret_cast<Vec<T, E>*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; i++) p[i] = v.v[i];
+  }
+}
+
+template <class T, int D, int FORM>
+__global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(const __grid_constant__ RopeArgs args) {
+  constexpr int E = 16 / sizeof(T), kLanes = D / E, kRows = 32 / kLanes;
+  constexpr bool kNarrow = sizeof(T) == 2;
+  using Query = typename std::conditional<kNarrow, float, double>::type;
+  using Piece = Vec<T, E>;
+  __shared__ double2 angles[kRopeWarps][kMaxPairs];
+  __shared__ float2 angles32[kNarrow ? kRopeWarps : 1][kMaxPairs];
+  __shared__ alignas(16) double k_factors[D];
+  __shared__ alignas(16) Query q_factors[D];
   const needle_rope_append& a = args.a;
-  const int64_t t = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int pairs = a.rotary_dim >> 1;
-  if (tid < pairs) {
-    double s, c;
-    sincos((double)a.positions[t] * args.inverse[tid], &s, &c);
-    cs[tid] = make_double2(c * a.magnitude, s * a.magnitude);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / kLanes, sub = lane % kLanes;
+  const int parts = args.parts, mine = warp / parts, part = warp % parts;
+  const int64_t token = (int64_t)blockIdx.x * (kRopeWarps / parts) + mine;
+  const bool live = token < a.tokens;
+  const int step = parts * kRows;  // heads a turn
+  // the first head of this warp, of each kind: few heads are spread over the warps
+  const int q0 = part * kRows, k0 = (parts - 1 - part) * kRows, v0 = (part + parts / 2) % parts * kRows;
+  auto load = [&](const void* base, int64_t stride, int head, int heads) {
+    Piece v{};
+    if (head + group < heads)
+      v = load_piece<T, E, FORM>(static_cast<const T*>(base) + token * stride + (int64_t)(head + group) * D + sub * E);
+    return v;
+  };
+  Piece qs[kQueriesAhead], ks[1], vs[1];
+  int64_t at = -1;
+  if (live) {
+    ks[0] = load(a.k, a.k_stride, k0, a.kv_heads);  // on its way while the angles are computed
+    const int slot = a.slots[token], entry = a.entries[token];
+    if (slot >= 0 && slot < a.slot_count && entry >= 0 && entry < a.capacity)
+      at = (int64_t)slot * a.kv_heads * a.capacity + entry;
+    const double position = a.positions[token];
+    for (int i = part * 32 + lane; i < a.rotary_dim >> 1; i += parts * 32) {
+      double s, c;
+      sincos(position * args.inverse[i], &s, &c);
+      c *= a.magnitude, s *= a.magnitude;
+      angles[mine][angle_at(i)] = make_double2(c, s);
+      if constexpr (kNarrow) angles32[mine][angle_at(i)] = make_float2((float)c, (float)s);
+    }
   }
-  const int slot = a.slots[t], entry = a.entries[t];
-  const bool stored = slot >= 0 && slot < a.slot_count && entry >= 0 && entry < a.capacity;
-  __syncthreads();
-  using Query = typename std::conditional<sizeof(T) == 4, double, float>::type;
-  for (int r = tid >> 5; r < a.heads + 2 * a.kv_heads; r += kRopeThreads / 32) {
-    float x[EPL];
-    if (r < a.heads) {
-      load_row<T, EPL>(static_cast<const T*>(a.q) + t * a.q_stride + (int64_t)r * kDimension, lane, q_vec, x);
-      turn_row<Query, EPL>(x, a.q_norm, cs, lane, a.rotary_dim, a.interleaved != 0);
-      store_row<T, EPL>(static_cast<T*>(a.q_out) + t * a.q_out_stride + (int64_t)r * kDimension, lane, qo_vec, x);
-      continue;
-    }
-    const bool key = r < a.heads + a.kv_heads;
-    const int h = r - a.heads - (key ? 0 : a.kv_heads);
-    if (key) {
-      load_row<T, EPL>(static_cast<const T*>(a.k) + t * a.k_stride + (int64_t)h * kDimension, lane, k_vec, x);
-      turn_row<double, EPL>(x, a.k_norm, cs, lane, a.rotary_dim, a.interleaved != 0);
-    } else {
-      load_row<T, EPL>(static_cast<const T*>(a.v) + t * a.v_stride + (int64_t)h * kDimension, lane, v_vec, x);
-    }
+  if (a.k_norm)
+    for (int i = threadIdx.x; i < D; i += kRopeThreads) k_factors[i] = 1.0 + (double)a.k_norm[i];
+  if (a.q_norm)
+    for (int i = threadIdx.x; i < D; i += kRopeThreads) q_factors[i] = (Query)1 + (Query)a.q_norm[i];
+  if (parts > 1 || a.k_norm || a.q_norm)
+    __syncthreads();
+  else
+    __syncwarp();
+  if (!live) return;
+
+  auto keep = [&](float (&x)[E], int head, int8_t* codes, float* scales, void* out, int64_t stride) {
     float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < EPL; i++) top = fmaxf(top, fabsf(x[i]));
+    for (int i = 0; i < E; i++) top = fmaxf(top, fabsf(x[i]));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const double scale = fmax(1e-12, (double)top) * (1.0 / 127.0);
-    const float scale32 = (float)scale, inverse = (float)(1.0 / scale);
-    Vec<int8_t, EPL> code;
-    float value[EPL];
+    const float scale32 = (float)scale, inverse = 1.0f / scale32;
+    // The quotient in binary32 is within 2^-15 of the exact one; adding 1.5 * 2^23 rounds it to an integer,
+    // which the sum's lowest byte holds.  One that near a border between codes, or a NaN, is divided in binary64.
+    constexpr float kRound = 12582912.0f;
+    uint32_t border = 0;
+    float r[E];
 #pragma unroll
-    for (int i = 0; i < EPL; i++) {
-      const int c = quantise(x[i], inverse, scale);
-      code.v[i] = (int8_t)c;
-      value[i] = (float)c * scale32;
+    for (int i = 0; i < E; i++) {
+      const float t = x[i] * inverse;
+      r[i] = t + kRound;
+      border |= !(fabsf(t - (r[i] - kRound)) < 0.4999f) ? 1u << i : 0u;
     }
-    if (stored) {
-      const int64_t row = ((int64_t)slot * a.kv_heads + h) * a.capacity + entry;
-      *reinterpret_cast<Vec<int8_t, EPL>*>((key ? a.key_codes : a.value_codes) + row * kDimension + lane * EPL) = code;
-      if (lane == 0) (key ? a.key_scales : a.value_scales)[row] = scale32;
+    while (border) {
+      const int at = __ffs(border) - 1;
+      border &= border - 1;
+      float value = x[0];
+#pragma unroll
+      for (int i = 1; i < E; i++) value = i == at ? x[i] : value;
+      float code = (float)rint((double)value / scale);
+      code = code != code ? 0.0f : fminf(fmaxf(code, -127.0f), 127.0f);
+#pragma unroll
+      for (int i = 0; i < E; i++) r[i] = i == at ? code + kRound : r[i];
     }
-    void* out = key ? a.k_out : a.v_out;
-    if (out)
-      store_row<T, EPL>(static_cast<T*>(out) + t * (key ? a.k_out_stride : a.v_out_stride) + (int64_t)h * kDimension,
-                        lane, key ? ko_vec : vo_vec, value);
-  }
+    Vec<int8_t, E> code;
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+      code.v[i] = (int8_t)__float_as_int(r[i]);
+      x[i] = (r[i] - kRound) * scale32;
+    }
+    if (head + group >= a.kv_heads) return;
+    if (at >= 0) {
+      const int64_t row = at + (int64_t)(head + group) * a.capacity;
+      *reinterpret_cast<Vec<int8_t, E>*>(codes + row * D + sub * E) = code;
+      if (sub == 0) scales[row] = scale32;
+    }
+    if (out) store_piece<T, E, FORM>(static_cast<T*>(out) + token * stride + (int64_t)(head + group) * D + sub * E, x);
+  };
+  // body(x, head) for the heads of a kind, the loads of the next ones in flight.
+  auto walk = [&](auto& ahead, const void* base, int64_t stride, int head, int heads, auto body) {
+    constexpr int kAhead = sizeof(ahead) / sizeof(Piece);
+    for (;;) {
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) {
+        if (head >= heads) return;
+        float x[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) x[i] = to_f32(ahead[j].v[i]);
+        ahead[j] = load(base, stride, head + kAhead * step, heads);
+        body(x, head);
+        head += step;
+      }
+    }
+  };
+  const Turn<double, D, E, FORM> turn_key(a.k_norm != nullptr, k_factors, angles[mine], sub, a.rotary_dim,
+                                          a.interleaved);
+  walk(ks, a.k, a.k_stride, k0, a.kv_heads, [&](float (&x)[E], int head) {
+    turn_key(x);
+    keep(x, head, a.key_codes, a.key_scales, a.k_out, a.k_out_stride);
+  });
+  vs[0] = load(a.v, a.v_stride, v0, a.kv_heads);
+  walk(vs, a.v, a.v_stride, v0, a.kv_heads, [&](float (&x)[E], int head) {
+    keep(x, head, a.value_codes, a.value_scales, a.v_out, a.v_out_stride);
+  });
+  const auto* query_angles = [&] {
+    if constexpr (kNarrow)
+      return angles32[mine];
+    else
+      return angles[mine];
+  }();
+  const Turn<Query, D, E, FORM> turn_query(a.q_norm != nullptr, q_factors, query_angles, sub, a.rotary_dim, a.interleaved);
+#pragma unroll
+  for (int i = 0; i < kQueriesAhead; i++) qs[i] = load(a.q, a.q_stride, q0 + i * step, a.heads);
+  walk(qs, a.q, a.q_stride, q0, a.heads, [&](float (&x)[E], int head) {
+    turn_query(x);
+    if (head + group < a.heads)
+      store_piece<T, E, FORM>(static_cast<T*>(a.q_out) + token * a.q_out_stride + (int64_t)(head + group) * D + sub * E, x);
+  });
 }
 
-// Whether every head row of a [tokens][*][dim] view can be accessed in a lane's whole share at once.
-bool rows_aligned(const void* p, int64_t stride, int32_t dim, size_t element) {
-  const size_t share = size_t(dim) / 32 * element;
-  return aligned_to(p, share) && (stride * int64_t(element)) % int64_t(share) == 0;
-}
-
-cudaError_t launch_rope(const RopeArgs& args, cudaStream_t s) {
+cudaError_t launch_rope(RopeArgs& args, cudaStream_t s) {
   const needle_rope_append& a = args.a;
+  const int e = int(type_bytes(a.type)), half = a.rotary_dim / 2;
+  // A warp a token computes its angles once and waits for no other; with few tokens, several share one.
+  args.parts = 1;
+  while (args.parts < kRopeWarps && int64_t(a.tokens) * args.parts < int64_t(kRopeFill) * kRopeWarps) args.parts *= 2;
+  auto wide = [&](const void* p, int64_t stride) { return aligned_to(p, 16) && (a.tokens == 1 || stride * e % 16 == 0); };
+  const bool all_wide = wide(a.q, a.q_stride) && wide(a.k, a.k_stride) && wide(a.v, a.v_stride) &&
+                        wide(a.q_out, a.q_out_stride) && wide(a.k_out, a.k_out_stride) && wide(a.v_out, a.v_out_stride);
+  const unsigned grid = unsigned((int64_t(a.tokens) * args.parts + kRopeWarps - 1) / kRopeWarps);
   return with_type(a.type, [&](auto zero) {
     using T = decltype(zero);
-    const size_t e = sizeof(T);
-    auto go = [&](auto kernel) {
-      kernel<<<(unsigned)a.tokens, kRopeThreads, 0, s>>>(
-          args, rows_aligned(a.q, a.q_stride, a.head_dim, e), rows_aligned(a.k, a.k_stride, a.head_dim, e),
-          rows_aligned(a.v, a.v_stride, a.head_dim, e), rows_aligned(a.q_out, a.q_out_stride, a.head_dim, e),
-          rows_aligned(a.k_out, a.k_out_stride, a.head_dim, e), rows_aligned(a.v_out, a.v_out_stride, a.head_dim, e));
+    auto go = [&](auto* interleaved, auto* halves, auto* any) {
+      auto* kernel = !all_wide || (a.interleaved ? 2 : 1) * half % (16 / e) != 0 ? any : a.interleaved ? interleaved : halves;
+      kernel<<<grid, kRopeThreads, 0, s>>>(args);
       return cudaGetLastError();
     };
-    return a.head_dim == 64 ? go(k_rope_append<T, 2>) : go(k_rope_append<T, 4>);
+    return a.head_dim == 64
+               ? go(k_rope_append<T, 64, kInterleaved>, k_rope_append<T, 64, kHalves>, k_rope_append<T, 64, kAny>)
+               : go(k_rope_append<T, 128, kInterleaved>, k_rope_append<T, 128, kHalves>, k_rope_append<T, 128, kAny>);
   });
 }
 
