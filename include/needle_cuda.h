@@ -445,7 +445,7 @@ typedef struct needle_logits_rules {
   const int32_t* bias_counts;     /* [rows] */
   const uint32_t* masks;          /* [mask_count][ceil(vocab / 32)] */
   const int32_t* mask_slots;      /* [rows] */
-  int32_t mask_count, type, rows /* at most 65535 */, vocab;
+  int32_t mask_count, type, rows /* at most 65535 */, vocab /* at most 2^30 */;
 } needle_logits_rules;
 
 /* The ruled logits, rounded to `type`, rows out_stride elements apart; out may be logits (same stride). */
@@ -458,17 +458,19 @@ int needle_cuda_logits_rules_dev(const needle_logits_rules* args, void* out, int
 int needle_cuda_logits_select_dev(const needle_logits_rules* args, int32_t* ids, float* log_probabilities, void* stream);
 
 /* ---- Bounded device waits ----
- * The kernels that wait on asynchronous copies or barriers -- the fast attention, the table matvec and
- * the tensor-core matvec -- give up after 2 s instead of spinning forever.  The outputs of that call
- * are then NaN, and the kernel records its kind in the device's wait-status word (pinned host memory:
- * readable without synchronising).  The next needle_cuda_cq_matvec_dev_fast or
- * needle_cuda_attention_dev_fast call on that device returns BACKEND_UNAVAILABLE, naming the kernels,
- * and clears the word.  (The reference's GPU path is WebGPU, whose device loss the browser reports;
+ * The kernels that wait on asynchronous copies or barriers -- the fast attention, the table matvec,
+ * the tensor-core matvec, the prefix attention and the logits operators -- give up after 2 s instead of
+ * spinning forever.  The outputs of that call are then NaN (a selection's log probability; its id is not
+ * to be used), and the kernel records its kind in the device's wait-status word (pinned host memory:
+ * readable without synchronising).  The next needle_cuda_cq_matvec_dev_fast,
+ * needle_cuda_attention_dev_fast, needle_cuda_prefix_attention_dev or needle_cuda_logits_*_dev call on
+ * that device returns BACKEND_UNAVAILABLE, naming the kernels, and clears the word.  (The reference's GPU path is WebGPU, whose device loss the browser reports;
  * these statuses play that part.) */
-#define NEEDLE_WAIT_ATTENTION 1u   /* k_attention_fast_mma */
+#define NEEDLE_WAIT_ATTENTION 1u   /* k_attention_fast_mma, k_attend_prefix, k_attend_stream */
 #define NEEDLE_WAIT_TABLE_GEMV 2u  /* k_cq_gemv_table */
 #define NEEDLE_WAIT_TENSOR_GEMM 4u /* k_cq_gemm_tc */
 #define NEEDLE_WAIT_SELFTEST 8u    /* needle_cuda_wait_selftest */
+#define NEEDLE_WAIT_LOGITS 16u     /* k_logits_rules, k_logits_select */
 
 /* The wait-status bits of `device` (NEEDLE_WAIT_*) through *kinds; clear = 1 resets them. */
 int needle_cuda_wait_status(int32_t device, uint32_t* kinds, int32_t clear);

@@ -177,7 +177,14 @@ __device__ __forceinline__ double round32_add(double v) {
 // after a time limit; it then records its kind in the library's wait-status words of the device
 // (mapped pinned host memory, so the host reads them without synchronising) and its outputs of
 // that call are NaN.  The next operator call on the device reports BACKEND_UNAVAILABLE.
-enum WaitKind { kWaitAttention = 0, kWaitTableGemv = 1, kWaitTensorGemm = 2, kWaitSelftest = 3, kWaitKinds = 4 };
+enum WaitKind {
+  kWaitAttention = 0,
+  kWaitTableGemv = 1,
+  kWaitTensorGemm = 2,
+  kWaitSelftest = 3,
+  kWaitLogits = 4,
+  kWaitKinds = 5
+};
 
 __device__ __forceinline__ void report_wait_timeout(uint32_t* words, int kind) {
   if (words) *reinterpret_cast<volatile uint32_t*>(words + kind) = 1u;

@@ -7,13 +7,26 @@
 //   x = x + bias;  ids the mask leaves out: x = -inf       (every step rounded to binary32)
 //   id = argmax x, the lowest on ties;  log p = l[id] - max l - log sum exp(l - max l)
 //
-// A CTA takes a chunk of 16 ids per thread of one row, its logits held in registers from first to last,
-// so a row is read once.  What the rules touch is sparse: per chunk, bitmaps in shared memory say which
-// ids are seen, biased and allowed, and a table has counts and bias positions, its entries cleared one by
-// one for the ids that occur.  The stream over the chunk knows only the mask; ids with a rule are left to
-// the threads that hold them in their lists, which fetch those logits again.  All loads that depend on nothing but the row (logits, lengths, the first ids of the
-// lists) are issued before the first barrier.
+// A row is read once.  What the rules touch is sparse, so the stream over a row knows only one bit an id:
+// "free", allowed by the mask and without a rule.  The ids with a rule (history, biases) go into a hash table in
+// shared memory, which counts them and keeps their last bias; its entries are ruled one by one from a second,
+// gathered read of their logits.  CTAs of four warps take parts of rows (at most kPartIds ids; several CTAs or
+// one a row as the batch needs), one after another, and build the table for each.  Every warp streams its slice of
+// a part through a ring of its own in shared memory, filled by bulk copies that run on over the ends of parts
+// and rows: the copies never pause, and no barrier is needed for them.
+//
+// Bytes bound the stream, the lists' chains of dependent accesses the rest.  Without rules, 512 rows of 50001 bf16 ids
+// (102 MB) take 17 us, a copy's rate; with histories of up to 1000 ids, 50 biases and masks 42 us (2.4 TB/s of
+// logits).  Select: 4096 rows of 8192 binary32 ids with histories of 256: 61 us (2.2 TB/s), 37 us without rules;
+// 200 rows of 128000 fp16 ids with histories of 2000: 46 us (1.1 TB/s; each of a row's two CTAs builds a table).
+// Measured beside it: chunks of a row in registers, direct tables of counts instead of the hash, one CTA a chunk:
+// 47, 72, 63 us; the hash twice as large as its list (5/4: 50, 66, 55 us, probes; 4 times: 71, 66, 129 us, fewer
+// CTAs resident); one warp a row: 110 us for the 4096 rows (too few warps hide the lists' latency); parts of 32 KB
+// in shared memory with the lists ruled there, 8 warps: 51, 81, 85 us (every warp repeats a part's fixed work).
 #include <cooperative_groups.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "serving.cuh"
 
@@ -23,39 +36,54 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kPerThread = 16;
-constexpr int kRulesThreads = 256;   // chunks of 4096: eight CTAs an SM
-constexpr int kSelectThreads = 512;  // chunks of 8192: the engine's vocabulary in one CTA
-constexpr int kListIds = 4;          // history ids of a thread kept in registers
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnits = 4;                        // 16-byte units of a thread in a step of the stream
+constexpr int kStages = 2;                       // steps of a warp's ring
+constexpr int kSliceBytes = 32 * kUnits * 16;    // of a warp in a step
+constexpr int kPartIds = 65536;                  // most ids of a part: 8 KB of bits
+constexpr int kListIds = 2;                      // list ids of a thread loaded at once
+constexpr int kMostEntries = 4096;               // hash entries of a part; a part of as many ids never has more
 
-// A chunk's tables; count and bias (of THREADS * kPerThread entries each) only where a rule needs them.
-template <int THREADS>
-struct Tables {
-  static constexpr int kChunk = THREADS * kPerThread, kWords = kChunk / 32, kWarps = THREADS / 32;
-  uint32_t seen[kWords], biased[kWords], allowed[kWords];
-  // one entry per warp, then the CTA's
-  float top[kWarps], sum[kWarps];
-  uint32_t key[kWarps], id[kWarps], lowest[kWarps];
-  float cta_top, cta_sum;
-  uint32_t cta_key, cta_id, cta_lowest;
+__host__ __device__ constexpr int step_ids(size_t element) { return kWarps * kSliceBytes / int(element); }
+// CTAs of an SM by their registers: a thread holds 16 binary32 logits of a step, or 32 of 16 bits.
+__host__ __device__ constexpr int resident(size_t element) { return element == 4 ? 6 : 4; }
+
+// The hash table of a part's ids with a rule.  word: bit 31 the mask allows the id, bit 0 it is in the prompt,
+// bits 1..30 how often it was answered.
+struct Table {
+  uint32_t *key, *word, *bias;  // key: id + 1, 0 for a free slot; bias: 1 + position of the id's last bias
+  uint32_t* free;               // bit per id of the part
+  int slots;                    // a multiple of 4, more than the part can have entries
 };
 
-template <int THREADS>
-__host__ __device__ constexpr size_t tables_bytes() {
-  return (sizeof(Tables<THREADS>) + 15) / 16 * 16;
-}
-
-template <int THREADS>
-size_t smem_bytes(const needle_logits_rules& a) {
-  const size_t each = size_t(THREADS) * kPerThread * 4;
-  return tables_bytes<THREADS>() + (a.history ? each : 0) + (a.bias_ids ? each : 0);
-}
+// How a call is cut (plan_for).
+struct LogitsPlan {
+  int part;   // ids of a part (a multiple of a step's)
+  int parts;  // parts of a row
+  int slots;  // of the hash table; 0: no lists
+};
 
 // Order-preserving key of a binary32 value that is not NaN (-0 as +0); 0 is below every key.
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+
+constexpr float kLog2eL = 1.4426950408889634f;
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float exp2_of(float v) {  // 2^v, relative error 2^-22
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float exp_below(float v) { return exp2_of(v * kLog2eL); }  // e^v, v <= 0
 
 // First id (possibly below 0) of 16-byte unit 0 of the row: rows that do not start on a 16-byte
 // boundary are taken from the boundary before them, with the ids outside the row left out.
@@ -64,23 +92,30 @@ __device__ __forceinline__ int row_offset(const T* row) {
   return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
 }
 
-// Loads the unit at id e (VEC ids); ids outside [0, vocab) become -inf.
+// Ids of a unit whose bit is not set become -inf.
+template <int VEC>
+__device__ __forceinline__ void keep_free(Vec<float, VEC>& v, uint32_t free) {
+#pragma unroll
+  for (int i = 0; i < VEC; i++)
+    if (!(free & (1u << i))) v.v[i] = -INFINITY;
+}
 template <class T, int VEC>
-__device__ __forceinline__ void load_unit(const T* row, int64_t e, int vocab, float* x) {
-  if (e >= 0 && e + VEC <= vocab) {
-    const Vec<T, VEC> v = *reinterpret_cast<const Vec<T, VEC>*>(row + e);
+__device__ __forceinline__ void keep_free(Vec<T, VEC>& v, uint32_t free) {
+  static_assert(sizeof(T) == 2, "two ids a word");
+  const uint32_t low = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf twice
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  free &= (1u << VEC) - 1u;
 #pragma unroll
-    for (int i = 0; i < VEC; i++) x[i] = to_f32(v.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; i++) x[i] = e + i >= 0 && e + i < vocab ? to_f32(row[e + i]) : -INFINITY;
+  for (int i = 0; i < VEC / 2; i++) {
+    const uint32_t b = free >> (2 * i), keep = ((b | (b << 15)) & 0x00010001u) * 0xffffu;  // bits 0, 1 as two halves
+    w[i] = (w[i] & keep) | (low & ~keep);
   }
 }
 
 // What the rules of a row need from memory, loaded ahead.
 struct RowRules {
   float repetition, frequency, presence;
-  int64_t length, prompt, biases;
+  int length, prompt, biases;
   const int32_t *history, *bias_ids;
   const float* bias_values;
   const uint32_t* mask;  // NULL: every id is allowed, or none (`none`)
@@ -92,329 +127,540 @@ __device__ __forceinline__ RowRules row_rules(const needle_logits_rules& a, int6
   r.repetition = a.history && a.repetition ? __ldg(a.repetition + row) : 1.0f;
   r.frequency = a.history && a.frequency ? __ldg(a.frequency + row) : 0.0f;
   r.presence = a.history && a.presence ? __ldg(a.presence + row) : 0.0f;
-  r.length = a.history ? min((int64_t)max(__ldg(a.history_lengths + row), 0), a.history_stride) : 0;
+  r.length = a.history ? (int)min((int64_t)max(__ldg(a.history_lengths + row), 0), a.history_stride) : 0;
   r.prompt = a.history && a.prompt_lengths ? __ldg(a.prompt_lengths + row) : 0;
-  r.biases = a.bias_ids ? min((int64_t)max(__ldg(a.bias_counts + row), 0), a.bias_stride) : 0;
+  r.biases = a.bias_ids ? (int)min((int64_t)max(__ldg(a.bias_counts + row), 0), a.bias_stride) : 0;
   r.history = a.history + row * a.history_stride;
   r.bias_ids = a.bias_ids + row * a.bias_stride;
   r.bias_values = a.bias_values + row * a.bias_stride;
   const int slot = a.masks ? __ldg(a.mask_slots + row) : -1;
-  r.none = slot >= a.mask_count && a.masks;  // a slot that does not exist
+  r.none = a.masks && slot >= a.mask_count;  // a slot that does not exist
   r.mask = slot >= 0 && !r.none ? a.masks + (int64_t)slot * ((a.vocab + 31) >> 5) : nullptr;
   return r;
 }
 
-// A thread's list entries: places in the chunk (or -1) of its first history ids and its first bias.
-struct ListPlaces {
-  int history[kListIds], bias;
-};
-
-// Place of an id in the chunk from `low` on, or -1.
-template <int THREADS>
-__device__ __forceinline__ int place_of(int32_t id, int vocab, int64_t low) {
-  const int64_t p = (int64_t)id - low;
-  return id >= 0 && id < vocab && p >= 0 && p < Tables<THREADS>::kChunk ? (int)p : -1;
+// Slot of an id of the part (claimed for it when it has none yet).
+__device__ __forceinline__ int slot_of(const Table& t, int id, int low) {
+  const uint32_t key = (uint32_t)id + 1u;
+  uint32_t s = __umulhi((uint32_t)id * 2654435761u, (uint32_t)t.slots);  // multiplicative hashing
+  for (;;) {
+    const uint32_t k = atomicCAS(&t.key[s], 0u, key);
+    if (k == 0u) {  // this thread's: the id leaves the stream
+      const int p = id - low;
+      const uint32_t bit = 1u << (p & 31);
+      if (atomicAnd(&t.free[p >> 5], ~bit) & bit) atomicOr(&t.word[s], 0x80000000u);
+      return (int)s;
+    }
+    if (k == key) return (int)s;
+    if (++s == (uint32_t)t.slots) s = 0;  // there are more slots than ids, so this ends
+  }
 }
 
-// Fills the bitmaps and tables of ids [low, low + kChunk).  Begins before and ends with a barrier; gives the
-// first id of the chunk that the thread found allowed, 0xffffffff for none.
-template <int THREADS>
-__device__ __forceinline__ uint32_t build_tables(const RowRules& r, int vocab, int64_t low, Tables<THREADS>& t,
-                                                 uint32_t* count, uint32_t* bias, ListPlaces& mine) {
-  using S = Tables<THREADS>;
-  const int tid = threadIdx.x, words = (vocab + 31) >> 5;
-  uint32_t lowest = 0xffffffffu;
-  auto place = [&](int32_t id) { return place_of<THREADS>(id, vocab, low); };
-  int (&at)[kListIds] = mine.history;
+// The thread's share of a list, kListIds loads at a time, the first of them issued by begin().
+struct List {
+  const int32_t* list;
+  int length;
+  int32_t first[kListIds];
+
+  __device__ __forceinline__ void load(int i0, int32_t (&ids)[kListIds]) const {
 #pragma unroll
-  for (int k = 0; k < kListIds; k++) {
-    const int64_t i = tid + k * THREADS;
-    at[k] = i < r.length ? __ldg(r.history + i) : -1;
+    for (int k = 0; k < kListIds; k++)
+      if (i0 + k * kThreads < length) ids[k] = __ldg(list + i0 + k * kThreads);
   }
-  const int32_t first_bias = tid < r.biases ? __ldg(r.bias_ids + tid) : -1;
-  for (int w = tid; w < S::kWords; w += THREADS) {
-    t.seen[w] = 0;
-    t.biased[w] = 0;
-    // ids low + 32 w .. + 31: two words of the mask, and none outside the vocabulary
-    const int64_t first = low + 32 * w;
+  __device__ __forceinline__ void begin(const int32_t* l, int n) {
+    list = l;
+    length = n;
+    load(threadIdx.x, first);
+  }
+  // Calls f(id, position).
+  template <class F>
+  __device__ __forceinline__ void each(F f) {
+    for (int i0 = threadIdx.x; i0 < length; i0 += kListIds * kThreads) {
+      if (i0 != (int)threadIdx.x) load(i0, first);
+#pragma unroll
+      for (int k = 0; k < kListIds; k++)
+        if (i0 + k * kThreads < length) f(first[k], i0 + k * kThreads);
+    }
+  }
+};
+
+// Builds the table and the bits of ids [low, low + len) of a row (low may be below 0 by less than a unit).  Ends
+// with a barrier; gives the lowest id the thread found allowed, 0xffffffff for none.
+__device__ __forceinline__ uint32_t build_table(const RowRules& r, const Table& t, int vocab, int low, int len) {
+  const int tid = threadIdx.x, from = max(low, 0), to = min(vocab - low, len) + low;  // the part's ids
+  uint32_t lowest = 0xffffffffu;
+  List history, biases;  // on their way beside the mask
+  history.begin(r.history, r.length);
+  biases.begin(r.bias_ids, r.biases);
+  const int words = (vocab + 31) >> 5;
+#pragma unroll 4
+  for (int w = tid; w < len / 32; w += kThreads) {
+    // ids first .. first + 31: two words of the mask, and none outside the vocabulary
+    const int first = low + 32 * w;
     uint32_t bits = r.none ? 0u : 0xffffffffu;
     if (r.mask) {
-      const int64_t word = first >> 5;  // floor
-      const uint32_t a0 = word >= 0 && word < words ? __ldg(r.mask + word) : 0;
-      const uint32_t a1 = word + 1 >= 0 && word + 1 < words ? __ldg(r.mask + word + 1) : 0;
+      const int word = first >> 5;  // floor
+      const uint32_t a0 = (uint32_t)word < (uint32_t)words ? __ldg(r.mask + word) : 0;
+      const uint32_t a1 = (uint32_t)(word + 1) < (uint32_t)words ? __ldg(r.mask + word + 1) : 0;
       bits = __funnelshift_r(a0, a1, (uint32_t)(first & 31));
     }
-    if (first < 0) bits &= first <= -32 ? 0u : 0xffffffffu << (int)(-first);
-    const int64_t left = (int64_t)vocab - first;
-    if (left < 32) bits &= left <= 0 ? 0u : 0xffffffffu >> (32 - (int)left);
-    t.allowed[w] = bits;
+    if (first < 0) bits &= 0xffffffffu << -first;
+    const int left = vocab - first;
+    if (left < 32) bits &= left <= 0 ? 0u : 0xffffffffu >> (32 - left);
+    t.free[w] = bits;
     if (bits) lowest = min(lowest, (uint32_t)(first + __ffs(bits) - 1));
   }
+  const bool listed = r.length > 0 || r.biases > 0;
+  if (listed)  // key, word and, where there are biases, bias lie behind one another
+    for (int s = tid * 4; s < t.slots * (t.bias ? 3 : 2); s += kThreads * 4)
+      *reinterpret_cast<uint4*>(t.key + s) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kListIds; k++) at[k] = place(at[k]);
-  mine.bias = place(first_bias);
-  if (r.length == 0 && r.biases == 0) return lowest;
-  auto see = [&](int p) {
-    if (p >= 0) {
-      count[p] = 0;
-      atomicOr(&t.seen[p >> 5], 1u << (p & 31));
-    }
-  };
-  auto weigh = [&](int p) {
-    if (p >= 0) {
-      bias[p] = 0;
-      atomicOr(&t.biased[p >> 5], 1u << (p & 31));
-    }
-  };
-#pragma unroll
-  for (int k = 0; k < kListIds; k++) see(at[k]);
-  for (int64_t i = tid + kListIds * THREADS; i < r.length; i += THREADS) see(place(__ldg(r.history + i)));
-  weigh(mine.bias);
-  for (int64_t i = tid + THREADS; i < r.biases; i += THREADS) weigh(place(__ldg(r.bias_ids + i)));
-  __syncthreads();
-  auto answer = [&](int64_t i, int p) {
-    if (p >= 0 && i >= r.prompt) atomicAdd(&count[p], 1u);
-  };
-#pragma unroll
-  for (int k = 0; k < kListIds; k++) answer(tid + k * THREADS, at[k]);
-  for (int64_t i = tid + kListIds * THREADS; i < r.length; i += THREADS) answer(i, place(__ldg(r.history + i)));
-  for (int64_t i = tid; i < r.biases; i += THREADS) {
-    const int p = i < THREADS ? mine.bias : place(__ldg(r.bias_ids + i));
-    if (p >= 0) atomicMax(&bias[p], (uint32_t)i + 1u);
-  }
+  if (!listed) return lowest;
+  history.each([&](int id, int i) {
+    if (id < from || id >= to) return;
+    const int s = slot_of(t, id, low);
+    if (i >= r.prompt) atomicAdd(&t.word[s], 2u);
+    else atomicOr(&t.word[s], 1u);
+  });
+  biases.each([&](int id, int i) {
+    if (id >= from && id < to) atomicMax(&t.bias[slot_of(t, id, low)], (uint32_t)i + 1u);
+  });
   __syncthreads();
   return lowest;
 }
 
-// Calls f(place) for the thread's share of the chunk's ids with a rule, some perhaps more than once.
-template <int THREADS, class F>
-__device__ __forceinline__ void for_ruled(const RowRules& r, int vocab, int64_t low, const ListPlaces& mine, F f) {
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int k = 0; k < kListIds; k++)
-    if (mine.history[k] >= 0) f(mine.history[k]);
-  if (mine.bias >= 0) f(mine.bias);
-  for (int64_t i = tid + kListIds * THREADS; i < r.length; i += THREADS) {
-    const int p = place_of<THREADS>(__ldg(r.history + i), vocab, low);
-    if (p >= 0) f(p);
-  }
-  for (int64_t i = tid + THREADS; i < r.biases; i += THREADS) {
-    const int p = place_of<THREADS>(__ldg(r.bias_ids + i), vocab, low);
-    if (p >= 0) f(p);
-  }
-}
-
-__device__ __forceinline__ bool bit_of(const uint32_t* bits, int p) { return (bits[p >> 5] >> (p & 31)) & 1u; }
-
-// Ruled value (not the mask) of the id at place p, raw logit l.
-template <int THREADS>
-__device__ __forceinline__ float ruled(float l, int p, const RowRules& r, const Tables<THREADS>& t, const uint32_t* count,
-                                       const uint32_t* bias) {
-  float x = l;
-  if (bit_of(t.seen, p)) {
-    x = x > 0.0f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
-    const uint32_t c = count[p];
-    if (c) {
-      x = __fsub_rn(x, __fmul_rn(r.frequency, (float)c));
-      x = __fsub_rn(x, r.presence);
-    }
-  }
-  if (bit_of(t.biased, p)) x = __fadd_rn(x, __ldg(r.bias_values + bias[p] - 1));
-  return x;
-}
-
-// exp(v), v <= 0: relative error 2^-22 + |v| 2^-23.
-__device__ __forceinline__ float exp_below(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v * 1.4426950408889634f));
-  return r;
-}
-
-template <class T>
-__global__ void __launch_bounds__(kRulesThreads, 6) k_logits_rules(const __grid_constant__ needle_logits_rules a, T* out,
-                                                                int64_t out_stride) {
-  constexpr int THREADS = kRulesThreads, VEC = 16 / sizeof(T), UNITS = kPerThread / VEC;
-  using S = Tables<THREADS>;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  S& t = *reinterpret_cast<S*>(smem_raw);
-  uint32_t* count = reinterpret_cast<uint32_t*>(smem_raw + tables_bytes<THREADS>());
-  uint32_t* bias = count + (a.history ? S::kChunk : 0);
-  const int64_t row = blockIdx.y;
-  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-  T* to = out + row * out_stride;
-  const int tid = threadIdx.x, off = row_offset(in);
-  const int64_t low = (int64_t)blockIdx.x * S::kChunk - off;
-  if (low >= a.vocab) return;
-  const RowRules r = row_rules(a, row);
-  float x[UNITS][VEC];
-#pragma unroll
-  for (int u = 0; u < UNITS; u++) load_unit<T, VEC>(in, low + (int64_t)(u * THREADS + tid) * VEC, a.vocab, x[u]);
-  ListPlaces mine;
-  build_tables<THREADS>(r, a.vocab, low, t, count, bias, mine);
-  const bool same = row_offset(to) == off;  // 16-byte units of the output line up with the input's
-#pragma unroll
-  for (int u = 0; u < UNITS; u++) {
-    const int p0 = (u * THREADS + tid) * VEC;
-    const uint32_t allowed = t.allowed[p0 >> 5] >> (p0 & 31);
-    Vec<T, VEC> v;
-#pragma unroll
-    for (int i = 0; i < VEC; i++) v.v[i] = from_f32<T>((allowed >> i) & 1 ? x[u][i] : -INFINITY);
-    const int64_t e = low + p0;
-    if (same && e >= 0 && e + VEC <= a.vocab) {
-      *reinterpret_cast<Vec<T, VEC>*>(to + e) = v;
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; i++)
-        if (e + i >= 0 && e + i < a.vocab) to[e + i] = v.v[i];
-    }
-  }
+// Calls f(slot, id, raw logit, ruled logit) for the thread's share of the part's allowed ids with a rule.  Four
+// gathers at a time are in flight.  Keys of ids that are not allowed go.
+template <class T, class F>
+__device__ __forceinline__ void for_ruled(const RowRules& r, const Table& t, const T* row, F f) {
   if (r.length == 0 && r.biases == 0) return;
-  __syncthreads();  // ids with a rule are written after the stream has passed them
-  // one thread takes each id that is allowed, by clearing its bit: in place, where the stream has put the same
-  // logit back, nobody else may read or write it
-  for_ruled<THREADS>(r, a.vocab, low, mine, [&](int p) {
-    const uint32_t bit = 1u << (p & 31);
-    if (atomicAnd(&t.allowed[p >> 5], ~bit) & bit)
-      to[low + p] = from_f32<T>(ruled<THREADS>(to_f32(in[low + p]), p, r, t, count, bias));
-  });
+  for (int s0 = threadIdx.x; s0 < t.slots; s0 += 4 * kThreads) {
+    uint32_t key[4], word[4];
+    float raw[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int s = s0 + k * kThreads;
+      key[k] = s < t.slots ? t.key[s] : 0;
+      word[k] = key[k] ? t.word[s] : 0;
+      if (key[k] && !(word[k] & 0x80000000u)) {
+        t.key[s] = 0;
+        key[k] = 0;
+      }
+      raw[k] = key[k] ? to_f32(row[key[k] - 1u]) : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (key[k] == 0) continue;
+      const int s = s0 + k * kThreads;
+      float x = raw[k];
+      const uint32_t seen = word[k] & 0x7fffffffu, c = seen >> 1;
+      if (seen) x = x > 0.0f ? __fdiv_rn(x, r.repetition) : __fmul_rn(x, r.repetition);
+      if (c) {
+        x = __fsub_rn(x, __fmul_rn(r.frequency, (float)c));
+        x = __fsub_rn(x, r.presence);
+      }
+      if (t.bias) {
+        const uint32_t b = t.bias[s];
+        if (b) x = __fadd_rn(x, __ldg(r.bias_values + b - 1));
+      }
+      f(s, (int)(key[k] - 1u), raw[k], x);
+    }
+  }
 }
 
-// One cluster per row; its CTAs take the row's chunks in turn.
+// The table lies behind the warps' rings.
 template <class T>
-__global__ void __launch_bounds__(kSelectThreads, 3) k_logits_select(const __grid_constant__ needle_logits_rules a,
-                                                                  int32_t* __restrict__ ids,
-                                                                  float* __restrict__ log_probabilities) {
-  constexpr int THREADS = kSelectThreads, VEC = 16 / sizeof(T), UNITS = kPerThread / VEC;
-  using S = Tables<THREADS>;
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  S& t = *reinterpret_cast<S*>(smem_raw);
-  uint32_t* count = reinterpret_cast<uint32_t*>(smem_raw + tables_bytes<THREADS>());
-  uint32_t* bias = count + (a.history ? S::kChunk : 0);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int64_t row = blockIdx.y;
-  const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, off = row_offset(in);
-  const RowRules r = row_rules(a, row);
-  // the thread's running best, largest raw logit and sum of exponentials
-  uint32_t id = 0xffffffffu;
-  float best = -INFINITY, top = -INFINITY, sum = 0.0f;
-  uint32_t lowest = 0xffffffffu;  // the lowest allowed id: the choice where every allowed logit is -inf
-  for (int64_t c = blockIdx.x; c * S::kChunk - off < a.vocab; c += gridDim.x) {
-    const int64_t low = c * S::kChunk - off;
-    float x[UNITS][VEC];
+__device__ __forceinline__ Table table_in(unsigned char* smem, const needle_logits_rules& a, const LogitsPlan& plan) {
+  Table t;
+  t.slots = plan.slots;
+  t.key = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * kSliceBytes);
+  t.word = t.key + plan.slots;
+  t.bias = a.bias_ids ? t.word + plan.slots : nullptr;
+  t.free = t.key + plan.slots * (a.bias_ids ? 3 : 2);
+  return t;
+}
+
+// The steps a CTA streams: the rows blockIdx.y, + gridDim.y, ..., of each the parts blockIdx.x, + gridDim.x, ...
+template <class T>
+struct Steps {
+  const T* in;   // the row
+  int64_t row;
+  int off, part, at, end;  // the step's first id, and where its part ends
+
+  __device__ __forceinline__ void begin_part(const needle_logits_rules& a, const LogitsPlan& plan) {
+    at = part * plan.part - off;
+    end = min(at + plan.part, a.vocab);
+  }
+  // The next row, from this one on, that has ids in the CTA's first part (a row's units may begin before it, so
+  // the last part of a row can be empty where another's is not).
+  __device__ __forceinline__ void begin_row(const needle_logits_rules& a, const LogitsPlan& plan) {
+    part = blockIdx.x;
+    for (; row < a.rows; row += gridDim.y) {
+      in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+      off = row_offset(in);
+      begin_part(a, plan);
+      if (at < a.vocab) return;
+    }
+  }
+  __device__ __forceinline__ void next(const needle_logits_rules& a, const LogitsPlan& plan) {
+    at += step_ids(sizeof(T));
+    if (at < end) return;
+    part += gridDim.x;
+    begin_part(a, plan);
+    if (part < plan.parts && at < a.vocab) return;
+    row += gridDim.y;
+    begin_row(a, plan);
+  }
+};
+
+// A warp's stream: its slice of every step, kStages of them in shared memory or on their way.
+template <class T>
+struct Stream {
+  static constexpr int VEC = 16 / sizeof(T), N = kUnits, kSlice = 32 * VEC * N;  // ids of a 16-byte unit, units of a lane, ids of a step
+  T* ring;
+  uint64_t* bars;  // kStages of them
+  Steps<T> steps;  // what is copied next
+  int stage;       // of the next step to be read
+  uint32_t parity;
+  bool ok;
+
+  // Whole units of a slice that begins with id e inside the row: from unit `begin` to unit `end`.
+  static __device__ __forceinline__ void whole_units(int e, int vocab, int& begin, int& end) {
+    begin = e < 0 ? (-e + VEC - 1) / VEC : 0;
+    end = max(begin, min(32 * N, (vocab - e) / VEC));
+    if (e >= vocab) end = begin;
+  }
+  __device__ __forceinline__ void copy(const needle_logits_rules& a, const LogitsPlan& plan, int s) {
+    if (steps.row >= a.rows) return;
+    if ((threadIdx.x & 31) == 0) {
+      const int e = steps.at + (int)(threadIdx.x >> 5) * kSlice;
+      int begin, end;
+      whole_units(e, a.vocab, begin, end);
+      const uint32_t bytes = (uint32_t)(end - begin) * 16;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_address(&bars[s])), "r"(bytes) : "memory");
+      if (bytes) copy_bulk(ring + s * kSlice + begin * VEC, steps.in + e + begin * VEC, bytes, &bars[s]);
+    }
+    steps.next(a, plan);
+  }
+  __device__ __forceinline__ void begin(const needle_logits_rules& a, const LogitsPlan& plan, unsigned char* smem, uint64_t* all) {
+    const int warp = threadIdx.x >> 5;
+    ring = reinterpret_cast<T*>(smem) + warp * kStages * kSlice;
+    bars = all + warp * kStages;
+    if ((threadIdx.x & 31) == 0) {
+      for (int s = 0; s < kStages; s++) barrier_init(&bars[s], 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    steps.row = blockIdx.y;
+    steps.begin_row(a, plan);
+    for (int s = 0; s < kStages; s++) copy(a, plan, s);
+    stage = 0;
+    parity = 0;
+    ok = true;
+  }
+  // The lane's units of the next step, which begins at id `at` of row `in`; ids outside [0, vocab) are -inf.
+  // After a wait that ran out everything is NaN.
+  __device__ __forceinline__ void read(const T* in, int at, int vocab, Vec<T, VEC> (&v)[N]) {
+    const int lane = threadIdx.x & 31, e = at + (int)(threadIdx.x >> 5) * kSlice;
+    ok = ok && barrier_wait_warp(&bars[stage], parity);
+    const Vec<T, VEC>* p = reinterpret_cast<const Vec<T, VEC>*>(ring + stage * kSlice) + lane;
+    if (ok && e >= 0 && e <= vocab - kSlice) {
 #pragma unroll
-    for (int u = 0; u < UNITS; u++) load_unit<T, VEC>(in, low + (int64_t)(u * THREADS + tid) * VEC, a.vocab, x[u]);
-    if (c != blockIdx.x) __syncthreads();  // the tables of the chunk before are read
-    ListPlaces mine;
-    lowest = min(lowest, build_tables<THREADS>(r, a.vocab, low, t, count, bias, mine));
-    float m = top;
+      for (int u = 0; u < N; u++) v[u] = p[u * 32];
+      return;
+    }
+    int begin, end;
+    whole_units(e, vocab, begin, end);
 #pragma unroll
-    for (int u = 0; u < UNITS; u++)
+    for (int u = 0; u < N; u++) {
+      const int k = u * 32 + lane, first = e + k * VEC;
+      if (k >= begin && k < end) {
+        v[u] = p[u * 32];
+      } else {
 #pragma unroll
-      for (int i = 0; i < VEC; i++) m = fmaxf(m, x[u][i]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    sum = top == -INFINITY ? 0.0f : sum * exp_below(top - base);
-    top = m;
-    int at = -1;
+        for (int i = 0; i < VEC; i++) v[u].v[i] = first + i >= 0 && first + i < vocab ? in[first + i] : from_f32<T>(-INFINITY);
+      }
+      if (!ok) {
 #pragma unroll
-    for (int u = 0; u < UNITS; u++) {
-      const int p0 = (u * THREADS + tid) * VEC, w = p0 >> 5;
-      const uint32_t free = (t.allowed[w] & ~(t.seen[w] | t.biased[w])) >> (p0 & 31);  // allowed, without a rule
+        for (int i = 0; i < VEC; i++) v[u].v[i] = from_f32<T>(NAN);
+      }
+    }
+  }
+  // The step's units have been taken: its place is filled again.
+  __device__ __forceinline__ void advance(const needle_logits_rules& a, const LogitsPlan& plan) {
+    __syncwarp();
+    if (ok) copy(a, plan, stage);
+    if (++stage == kStages) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+  // Before the warp ends: a wait that ran out is reported, and copies on their way get their time.
+  __device__ __forceinline__ void finish(uint32_t* wait_words) {
+    if (ok) return;
+    if ((threadIdx.x & 31) == 0) {
+      report_wait_timeout(wait_words, kWaitLogits);
+      for (int s = 0; s < kStages; s++) barrier_wait(&bars[s], parity);
+    }
+    __syncwarp();
+  }
+};
+
+template <class T>
+__global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_rules(const __grid_constant__ needle_logits_rules a,
+                                                            const LogitsPlan plan, T* out, int64_t out_stride,
+                                                            uint32_t* wait_words) {
+  using S = Stream<T>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t bars[kWarps * kStages];
+  const Table t = table_in<T>(smem, a, plan);
+  const int tid = threadIdx.x, lane = tid & 31, slice = (tid >> 5) * S::kSlice;
+  S stream;
+  stream.begin(a, plan, smem, bars);
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    T* to = out + row * out_stride;
+    const int off = row_offset(in);
+    const RowRules r = row_rules(a, row);
+    const bool listed = r.length > 0 || r.biases > 0;
+    // whole units can be written where the output's 16-byte units line up with the input's
+    const bool same = row_offset(to) == off;
+    for (int part = blockIdx.x; part < plan.parts; part += gridDim.x) {
+      const int low = part * plan.part - off, end = min(low + plan.part, a.vocab);
+      if (low >= a.vocab) break;
+      build_table(r, t, a.vocab, low, plan.part);
+      // ruled logits are taken before the stream writes (out may be the logits) and written behind it
+      for_ruled(r, t, in, [&](int s, int, float, float x) { t.word[s] = __float_as_uint(x); });
+      if (listed) __syncthreads();
+      for (int at = low; at < end; at += step_ids(sizeof(T))) {
+        Vec<T, S::VEC> x[S::N];
+        stream.read(in, at, a.vocab, x);
+        stream.advance(a, plan);
+        const int e0 = at + slice + lane * S::VEC;
+        const bool whole = same && at + slice >= 0 && at + slice <= a.vocab - S::kSlice;
 #pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        sum += exp_below(x[u][i] - base);
-        if (((free >> i) & 1) && x[u][i] > best) {  // ids rise: an equal logit keeps the lower id
-          best = x[u][i];
-          at = u * VEC + i;
+        for (int u = 0; u < S::N; u++) {
+          const int e = e0 + u * 32 * S::VEC, p = e - low;
+          const uint32_t free = t.free[p >> 5] >> (p & 31);
+          keep_free(x[u], free);
+          if (whole || (same && e >= 0 && e <= a.vocab - S::VEC)) {
+            *reinterpret_cast<Vec<T, S::VEC>*>(to + e) = x[u];
+          } else {
+#pragma unroll
+            for (int i = 0; i < S::VEC; i++)
+              if (e + i >= 0 && e + i < a.vocab) to[e + i] = x[u].v[i];
+          }
         }
       }
-    }
-    if (at >= 0) id = (uint32_t)(low + (at / VEC * THREADS + tid) * VEC + at % VEC);
-    for_ruled<THREADS>(r, a.vocab, low, mine, [&](int p) {
-      if (!bit_of(t.allowed, p)) return;
-      const float v = ruled<THREADS>(to_f32(in[low + p]), p, r, t, count, bias);
-      const uint32_t i = (uint32_t)(low + p);
-      if (v > best || (v == best && i < id && v > -INFINITY)) {
-        best = v;
-        id = i;
+      __syncthreads();
+      if (listed) {
+        for (int s = tid; s < t.slots; s += kThreads) {
+          const uint32_t key = t.key[s];
+          if (key) to[key - 1u] = from_f32<T>(__uint_as_float(t.word[s]));
+        }
+        __syncthreads();
       }
-    });
-  }
-  // warp, CTA, cluster; sums in a fixed order
-  auto warp_merge = [&](float& m, float& s) {
-    const float m0 = m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    s = m0 == -INFINITY ? s : s * exp_below(m0 - m);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  };
-  auto warp_best = [&](uint32_t& k, uint32_t& i) {
-    const uint32_t best = __reduce_max_sync(0xffffffffu, k);
-    i = __reduce_min_sync(0xffffffffu, k == best ? i : 0xffffffffu);
-    k = best;
-  };
-  uint32_t k = id == 0xffffffffu ? 0 : order_key(best);
-  warp_best(k, id);
-  warp_merge(top, sum);
-  lowest = __reduce_min_sync(0xffffffffu, lowest);
-  if (lane == 0) {
-    t.top[warp] = top;
-    t.sum[warp] = sum;
-    t.key[warp] = k;
-    t.id[warp] = id;
-    t.lowest[warp] = lowest;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    const bool in_use = lane < S::kWarps;
-    k = in_use ? t.key[lane] : 0;
-    id = in_use ? t.id[lane] : 0xffffffffu;
-    lowest = __reduce_min_sync(0xffffffffu, in_use ? t.lowest[lane] : 0xffffffffu);
-    top = in_use ? t.top[lane] : -INFINITY;
-    sum = in_use ? t.sum[lane] : 0.0f;
-    warp_best(k, id);
-    warp_merge(top, sum);
-    if (lane == 0 && gridDim.x > 1) {
-      t.cta_top = top;
-      t.cta_sum = sum;
-      t.cta_key = k;
-      t.cta_id = id;
-      t.cta_lowest = lowest;
     }
   }
-  if (gridDim.x > 1) cluster.sync();
-  if (blockIdx.x == 0 && warp == 0) {
-    if (gridDim.x > 1) {
-      const bool in_use = lane < (int)gridDim.x;
-      const S& o = *cluster.map_shared_rank(&t, in_use ? lane : 0);
-      k = in_use ? o.cta_key : 0;
-      id = in_use ? o.cta_id : 0xffffffffu;
-      lowest = __reduce_min_sync(0xffffffffu, in_use ? o.cta_lowest : 0xffffffffu);
-      top = in_use ? o.cta_top : -INFINITY;
-      sum = in_use ? o.cta_sum : 0.0f;
-      warp_best(k, id);
-      warp_merge(top, sum);
-    }
-    if (lane == 0) {
-      if (k == 0) id = lowest;
-      ids[row] = (int32_t)id;  // 0xffffffff is -1
-      log_probabilities[row] = id != 0xffffffffu ? (to_f32(in[id]) - top) - logf(sum) : -INFINITY;
-    }
-  }
-  if (gridDim.x > 1) cluster.sync();  // shared memory lives until its readers are done
+  stream.finish(wait_words);
 }
 
-// Chunks of a row: one more id range is needed only where rows do not all start on 16 bytes.
-int chunks_of(const needle_logits_rules& a, int chunk) {
+// One cluster per row (and the rows gridDim.y on); its CTAs take the row's parts in turn.
+template <class T>
+__global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_select(const __grid_constant__ needle_logits_rules a,
+                                                             const LogitsPlan plan, int32_t* __restrict__ ids,
+                                                             float* __restrict__ log_probabilities, uint32_t* wait_words) {
+  using S = Stream<T>;
+  struct Best {  // of a warp, of a CTA
+    float top, sum, raw;
+    uint32_t key, id, lowest;
+  };
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(8) uint64_t bars[kWarps * kStages];
+  __shared__ Best of_warp[kWarps], of_cta;
+  const Table t = table_in<T>(smem, a, plan);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, slice = warp * S::kSlice;
+  S stream;
+  stream.begin(a, plan, smem, bars);
+  // sums in a fixed order
+  auto merge = [&](Best& b) {
+    const float m = b.top;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b.top = fmaxf(b.top, __shfl_xor_sync(0xffffffffu, b.top, o));
+    b.sum = m == -INFINITY ? b.sum : b.sum * exp_below(m - b.top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b.sum += __shfl_xor_sync(0xffffffffu, b.sum, o);
+    const uint32_t key = __reduce_max_sync(0xffffffffu, b.key);
+    const uint32_t id = __reduce_min_sync(0xffffffffu, b.key == key ? b.id : 0xffffffffu);
+    const uint32_t who = __ballot_sync(0xffffffffu, b.key == key && b.id == id);
+    b.raw = __shfl_sync(0xffffffffu, b.raw, __ffs(who) - 1);
+    b.key = key;
+    b.id = id;
+    b.lowest = __reduce_min_sync(0xffffffffu, b.lowest);
+  };
+  const Best nothing = {-INFINITY, 0.0f, 0.0f, 0u, 0xffffffffu, 0xffffffffu};
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const int off = row_offset(in);
+    const RowRules r = row_rules(a, row);
+    // the warp's best of the stream; the thread's best of the ids with a rule and its raw logit; the thread's
+    // largest raw logit and sum of exponentials
+    float best = -INFINITY, ruled_best = -INFINITY, raw = 0.0f, top = -INFINITY, sum = 0.0f;
+    uint32_t id = 0xffffffffu, ruled_id = 0xffffffffu;
+    uint32_t lowest = 0xffffffffu;  // the lowest allowed id: the choice where every allowed logit is -inf
+    for (int part = blockIdx.x; part < plan.parts; part += gridDim.x) {
+      const int low = part * plan.part - off, end = min(low + plan.part, a.vocab);
+      if (low >= a.vocab) break;
+      if (part != (int)blockIdx.x) __syncthreads();  // the table of the part before has been read
+      lowest = min(lowest, build_table(r, t, a.vocab, low, plan.part));
+      for (int at = low; at < end; at += step_ids(sizeof(T))) {
+        float x[S::N][S::VEC];
+        {
+          Vec<T, S::VEC> v[S::N];
+          stream.read(in, at, a.vocab, v);
+#pragma unroll
+          for (int u = 0; u < S::N; u++)
+#pragma unroll
+            for (int i = 0; i < S::VEC; i++) x[u][i] = to_f32(v[u].v[i]);
+        }
+        stream.advance(a, plan);
+        float most = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < S::N; u++)
+#pragma unroll
+          for (int i = 0; i < S::VEC; i += 2) most = max3(most, x[u][i], x[u][i + 1]);
+        const float m = fmaxf(top, most), base = m == -INFINITY ? 0.0f : m;
+        sum = top == -INFINITY ? 0.0f : sum * exp_below(top - base);
+        top = m;
+        if (fabsf(base) < 1e38f) {
+          // 2^(x log2 e - m log2 e): the rounding of m log2 e is the same factor for all of a step's terms, off
+          // by |m| 2^-24 at most
+          const float2 scale = make_float2(kLog2eL, kLog2eL), minus = make_float2(-base * kLog2eL, -base * kLog2eL);
+          float2 more = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int u = 0; u < S::N; u++)
+#pragma unroll
+            for (int i = 0; i < S::VEC; i += 2) {
+              float2 d = __ffma2_rn(make_float2(x[u][i], x[u][i + 1]), scale, minus);
+              d.x = exp2_of(d.x);
+              d.y = exp2_of(d.y);
+              more = __fadd2_rn(more, d);
+            }
+          sum += more.x + more.y;
+        } else {
+#pragma unroll
+          for (int u = 0; u < S::N; u++)
+#pragma unroll
+            for (int i = 0; i < S::VEC; i++) sum += exp_below(x[u][i] - base);
+        }
+        // the free ids matter only where some id of the step beats the best one so far
+        if (__any_sync(0xffffffffu, most > best)) {
+          uint32_t free[S::N];
+          float top_free = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < S::N; u++) {
+            const int p = at - low + slice + (u * 32 + lane) * S::VEC;
+            free[u] = t.free[p >> 5] >> (p & 31);
+#pragma unroll
+            for (int i = 0; i < S::VEC; i++)
+              if (free[u] & (1u << i)) top_free = fmaxf(top_free, x[u][i]);
+          }
+          const uint32_t key = __reduce_max_sync(0xffffffffu, order_key(top_free));
+          if (key > order_key(best)) {
+            uint32_t mine = 0xffffffffu;
+            if (order_key(top_free) == key) {
+#pragma unroll
+              for (int u = S::N - 1; u >= 0; u--)
+#pragma unroll
+                for (int i = S::VEC - 1; i >= 0; i--)
+                  if ((free[u] & (1u << i)) && x[u][i] == top_free)
+                    mine = (uint32_t)(at + slice + (u * 32 + lane) * S::VEC + i);
+            }
+            id = __reduce_min_sync(0xffffffffu, mine);
+            best = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+          }
+        }
+      }
+      for_ruled(r, t, in, [&](int, int id_of, float l, float v) {
+        const uint32_t i = (uint32_t)id_of;
+        if (v > ruled_best || (v == ruled_best && i < ruled_id && v > -INFINITY)) {
+          ruled_best = v;
+          raw = l;
+          ruled_id = i;
+        }
+      });
+    }
+    // warp, CTA, cluster
+    if (best > ruled_best || (best == ruled_best && id < ruled_id)) {
+      ruled_best = raw = best;
+      ruled_id = id;
+    }
+    Best b = {top, sum, raw, ruled_id == 0xffffffffu ? 0u : order_key(ruled_best), ruled_id, lowest};
+    merge(b);
+    if (lane == 0) of_warp[warp] = b;
+    __syncthreads();
+    if (warp == 0) {
+      b = lane < kWarps ? of_warp[lane] : nothing;
+      merge(b);
+      if (lane == 0 && gridDim.x > 1) of_cta = b;
+    }
+    if (gridDim.x > 1) cluster.sync();
+    if (blockIdx.x == 0 && warp == 0) {
+      if (gridDim.x > 1) {
+        b = nothing;
+        if (lane < (int)gridDim.x) b = *cluster.map_shared_rank(&of_cta, lane);
+        merge(b);
+      }
+      if (lane == 0) {
+        const bool only = b.key == 0 && b.lowest != 0xffffffffu;  // no allowed logit above -inf
+        if (only) {
+          b.id = b.lowest;
+          b.raw = to_f32(in[b.id]);
+        }
+        ids[row] = (int32_t)b.id;  // 0xffffffff is -1
+        log_probabilities[row] = b.id != 0xffffffffu ? (b.raw - b.top) - logf(b.sum) : -INFINITY;
+      }
+    }
+    if (gridDim.x > 1) cluster.sync();  // the CTAs' results have been read
+  }
+  stream.finish(wait_words);
+}
+
+size_t smem_bytes(const needle_logits_rules& a, const LogitsPlan& p) {
+  return size_t(kWarps * kStages * kSliceBytes) + size_t(p.slots) * (a.bias_ids ? 12 : 8) + size_t(p.part) / 8;
+}
+
+// CTAs that the GPU holds at once: by shared memory, and by registers.
+int64_t resident_ctas(const needle_logits_rules& a, size_t smem) {
+  return 148 * std::max<int64_t>(1, std::min<int64_t>(resident(type_bytes(a.type)), int64_t(226 * 1024 / (smem + 1536))));
+}
+
+// Rows a CTA (or cluster) of `parts` CTAs takes side by side with the others: as few turns as the GPU can hold,
+// all of them full.
+unsigned rows_at_once(const needle_logits_rules& a, size_t smem, int parts) {
+  const int64_t fit = std::max<int64_t>(1, resident_ctas(a, smem) / parts), turns = (a.rows + fit - 1) / fit;
+  return unsigned((a.rows + turns - 1) / turns);
+}
+
+LogitsPlan plan_for(const needle_logits_rules& a, int most_parts) {
+  LogitsPlan p{};
   const int64_t element = int64_t(type_bytes(a.type));
   const bool lined_up = aligned_to(a.logits, 16) && (a.rows == 1 || a.logits_stride * element % 16 == 0);
-  return int((int64_t(a.vocab) + (lined_up ? 0 : 16 / element - 1) + chunk - 1) / chunk);
+  const int64_t ids = int64_t(a.vocab) + (lined_up ? 0 : 16 / element - 1);  // with those before a row's first unit
+  const int64_t entries = (a.history ? a.history_stride : 0) + (a.bias_ids ? a.bias_stride : 0);
+  const int64_t step = step_ids(size_t(element)), steps = (ids + step - 1) / step;
+  // parts: as many as keep the GPU busy, each rescanning the lists; small enough for their bits and, with long
+  // lists, for a table that has room for every id of the part
+  const int64_t most = (entries > kMostEntries ? kMostEntries : kPartIds) / step;
+  int64_t parts = std::max<int64_t>(1, std::min<int64_t>({steps, 148 * 4 / a.rows, most_parts}));
+  parts = std::max(parts, (steps + most - 1) / most);
+  const int64_t per = (steps + parts - 1) / parts;
+  p.part = int(per * step);
+  p.parts = int((steps + per - 1) / per);
+  if (entries > 0) p.slots = int((std::min(entries, int64_t(p.part)) * 2 + 35) / 4 * 4);
+  return p;
 }
-
-// CTAs that keep the GPU busy: four of kSelectThreads an SM.
-constexpr int64_t kSelectCtas = 148 * 4;
 
 int check_rules(const needle_logits_rules* a, int* device, const char* op) {
   if (!a) return refuse("null argument");
@@ -422,12 +668,15 @@ int check_rules(const needle_logits_rules* a, int* device, const char* op) {
   if (a->rows < 0 || a->vocab < 0) return refuse("bad row or vocabulary count");
   if (a->rows == 0 || a->vocab == 0) return NEEDLE_OK;
   if (a->rows > 65535) return refuse("at most 65535 rows in a call");
+  if (a->vocab > 1 << 30) return refuse("at most 2^30 ids");
   if (!a->logits) return refuse("null argument");
   if (a->rows > 1 && a->logits_stride < a->vocab) return refuse("a row stride is shorter than its row");
   if (!aligned_to(a->logits, type_bytes(a->type))) return refuse("a buffer is not aligned to its element type");
   if (a->history && (!a->history_lengths || a->history_stride < 0)) return refuse("history without lengths");
-  if (a->bias_ids && (!a->bias_values || !a->bias_counts || a->bias_stride < 0 || a->bias_stride >= 0x7fffffff))
+  if (a->bias_ids && (!a->bias_values || !a->bias_counts || a->bias_stride < 0))
     return refuse("bias ids without values or counts");
+  if ((a->history && a->history_stride > 1 << 30) || (a->bias_ids && a->bias_stride > 1 << 30))
+    return refuse("at most 2^30 history entries or biases a row");
   if (a->masks && (!a->mask_slots || a->mask_count < 0)) return refuse("masks without slots");
   const cudaError_t e = cudaGetDevice(device);
   if (e != cudaSuccess) return refuse_cuda(op, e);
@@ -454,13 +703,15 @@ extern "C" int needle_cuda_logits_rules_dev(const needle_logits_rules* a, void* 
     if (a->rows > 1 && out_stride < a->vocab) return refuse("a row stride is shorter than its row");
     if (!aligned_to(out, type_bytes(a->type))) return refuse("a buffer is not aligned to its element type");
     if (int rc = check_buffer(out, "out", device)) return rc;
+    if (check_wait_status(device) != NEEDLE_OK) return int(NEEDLE_BACKEND_UNAVAILABLE);
+    const LogitsPlan plan = plan_for(*a, 1 << 30);
+    const size_t smem = smem_bytes(*a, plan);
     const cudaError_t e = with_type(a->type, [&](auto zero) {
       using T = decltype(zero);
-      const size_t smem = smem_bytes<kRulesThreads>(*a);
-      cudaError_t err = set_smem(k_logits_rules<T>, smem);
+      const cudaError_t err = set_smem(k_logits_rules<T>, smem);
       if (err != cudaSuccess) return err;
-      k_logits_rules<T><<<dim3(chunks_of(*a, kRulesThreads * kPerThread), a->rows), kRulesThreads, smem,
-                          static_cast<cudaStream_t>(stream)>>>(*a, static_cast<T*>(out), out_stride);
+      k_logits_rules<T><<<dim3(plan.parts, rows_at_once(*a, smem, plan.parts)), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
+          *a, plan, static_cast<T*>(out), out_stride, wait_status_words(device));
       return cudaGetLastError();
     });
     return e == cudaSuccess ? int(NEEDLE_OK) : refuse_cuda("logits_rules", e);
@@ -477,28 +728,27 @@ extern "C" int needle_cuda_logits_select_dev(const needle_logits_rules* a, int32
     if (!ids || !log_probabilities) return refuse("null argument");
     if (int rc = check_buffer(ids, "ids", device)) return rc;
     if (int rc = check_buffer(log_probabilities, "log_probabilities", device)) return rc;
+    if (check_wait_status(device) != NEEDLE_OK) return int(NEEDLE_BACKEND_UNAVAILABLE);
+    const LogitsPlan plan = plan_for(*a, 8);  // a row's CTAs are one cluster
+    const size_t smem = smem_bytes(*a, plan);
     const cudaError_t e = with_type(a->type, [&](auto zero) {
       using T = decltype(zero);
-      const size_t smem = smem_bytes<kSelectThreads>(*a);
-      cudaError_t err = set_smem(k_logits_select<T>, smem);
+      const cudaError_t err = set_smem(k_logits_select<T>, smem);
       if (err != cudaSuccess) return err;
-      const int chunks = chunks_of(*a, kSelectThreads * kPerThread);
-      int cluster = 1;
-      while (cluster < 8 && cluster < chunks && a->rows * int64_t(cluster) < kSelectCtas) cluster *= 2;
-      cudaLaunchConfig_t config{};
-      config.gridDim = dim3(cluster, a->rows);
-      config.blockDim = dim3(kSelectThreads);
-      config.dynamicSmemBytes = smem;
-      config.stream = static_cast<cudaStream_t>(stream);
+      const int cluster = std::min(8, plan.parts);
       cudaLaunchAttribute attribute{};
       attribute.id = cudaLaunchAttributeClusterDimension;
       attribute.val.clusterDim.x = cluster;
       attribute.val.clusterDim.y = 1;
       attribute.val.clusterDim.z = 1;
+      cudaLaunchConfig_t config{};
+      config.gridDim = dim3(cluster, rows_at_once(*a, smem, cluster));
+      config.blockDim = dim3(kThreads);
+      config.dynamicSmemBytes = smem;
+      config.stream = static_cast<cudaStream_t>(stream);
       config.attrs = &attribute;
       config.numAttrs = 1;
-      err = cudaLaunchKernelEx(&config, k_logits_select<T>, *a, ids, log_probabilities);
-      return err == cudaSuccess ? cudaGetLastError() : err;
+      return cudaLaunchKernelEx(&config, k_logits_select<T>, *a, plan, ids, log_probabilities, wait_status_words(device));
     });
     return e == cudaSuccess ? int(NEEDLE_OK) : refuse_cuda("logits_select", e);
   });

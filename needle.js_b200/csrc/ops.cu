@@ -78,7 +78,8 @@ std::mutex g_status_mu;
 uint32_t* g_status_host = nullptr;
 bool g_status_failed = false;
 
-const char* kWaitKindNames[kWaitKinds] = {"fast attention", "table matvec", "tensor-core matvec", "wait self-test"};
+const char* kWaitKindNames[kWaitKinds] = {"fast attention", "table matvec", "tensor-core matvec", "wait self-test",
+                                         "logits"};
 
 __device__ int g_never_set;  // nothing writes it: the self-test's wait always runs out
 

@@ -65,14 +65,6 @@ struct Stage {
   float ks[kBlock], vs[kBlock];  // zeros behind the last position
 };
 
-// Global -> shared bulk copy whose bytes are counted on `bar`.
-__device__ __forceinline__ void copy_bulk(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(shared_address(to)),
-      "l"(from), "r"(bytes), "r"(shared_address(bar))
-      : "memory");
-}
-
 // A warp's state of up to 4 NG heads: lane (g, c) keeps the heads c, 4 + c: their reference maximum, the sum of
 // its own weights, and the output dimensions g * D / 8 .. + D / 8 - 1.
 template <int D, int NG>

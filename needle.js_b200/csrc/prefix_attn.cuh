@@ -48,52 +48,6 @@ __device__ __forceinline__ float power2(int e) { return __int_as_float((e + 127)
 // Exponent of |v| (0 and subnormals -127, infinities and NaN 128).
 __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255u) - 127; }
 
-__device__ __forceinline__ uint32_t shared_address(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void barrier_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(b)) : "memory");
-}
-__device__ __forceinline__ bool barrier_try(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(shared_address(b)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-constexpr uint64_t kAttendWaitNs = 2000000000ull;
-// Waits for the phase of the given parity; false once kAttendWaitNs has passed without it.
-__device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
-  if (barrier_try(b, parity)) return true;
-  uint64_t start, now;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
-  for (;;) {
-    for (int i = 0; i < 64; i++)
-      if (barrier_try(b, parity)) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-    if (now - start > kAttendWaitNs) return false;
-  }
-}
-
-// The same for a converged warp, all lanes polling: a branch that one lane takes, and coming back from it,
-// costs a waiting warp about 200 cycles.
-__device__ __forceinline__ bool barrier_wait_warp(uint64_t* b, uint32_t parity) {
-  if (__all_sync(0xffffffffu, barrier_try(b, parity))) return true;
-  uint64_t start, now;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
-  for (;;) {
-    for (int i = 0; i < 64; i++)
-      if (__all_sync(0xffffffffu, barrier_try(b, parity))) return true;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-    if (__any_sync(0xffffffffu, now - start > kAttendWaitNs)) return false;
-  }
-}
-
 // The next kernel of the stream may be started (when it was launched to overlap) / the kernel before has ended
 // and its writes are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -33,6 +33,60 @@ struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
 
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void barrier_init(uint64_t* b, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void barrier_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(shared_address(b)) : "memory");
+}
+__device__ __forceinline__ bool barrier_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(shared_address(b)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+constexpr uint64_t kServingWaitNs = 2000000000ull;
+// Waits for the phase of the given parity; false once kServingWaitNs has passed without it.
+__device__ __forceinline__ bool barrier_wait(uint64_t* b, uint32_t parity) {
+  if (barrier_try(b, parity)) return true;
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+  for (;;) {
+    for (int i = 0; i < 64; i++)
+      if (barrier_try(b, parity)) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (now - start > kServingWaitNs) return false;
+  }
+}
+
+// The same for a converged warp, all lanes polling: a branch that one lane takes, and coming back from it,
+// costs a waiting warp about 200 cycles.
+__device__ __forceinline__ bool barrier_wait_warp(uint64_t* b, uint32_t parity) {
+  if (__all_sync(0xffffffffu, barrier_try(b, parity))) return true;
+  uint64_t start, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+  for (;;) {
+    for (int i = 0; i < 64; i++)
+      if (__all_sync(0xffffffffu, barrier_try(b, parity))) return true;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (__any_sync(0xffffffffu, now - start > kServingWaitNs)) return false;
+  }
+}
+
+// Global -> shared bulk copy whose bytes are counted on `bar`.
+__device__ __forceinline__ void copy_bulk(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(shared_address(to)),
+      "l"(from), "r"(bytes), "r"(shared_address(bar))
+      : "memory");
+}
+
 inline size_t type_bytes(int32_t type) { return type == NEEDLE_TYPE_F32 ? 4 : 2; }
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }

@@ -25,7 +25,7 @@ NUMERICS_EXACT = 0
 NUMERICS_FAST = 1
 NUMERICS_FAST_ATTENTION = 2
 NOALLOC_MAX_FLOATS = 1 << 20  # NEEDLE_NOALLOC_MAX_FLOATS
-WAIT_ATTENTION, WAIT_TABLE_GEMV, WAIT_TENSOR_GEMM, WAIT_SELFTEST = 1, 2, 4, 8  # NEEDLE_WAIT_*
+WAIT_ATTENTION, WAIT_TABLE_GEMV, WAIT_TENSOR_GEMM, WAIT_SELFTEST, WAIT_LOGITS = 1, 2, 4, 8, 16  # NEEDLE_WAIT_*
 
 
 class NeedleError(RuntimeError):

@@ -515,6 +515,33 @@ def test_logits_rules_in_place_and_single_rules(torch):
         np.testing.assert_array_equal(d.cpu().numpy(), np.where(allowed, ruled, -np.inf).astype(np.float32))
 
 
+def test_logits_rows_whose_last_part_is_empty_in_some(torch):
+    """Rows an odd stride apart begin at every place of a 16-byte unit; with parts of 4096 ids (long lists) a row
+    of 4096 ids has a second part only where it does not begin on a boundary.  Several rows a CTA."""
+    from needle_b200 import native
+    rows, v, stride, listed = 700, 4096, 4097, 5000
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(rows, stride, generator=g)
+    history = torch.randint(0, v, (rows, listed), generator=g, dtype=torch.int32)
+    lengths = torch.randint(0, 40, (rows,), generator=g, dtype=torch.int32)
+    lengths[5] = listed
+    d = x.cuda()
+    rules = {"history": history.cuda(), "history_lengths": lengths.cuda(), "frequency": torch.full((rows,), 0.5).cuda(),
+             "presence": torch.full((rows,), 0.25).cuda()}
+    ruled = x[:, :v].numpy().copy()
+    for r in range(rows):
+        ids, times = np.unique(history[r, :lengths[r]].numpy(), return_counts=True)
+        ruled[r, ids] = ruled[r, ids] - np.float32(0.5) * times.astype(np.float32) - np.float32(0.25)
+    a = rules_args(torch, "f32", d[:, :v], rules)
+    ids, lps = torch.zeros(rows, dtype=torch.int32).cuda(), torch.zeros(rows).cuda()
+    native.check(native.lib().needle_cuda_logits_select_dev(C.byref(a), ids.data_ptr(), lps.data_ptr(), stream_of(torch)))
+    out = torch.zeros(rows, v).cuda()
+    native.check(native.lib().needle_cuda_logits_rules_dev(C.byref(a), out.data_ptr(), v, stream_of(torch)))
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(out.cpu().numpy(), ruled)
+    np.testing.assert_array_equal(ids.cpu().numpy(), ruled.argmax(1))
+
+
 def test_logits_select_odd_values(torch):
     """NaN never wins, -0 ties with +0, a row of -inf takes the lowest allowed id, the type's lowest value is
     a value like any other."""
