@@ -22,7 +22,8 @@
 // Groups of more than 4 heads (NG 2) use every converted code twice.  With heads on the M side, where 2 of
 // 16 rows were of use for 2 heads, the kernel took 1.6 times the instructions.
 // A unit (row, KV head, 8 heads, split of the positions) has a CTA of 2 to 8 warps, merged in shared memory, or,
-// where units are many, one warp, beside those of the row's other KV heads: caches of one age end together; splits and the prefix's parts are merged from the workspace.
+// where units are many, one warp, beside those of the row's other KV heads: caches of one age end together.
+// Splits and the prefix's parts are merged from the workspace.
 #include <algorithm>
 #include <cmath>
 
@@ -519,20 +520,31 @@ __global__ void __launch_bounds__(kStreamThreads) k_attend_merge(const __grid_co
   if (lane == 0 && a.lse) a.lse[at] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
-// Warps that fill the GPU, at 16 an SM.
+// Warps that fill the GPU, 16 an SM: below them a unit gets more warps.  300 rows x 4 KV heads of 64, 64 + up to 700
+// positions: 22.3 us, 27.8 us with 8 an SM, 20.7 us with 32; 600 rows x 64 + 300: 21.1, 21.4, 22.7 us.
 constexpr int kFullWarps = 148 * 16;
-// Positions below which a warp's share is not worth a further split.
-constexpr int kLeastSplit = 256;
+// Positions below which a split is not worth its merge (a launch, about 3 us), and the warps that splits are made
+// for.  One row of 4 KV heads over 8448 positions: 11.9 us with splits of 512, 12.5 us of 1024, 15.8 us of 2048;
+// over 1280: 9.0 us in two splits, 7.8 us in one.  Over 64000: 21.8 us with 8 warps an SM, 24.3 us with 4, 28 us with
+// 16 (twice the parts to merge).
+constexpr int kLeastSplit = 768;
+constexpr int kSplitWarps = 148 * 8;
 
-// Rows (times heads of a KV head) and prefix positions from which the prefix goes to k_attend_prefix.
-constexpr int64_t kPrefixLeastRows = 64, kPrefixLeastPositions = 128;
+// When the prefix goes to k_attend_prefix, whose launch, partial results and merge take about 4 us (packed rows = rows
+// times heads of a KV head).  By scores, packed rows x positions, heads of 64, 4 KV heads (stream, prefix kernel):
+// 128 x 256: 7.3, 9.8 us; 64 x 1024: 11.4, 10.6 us; 128 x 1024: 12.1, 12.5 us; 128 x 4096: 29.7, 16.0 us; heads of 128,
+// 8 KV heads: 256 x 128: 22.7, 32 us; 64 x 1024: 19.2, 17.5 us; 256 x 4096: 114, 42.9 us.  By positions, 8192 packed
+// rows: x 64: 79, 75 us; 2048: x 64: 28.1, 31.2 us, x 127: 34.0, 31.5 us.  By rows: 16 x 4096: 11.5, 12.5 us; 32 x
+// 4096: 14.6, 14.4 us.
+constexpr int64_t kPrefixLeastRows = 32, kPrefixLeastPositions = 96, kPrefixLeastScores = 65536;
 
 StreamPlan plan_for(const needle_prefix_attention& a) {
   StreamPlan p{};
   const int group = a.heads / a.kv_heads;
   p.groups = (group + kGroupHeads - 1) / kGroupHeads;
   const int64_t packed = int64_t(a.rows) * group;
-  if (packed >= kPrefixLeastRows && a.prefix_length >= kPrefixLeastPositions) {
+  if (packed >= kPrefixLeastRows && a.prefix_length >= kPrefixLeastPositions &&
+      packed * a.prefix_length >= kPrefixLeastScores) {
     // parts of the prefix: as many as keep the waves of CTAs short, each costing about 6 tiles on top
     const int nt = prefix_tile();
     const int tiles = (a.prefix_length + nt - 1) / nt;
@@ -557,13 +569,13 @@ StreamPlan plan_for(const needle_prefix_attention& a) {
     p.warps *= 2;
     p.warps_log2++;
   }
-  p.together = 1;
+  p.together = 1;  // 4096 rows x 4 KV heads, 160 + 256 positions: 76.7 us with a row's four units in a CTA, 80.1 us apart
   if (p.warps == 1)
     for (int k = 2; k <= kStreamWarps; k++)
       if (a.kv_heads * p.groups % k == 0 && units / k >= kFullWarps) p.together = k;
   // the longest splits that still give every SM its warps
   int64_t splits = 1;
-  if (p.warps == kStreamWarps) splits = std::max<int64_t>(1, std::min(kFullWarps / (units * p.warps), positions / kLeastSplit));
+  if (p.warps == kStreamWarps) splits = std::max<int64_t>(1, std::min(kSplitWarps / (units * p.warps), positions / kLeastSplit));
   p.split_len = int(std::min<int64_t>((positions + splits - 1) / splits, 0x40000000));
   p.split_len = std::max(kBlock, (p.split_len + kBlock - 1) / kBlock * kBlock);
   p.splits = int(std::max<int64_t>(1, (positions + p.split_len - 1) / p.split_len));
