@@ -156,6 +156,38 @@ def test_rope_append(torch, name, tokens, heads, kv_heads, dim, rotary, interlea
         assert torch.equal(out.cpu().view(tokens, kv_heads, dim), stands_for)
 
 
+@pytest.mark.parametrize("tokens", [500, 1000, 1777, 3553])
+@pytest.mark.parametrize("name,heads,kv_heads,dim,rotary,interleaved,norm,fused", [
+    ("f32", 3, 1, 64, 64, False, True, True), ("bf16", 5, 2, 64, 32, True, False, False), ("f16", 2, 3, 128, 128, False, True, True),
+    ("f32", 1, 1, 128, 2, True, True, True), ("bf16", 7, 1, 128, 128, True, True, True)])
+def test_rope_append_tokens_shared_by_fewer_warps(torch, name, tokens, heads, kv_heads, dim, rotary, interleaved, norm, fused):
+    """Batches from which a token is shared by four warps, two, and one, the last ones not filling a CTA."""
+    test_rope_append(torch, name, tokens, heads, kv_heads, dim, rotary, interleaved, norm, fused)
+
+
+def test_rope_append_codes_next_to_a_border(torch):
+    """Values of half a step and of whole ones: the quotients that binary32 cannot place are divided exactly."""
+    d = 128
+    x = torch.zeros(3, d)
+    x[0] = torch.arange(d) - 63.5   # top 63.5: codes 2 x, and the scale is 0.5
+    x[1] = (torch.arange(d) - 64.0) * 0.5
+    x[1, 0] = 127.0                 # halves of a step of 1: ties to even
+    x[2] = torch.randn(d, generator=torch.Generator().manual_seed(1))
+    x[2, 7], x[2, 8], x[2, 9] = 4.0, 2.0, -2.0  # top and half of it: 63.5 steps
+    for name in TYPES:
+        v = x.to(dtype_of(torch, name)).cuda()
+        cache = [torch.zeros(1, 1, 3, d, dtype=torch.int8).cuda(), torch.zeros(1, 1, 3).cuda(),
+                 torch.zeros(1, 1, 3, d, dtype=torch.int8).cuda(), torch.zeros(1, 1, 3).cuda()]
+        at = torch.arange(3, dtype=torch.int32).cuda()
+        rope_call(torch, name, v, v, v, torch.zeros_like(v), None, None, None, None, at * 0, at * 0, at, cache, 1, 1, d, 0,
+                  False, [], 1.0)
+        torch.cuda.synchronize()
+        codes, scales = quantised(to_numpy(v))
+        for k in (0, 2):
+            np.testing.assert_array_equal(cache[k][0, 0].cpu().numpy(), codes)
+            np.testing.assert_array_equal(cache[k + 1][0, 0].cpu().numpy(), scales)
+
+
 def test_rope_append_in_place_and_next_to_each_other(torch):
     """q_out = q, k_out = k, v_out = v inside one fused buffer give what separate outputs give."""
     g = torch.Generator().manual_seed(4)
@@ -320,6 +352,31 @@ def test_prefix_attention_many_rows(torch, name, rows, heads, kv_heads, dim, pre
     """Batches whose rows share the prefix in tiles, with tiles and prefixes that end raggedly."""
     g = np.random.default_rng(rows)
     check_attention(torch, name, rows, heads, kv_heads, dim, prefix_length, 40, g.integers(0, 41, rows).tolist())
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,prefix_length", [
+    (130, 8, 4, 64, 300), (400, 4, 2, 64, 129), (513, 8, 4, 64, 128), (40, 32, 4, 128, 500), (32, 4, 4, 128, 2049),
+    (700, 2, 2, 128, 97), (11, 24, 4, 64, 1000)])
+def test_prefix_attention_enough_scores_for_the_dense_prefix(torch, name, rows, heads, kv_heads, dim, prefix_length):
+    """65536 scores a KV head and more; packed rows that fill a tile, end inside one, or are fewer than one."""
+    g = np.random.default_rng(rows)
+    check_attention(torch, name, rows, heads, kv_heads, dim, prefix_length, 24, g.integers(0, 25, rows).tolist())
+
+
+def test_prefix_attention_dense_prefix_padding_scales_and_strides(torch):
+    rows = 170
+    slots = [(5 * r) % 4 for r in range(rows)]
+    slots[1], slots[3], slots[-1] = -1, 4, 1 << 30
+    counts = [(7 * r) % 19 - 2 for r in range(rows)]
+    counts[2] = 1 << 30
+    check_attention(torch, "f32", rows, 8, 4, 64, 210, 16, counts, slots=slots, slot_count=4)
+    check_attention(torch, "bf16", rows, 8, 4, 64, 210, 16, [0] * rows, slots=[-1] * rows, slot_count=4)
+    for scale in (1e-3, 0.5):
+        check_attention(torch, "f16", rows, 8, 4, 64, 200, 12, [5] * rows, scale=scale, odd=True)
+    check_attention(torch, "f32", rows, 8, 4, 64, 300, 12, [5] * rows, spread=30.0)
+    check_attention(torch, "f32", rows, 8, 4, 64, 300, 12, [5] * rows, spread=1e-4)
+    check_attention(torch, "bf16", rows, 8, 4, 64, 300, 12, [5] * rows, spread=1000.0)
 
 
 @pytest.mark.parametrize("name", TYPES)
@@ -707,6 +764,66 @@ def test_decode_step_captured_and_replayed(torch, rows):
     for s, w in zip(states, wanted):
         for a, b in zip([s[k] for k in OUTPUTS] + s["cache"], w):
             assert torch.equal(a, b)
+
+
+def test_dense_prefix_captured_and_replayed_beside_each_other(torch):
+    """Steps whose prefix is long enough for the dense product: two graphs at the same time on two streams,
+    and an eager step between them, give what each gives alone."""
+    states = [decode_state(torch, 70, 80 + i, prefix_length=700) for i in range(3)]
+    wanted = []
+    for s in states:
+        decode_step(torch, s)
+        torch.cuda.synchronize()
+        wanted.append([s[k].clone() for k in OUTPUTS])
+    graphs = []
+    for s in states[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            decode_step(torch, s)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in states:
+        for k in OUTPUTS:
+            s[k].zero_()
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            decode_step(torch, states[2])
+    torch.cuda.synchronize()
+    for s, w in zip(states, wanted):
+        assert all(torch.equal(a, s[k]) for a, k in zip(w, OUTPUTS))
+
+
+def test_first_calls_of_a_process_captured(torch):
+    """The operators' first calls in a process may be captured ones."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = """
+import torch, sys
+sys.path[:0] = sys.argv[1:]
+import __graft_entry__ as entry
+entry.load()
+import test_gpu_serving_ops as t
+s = t.decode_state(torch, 70, 4, prefix_length=700)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    t.decode_step(torch, s)
+g.replay()
+torch.cuda.synchronize()
+first = [s[k].clone() for k in t.OUTPUTS]
+t.decode_step(torch, s)
+torch.cuda.synchronize()
+assert all(torch.equal(a, s[k]) for a, k in zip(first, t.OUTPUTS))
+print("captured first")
+"""
+    done = subprocess.run([sys.executable, "-c", code, os.path.dirname(here), here], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured first" in done.stdout, done.stderr[-2000:]
 
 
 def test_same_results_every_time(torch):
