@@ -331,7 +331,7 @@ int needle_cuda_attention_dev_fast(const float* q, const int8_t* key_codes, cons
  * needle_cuda_rope_append_dev -> needle_cuda_prefix_attention_dev -> ... ->
  * needle_cuda_logits_select_dev.  They run on `stream` without synchronising, allocate nothing and keep
  * nothing between calls, so they can be captured into CUDA graphs; the buffers, the stream and the
- * current device must belong together (a host pointer, or an output on another device, is refused with
+ * current device must belong together (a host pointer, or a buffer on another device, is refused with
  * BACKEND_UNAVAILABLE).  Lists of positions, slots, lengths and ids are device memory and are bounded in
  * the kernels: an index outside its range is left out, never followed. */
 
@@ -413,8 +413,9 @@ typedef struct needle_prefix_attention {
   int32_t type, rows, heads, kv_heads, head_dim /* 64 or 128 */, prefix_length, prefix_capacity, slot_count, capacity;
 } needle_prefix_attention;
 
-/* Bytes of workspace a call with these arguments needs.  Reads no device memory; depends only on the sizes,
- * so a caller may size it once for its largest batch and longest prefix. */
+/* Bytes of workspace a call with these arguments needs.  Reads no device memory; depends only on the sizes
+ * (type, rows, heads, prefix_length, capacity).  A smaller batch may need more, since it is split more: one
+ * workspace for several sizes is the largest of theirs. */
 int needle_cuda_prefix_attention_workspace(const needle_prefix_attention* args, size_t* bytes);
 
 /* `workspace`: 16-byte aligned device memory (NULL when none is needed), not read before it is written;

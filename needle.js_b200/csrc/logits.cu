@@ -662,7 +662,7 @@ LogitsPlan plan_for(const needle_logits_rules& a, int most_parts) {
   return p;
 }
 
-int check_rules(const needle_logits_rules* a, int* device, const char* op) {
+int check_rules(const needle_logits_rules* a) {
   if (!a) return refuse("null argument");
   if (a->type < NEEDLE_TYPE_F32 || a->type > NEEDLE_TYPE_BF16) return refuse("unknown element type");
   if (a->rows < 0 || a->vocab < 0) return refuse("bad row or vocabulary count");
@@ -671,22 +671,36 @@ int check_rules(const needle_logits_rules* a, int* device, const char* op) {
   if (a->vocab > 1 << 30) return refuse("at most 2^30 ids");
   if (!a->logits) return refuse("null argument");
   if (a->rows > 1 && a->logits_stride < a->vocab) return refuse("a row stride is shorter than its row");
-  if (!aligned_to(a->logits, type_bytes(a->type))) return refuse("a buffer is not aligned to its element type");
   if (a->history && (!a->history_lengths || a->history_stride < 0)) return refuse("history without lengths");
   if (a->bias_ids && (!a->bias_values || !a->bias_counts || a->bias_stride < 0))
     return refuse("bias ids without values or counts");
   if ((a->history && a->history_stride > 1 << 30) || (a->bias_ids && a->bias_stride > 1 << 30))
     return refuse("at most 2^30 history entries or biases a row");
   if (a->masks && (!a->mask_slots || a->mask_count < 0)) return refuse("masks without slots");
-  const cudaError_t e = cudaGetDevice(device);
-  if (e != cudaSuccess) return refuse_cuda(op, e);
-  return check_buffer(a->logits, "logits", *device);
+  return NEEDLE_OK;
 }
 
+// The buffers' alignment and device; gives the current device.
+int check_rules_buffers(const needle_logits_rules* a, Buffers outputs, int* device, const char* op) {
+  const Buffers buffers = {{a->logits, "logits", type_bytes(a->type)}, {a->history, "history", 4},
+                           {a->history_lengths, "history_lengths", 4}, {a->prompt_lengths, "prompt_lengths", 4},
+                           {a->repetition, "repetition", 4}, {a->presence, "presence", 4}, {a->frequency, "frequency", 4},
+                           {a->bias_ids, "bias_ids", 4}, {a->bias_values, "bias_values", 4}, {a->bias_counts, "bias_counts", 4},
+                           {a->masks, "masks", 4}, {a->mask_slots, "mask_slots", 4}};
+  if (int rc = check_alignment(buffers)) return rc;
+  if (int rc = check_alignment(outputs)) return rc;
+  const cudaError_t e = cudaGetDevice(device);
+  if (e != cudaSuccess) return refuse_cuda(op, e);
+  if (int rc = check_buffers(buffers, *device)) return rc;
+  return check_buffers(outputs, *device);
+}
+
+// Always the same limit, so that calls at the same time cannot lower each other's: rings, a table of kMostEntries
+// with their biases, and a bit an id of the largest part.
+constexpr size_t kMostSmem = kWarps * kStages * kSliceBytes + (kMostEntries * 2 + 36) * 12 + kPartIds / 8;
 template <class K>
-cudaError_t set_smem(K kernel, size_t bytes) {
-  return bytes <= 48 * 1024 ? cudaSuccess
-                            : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+cudaError_t set_smem(K kernel) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kMostSmem));
 }
 
 }  // namespace
@@ -696,19 +710,20 @@ using namespace needle;
 
 extern "C" int needle_cuda_logits_rules_dev(const needle_logits_rules* a, void* out, int64_t out_stride, void* stream) {
   return entry([&] {
-    int device = 0;
-    if (int rc = check_rules(a, &device, "logits_rules")) return rc;
+    if (int rc = check_rules(a)) return rc;
     if (a->rows == 0 || a->vocab == 0) return int(NEEDLE_OK);
     if (!out) return refuse("null argument");
     if (a->rows > 1 && out_stride < a->vocab) return refuse("a row stride is shorter than its row");
-    if (!aligned_to(out, type_bytes(a->type))) return refuse("a buffer is not aligned to its element type");
-    if (int rc = check_buffer(out, "out", device)) return rc;
+    if (a->rows > 1 && out == a->logits && out_stride != a->logits_stride)
+      return refuse("out may be logits only with the same row stride");
+    int device = 0;
+    if (int rc = check_rules_buffers(a, {{out, "out", type_bytes(a->type)}}, &device, "logits_rules")) return rc;
     if (check_wait_status(device) != NEEDLE_OK) return int(NEEDLE_BACKEND_UNAVAILABLE);
     const LogitsPlan plan = plan_for(*a, 1 << 30);
     const size_t smem = smem_bytes(*a, plan);
     const cudaError_t e = with_type(a->type, [&](auto zero) {
       using T = decltype(zero);
-      const cudaError_t err = set_smem(k_logits_rules<T>, smem);
+      const cudaError_t err = set_smem(k_logits_rules<T>);
       if (err != cudaSuccess) return err;
       k_logits_rules<T><<<dim3(plan.parts, rows_at_once(*a, smem, plan.parts)), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
           *a, plan, static_cast<T*>(out), out_stride, wait_status_words(device));
@@ -721,19 +736,19 @@ extern "C" int needle_cuda_logits_rules_dev(const needle_logits_rules* a, void* 
 extern "C" int needle_cuda_logits_select_dev(const needle_logits_rules* a, int32_t* ids, float* log_probabilities,
                                              void* stream) {
   return entry([&] {
-    int device = 0;
-    if (int rc = check_rules(a, &device, "logits_select")) return rc;
+    if (int rc = check_rules(a)) return rc;
     if (a->rows == 0) return int(NEEDLE_OK);
     if (a->vocab == 0) return refuse("an empty vocabulary has no id to select");
     if (!ids || !log_probabilities) return refuse("null argument");
-    if (int rc = check_buffer(ids, "ids", device)) return rc;
-    if (int rc = check_buffer(log_probabilities, "log_probabilities", device)) return rc;
+    int device = 0;
+    if (int rc = check_rules_buffers(a, {{ids, "ids", 4}, {log_probabilities, "log_probabilities", 4}}, &device, "logits_select"))
+      return rc;
     if (check_wait_status(device) != NEEDLE_OK) return int(NEEDLE_BACKEND_UNAVAILABLE);
     const LogitsPlan plan = plan_for(*a, 8);  // a row's CTAs are one cluster
     const size_t smem = smem_bytes(*a, plan);
     const cudaError_t e = with_type(a->type, [&](auto zero) {
       using T = decltype(zero);
-      const cudaError_t err = set_smem(k_logits_select<T>, smem);
+      const cudaError_t err = set_smem(k_logits_select<T>);
       if (err != cudaSuccess) return err;
       const int cluster = std::min(8, plan.parts);
       cudaLaunchAttribute attribute{};

@@ -671,19 +671,27 @@ extern "C" int needle_cuda_prefix_attention_dev(const needle_prefix_attention* a
     if (a->rows > 1 && (a->q_stride < width || a->out_stride < width))
       return refuse("a row stride is shorter than its row");
     const size_t element = type_bytes(a->type);
-    if (!aligned_to(a->q, element) || !aligned_to(a->out, element))
-      return refuse("a buffer is not aligned to its element type");
-    for (const void* p : {a->prefix_key_codes, a->prefix_value_codes, a->key_codes, a->value_codes})
-      if (!aligned_to(p, 16)) return refuse("key/value codes must be 16-byte aligned");
     const StreamPlan plan = plan_for(*a);
     const size_t need = workspace_bytes_for(*a, plan);
+    const bool prefix = a->prefix_length > 0, own = a->capacity > 0 && a->slot_count > 0;  // else never read
+    const Buffers buffers = {{a->q, "q", element}, {a->out, "out", element}, {a->lse, "lse", 4}, {a->slots, "slots", 4},
+                             {a->counts, "counts", 4}, {need > 0 ? workspace : nullptr, "workspace", 1},
+                             {prefix ? a->prefix_key_codes : nullptr, "prefix_key_codes", 1},
+                             {prefix ? a->prefix_key_scales : nullptr, "prefix_key_scales", 4},
+                             {prefix ? a->prefix_value_codes : nullptr, "prefix_value_codes", 1},
+                             {prefix ? a->prefix_value_scales : nullptr, "prefix_value_scales", 4},
+                             {own ? a->key_codes : nullptr, "key_codes", 1}, {own ? a->key_scales : nullptr, "key_scales", 4},
+                             {own ? a->value_codes : nullptr, "value_codes", 1},
+                             {own ? a->value_scales : nullptr, "value_scales", 4}};
+    if (int rc = check_alignment(buffers)) return rc;
+    for (const void* p : {a->prefix_key_codes, a->prefix_value_codes, a->key_codes, a->value_codes})
+      if (!aligned_to(p, 16)) return refuse("key/value codes must be 16-byte aligned");
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16)))
       return refuse("the workspace must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return refuse_cuda("prefix_attention", e);
-    if (int rc = check_buffer(a->out, "out", device)) return rc;
-    if (int rc = check_buffer(a->q, "q", device)) return rc;
+    if (int rc = check_buffers(buffers, device)) return rc;
     if (check_wait_status(device) != NEEDLE_OK) return int(NEEDLE_BACKEND_UNAVAILABLE);
     uint32_t* words = wait_status_words(device);
     const float scale = a->scale > 0.0f ? a->scale : 1.0f / std::sqrt(float(a->head_dim));

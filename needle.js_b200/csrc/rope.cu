@@ -383,8 +383,12 @@ extern "C" int needle_cuda_rope_append_dev(const needle_rope_append* a, const do
                           (a->v_out && a->v_out_stride < a->kv_heads * d)))
       return refuse("a row stride is shorter than its row");
     const size_t e = type_bytes(a->type);
-    for (const void* p : {a->q, a->k, a->v, (const void*)a->q_out, (const void*)a->k_out, (const void*)a->v_out})
-      if (!aligned_to(p, e)) return refuse("a buffer is not aligned to its element type");
+    const Buffers buffers = {{a->q, "q", e}, {a->k, "k", e}, {a->v, "v", e}, {a->q_out, "q_out", e}, {a->k_out, "k_out", e},
+                             {a->v_out, "v_out", e}, {a->q_norm, "q_norm", 4}, {a->k_norm, "k_norm", 4},
+                             {a->positions, "positions", 4}, {a->slots, "slots", 4}, {a->entries, "entries", 4},
+                             {a->key_codes, "key_codes", 1}, {a->key_scales, "key_scales", 4},
+                             {a->value_codes, "value_codes", 1}, {a->value_scales, "value_scales", 4}};
+    if (int rc = check_alignment(buffers)) return rc;
     if (!aligned_to(a->key_codes, 16) || !aligned_to(a->value_codes, 16))
       return refuse("key/value codes must be 16-byte aligned");
     RopeArgs args{};
@@ -397,8 +401,7 @@ extern "C" int needle_cuda_rope_append_dev(const needle_rope_append* a, const do
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return refuse_cuda("rope_append", err);
-    if (int rc = check_buffer(a->q_out, "q_out", device)) return rc;
-    if (int rc = check_buffer(a->key_codes, "key_codes", device)) return rc;
+    if (int rc = check_buffers(buffers, device)) return rc;
     err = launch_rope(args, static_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? int(NEEDLE_OK) : refuse_cuda("rope_append", err);
   });

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/needle_cuda.h"
@@ -120,6 +121,27 @@ inline int check_buffer(const void* p, const char* name, int device) {
   if (a.type == cudaMemoryTypeDevice && a.device != device)
     return refuse(std::string(name) + " is on device " + std::to_string(a.device) + ", the current device is " +
                   std::to_string(device));
+  return NEEDLE_OK;
+}
+
+// A device buffer of a call (NULL: not given) and the bytes its elements are aligned to.
+struct Buffer {
+  const void* p;
+  const char* name;
+  size_t element;
+};
+using Buffers = std::initializer_list<Buffer>;
+
+inline int check_alignment(Buffers buffers) {
+  for (const Buffer& b : buffers)
+    if (!aligned_to(b.p, b.element)) return refuse(std::string(b.name) + " is not aligned to its element type");
+  return NEEDLE_OK;
+}
+
+inline int check_buffers(Buffers buffers, int device) {
+  for (const Buffer& b : buffers)
+    if (b.p)
+      if (int rc = check_buffer(b.p, b.name, device)) return rc;
   return NEEDLE_OK;
 }
 

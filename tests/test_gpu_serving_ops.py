@@ -846,3 +846,62 @@ def test_host_buffers_are_refused(torch):
             native.check(native.lib().needle_cuda_logits_rules_dev(C.byref(a), o.data_ptr(), 64, None))
         assert e.value.code == "BACKEND_UNAVAILABLE" and "not device memory" in str(e.value)
     torch.cuda.synchronize()
+
+
+def test_host_lists_are_refused(torch):
+    """A list in host memory is refused before anything is launched, whichever it is."""
+    from needle_b200 import native
+    s = decode_state(torch, 4, 3, prefix_length=100)
+    decode_step(torch, s)
+    torch.cuda.synchronize()
+    for name in ("positions", "slots", "entries", "norm"):
+        with pytest.raises(native.NeedleError, match="not device memory"):
+            decode_step(torch, {**s, name: s[name].cpu()})
+    for name in ("counts", "slots"):
+        bad = {**s, name: s[name].cpu()}
+        with pytest.raises(native.NeedleError, match=name + " is not device memory"):
+            attention_call(torch, "f32", s["q_out"], s["out"], s["lse"], s["prefix"], s["cache"], bad["slots"], bad["counts"],
+                           8, 4, 64, 100, workspace=s["workspace"])
+    for name in s["rules"]:
+        rules = {**s["rules"], name: s["rules"][name].cpu()}
+        a = rules_args(torch, "f32", s["logits"], rules)
+        with pytest.raises(native.NeedleError, match=name + " is not device memory"):
+            native.check(native.lib().needle_cuda_logits_select_dev(C.byref(a), s["ids"].data_ptr(), s["lps"].data_ptr(),
+                                                                    stream_of(torch)))
+    torch.cuda.synchronize()
+
+
+def test_calls_from_two_threads_at_once(torch):
+    """Two host threads, each with its own stream and buffers and calls of different sizes, get what one gets."""
+    import threading
+    states = [[decode_state(torch, rows, seed, prefix_length=p, vocab=v) for rows, seed, p, v in sizes]
+              for sizes in (((2, 1, 100, 512), (70, 2, 700, 9000)), ((33, 3, 2000, 3001), (5, 4, 37, 20000)))]
+    wanted = []
+    for mine in states:
+        for s in mine:
+            decode_step(torch, s)
+            torch.cuda.synchronize()
+            wanted.append([s[k].clone() for k in OUTPUTS])
+            for k in OUTPUTS:
+                s[k].zero_()
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(mine):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    for s in mine:
+                        decode_step(torch, s)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(mine,)) for mine in states]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    for s, w in zip([s for mine in states for s in mine], wanted):
+        assert all(torch.equal(a, s[k]) for a, k in zip(w, OUTPUTS))

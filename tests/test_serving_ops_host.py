@@ -146,6 +146,34 @@ def test_logits_outputs_are_checked():
         assert rc != 0
 
 
+@pytest.mark.parametrize("name", ["q_norm", "k_norm", "positions", "slots", "entries", "key_scales", "value_scales", "k_out"])
+def test_rope_append_refuses_misaligned_lists(name):
+    refused(native.lib().needle_cuda_rope_append_dev(C.byref(rope_args(**{name: P + 2})), ONES, None), name + " is not aligned")
+
+
+@pytest.mark.parametrize("name", ["lse", "slots", "counts", "prefix_key_scales", "prefix_value_scales", "key_scales", "value_scales"])
+def test_prefix_attention_refuses_misaligned_lists(name):
+    a = attention_args(**{name: P + 2})
+    refused(native.lib().needle_cuda_prefix_attention_dev(C.byref(a), P, 1 << 40, None), name + " is not aligned")
+
+
+@pytest.mark.parametrize("name", ["history", "history_lengths", "prompt_lengths", "repetition", "presence", "frequency",
+                                  "bias_ids", "bias_values", "bias_counts", "masks", "mask_slots"])
+def test_logits_operators_refuse_misaligned_lists(name):
+    lists = dict.fromkeys(("history", "history_lengths", "bias_ids", "bias_values", "bias_counts", "masks", "mask_slots"), P)
+    a = logits_args(**{**lists, "history_stride": 4, "bias_stride": 4, "mask_count": 1, name: P + 1})
+    refused(native.lib().needle_cuda_logits_rules_dev(C.byref(a), P, 100, None), name + " is not aligned")
+    refused(native.lib().needle_cuda_logits_select_dev(C.byref(a), P, P, None), name + " is not aligned")
+
+
+def test_logits_outputs_are_refused():
+    a = logits_args(logits=P, logits_stride=120)
+    refused(native.lib().needle_cuda_logits_rules_dev(C.byref(a), P, 100, None), "same row stride")
+    refused(native.lib().needle_cuda_logits_rules_dev(C.byref(a), P + 2, 100, None), "out is not aligned")
+    refused(native.lib().needle_cuda_logits_select_dev(C.byref(a), P + 2, P, None), "ids is not aligned")
+    refused(native.lib().needle_cuda_logits_select_dev(C.byref(a), P, P + 1, None), "log_probabilities is not aligned")
+
+
 def _no_gpu():
     import torch
     return not torch.cuda.is_available()
