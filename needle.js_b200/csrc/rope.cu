@@ -15,14 +15,16 @@
 //
 // A warp reads kRows head rows at once, 16 bytes a lane, and works on one token (or a part of one, where there are
 // few): it computes the token's angles in binary64, leaves them in shared memory, and walks over the keys, the
-// values and the queries.  Bytes bound the operator (every row is read and written once), then instructions:
-// 88 for 256 query elements, about 250 for 256 key elements, of which the binary64 rotation and its conversions
-// are the larger part.  What paid, at 8191 tokens of 32 / 8 heads of 128 in bf16 (217 MB): 131 us with a CTA a
-// token and 8-byte accesses; 100 us with a warp a token; 64 us with the exact division only for quotients next to
-// a border, in a loop over them (it was inlined for every element and held registers), and accesses whose
-// width is known at compile time; 61.6 us = 3.5 TB/s, 54% of a copy's rate, with loads issued at the start of
-// each kind rather than all before the angles (fewer registers held).  4 resident CTAs of 64 registers: 3 take
-// 64 us, 5 take 72 us (spills).  4096 tokens of 8 / 4 heads of 64 in binary32 (36 MB): 13.4 us, 4 tokens: 3.3 us.
+// values and the queries, whose pieces come to a place of each lane in shared memory kAhead turns before they are
+// used (cp.async: a register a load in flight would cost resident warps).  Bytes bound the operator (every row is read
+// and written once), then instructions: about 90 for 256 query elements, 250 for 256 key elements, of which the
+// binary64 rotation and its conversions (quarter rate) are the larger part.
+// Measured, 8191 tokens of 32 / 8 heads of 128 in bf16 (217 MB): 131 us with a CTA a token and 8-byte accesses; 100 us
+// with a warp a token; 64 us with the exact division only for quotients next to a border, in a loop over them (inlined
+// for every element it held registers), and accesses whose width is known at compile time; 48 us = 4.5 TB/s, 69% of a
+// copy's rate, with the loads in shared memory (in registers: 61 us; 8 ahead instead of 4: 49 us).  4 resident CTAs of
+// 64 registers: 3 take 51 us, 5 take 60 us (spills).  4096 tokens of 8 / 4 heads of 64 in binary32 (36 MB): 14.6 us,
+// bound by conversions; 4 tokens: 3.5 us.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -38,11 +40,11 @@ constexpr int kRopeWarps = kRopeThreads / 32;
 constexpr int kMaxPairs = 64;        // rotated pairs of a head of 128
 constexpr int kRopeFill = 148 * 3;   // CTAs that keep the GPU busy (148 * 6: as fast; 148 * 12: 4096 tokens 14 -> 19 us)
 constexpr int kRopeResident = 4;     // CTAs of an SM
-constexpr int kQueriesAhead = 4;     // query loads of a lane in flight
+constexpr int kAhead = 4;            // 16-byte loads of a lane in flight
 
-// What a kernel is built for, E being the elements of a lane: pairs (2i, 2i + 1), rotary_dim a multiple of E, and
-// 16-byte accesses; pairs (i, i + half), half a multiple of E (a lane's partners are then one lane), and 16-byte
-// accesses; or any pairs and any alignment.
+// What a kernel is built for, E being the elements of a lane: pairs (2i, 2i + 1) and 16-byte accesses; pairs
+// (i, i + half), half a multiple of E (a lane's partners are then one lane), and 16-byte accesses; or any pairs and
+// any alignment.
 enum Form { kInterleaved, kHalves, kAny };
 
 struct RopeArgs {
@@ -70,12 +72,13 @@ struct Turn {
   const Angle* angles;  // of the token
   Angle kept[kKept ? kAngles : 1];
   int sub, half, other, pair0;
-  bool normed, interleaved, first, turns;
+  bool normed, interleaved, first, turns, whole;  // whole: all of the lane's elements turn
 
   __device__ __forceinline__ Turn(bool normed, const A* factors, const Angle* angles, int sub, int rotary, bool interleaved)
       : factors(factors + sub * E), angles(angles), sub(sub), half(rotary >> 1), normed(normed), interleaved(interleaved) {
     const int e0 = sub * E;
     turns = e0 < rotary;
+    whole = e0 + E <= rotary;
     first = e0 < half;
     other = first ? sub + half / E : sub - half / E;
     pair0 = FORM == kInterleaved ? e0 / 2 : first ? e0 : e0 - half;
@@ -113,9 +116,13 @@ struct Turn {
       }
     }
     if (FORM == kInterleaved) {
-      if (turns) {
+      if (whole) {
 #pragma unroll
         for (int i = 0; i < E; i += 2) turn_pair(x[i], x[i + 1], angle(i / 2));
+      } else if (turns) {
+#pragma unroll
+        for (int i = 0; i < E; i += 2)
+          if (sub * E + i < 2 * half) turn_pair(x[i], x[i + 1], angle(i / 2));
       }
     } else if (FORM == kHalves) {
       float y[E];
@@ -160,18 +167,6 @@ struct Turn {
 };
 
 template <class T, int E, int FORM>
-__device__ __forceinline__ Vec<T, E> load_piece(const T* p) {
-  if constexpr (FORM != kAny) {
-    return *reinterpret_cast<const Vec<T, E>*>(p);
-  } else {
-    Vec<T, E> v;
-#pragma unroll
-    for (int i = 0; i < E; i++) v.v[i] = p[i];
-    return v;
-  }
-}
-
-template <class T, int E, int FORM>
 __device__ __forceinline__ void store_piece(T* p, const float (&x)[E]) {
   Vec<T, E> v;
   if constexpr (sizeof(T) == 4) {
@@ -207,6 +202,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
   __shared__ float2 angles32[kNarrow ? kRopeWarps : 1][kMaxPairs];
   __shared__ alignas(16) double k_factors[D];
   __shared__ alignas(16) Query q_factors[D];
+  __shared__ Piece pieces[FORM == kAny ? 1 : kAhead][kRopeThreads];  // each lane's own
   const needle_rope_append& a = args.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / kLanes, sub = lane % kLanes;
   const int parts = args.parts, mine = warp / parts, part = warp % parts;
@@ -215,16 +211,44 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
   const int step = parts * kRows;  // heads a turn
   // the first head of this warp, of each kind: few heads are spread over the warps
   const int q0 = part * kRows, k0 = (parts - 1 - part) * kRows, v0 = (part + parts / 2) % parts * kRows;
-  auto load = [&](const void* base, int64_t stride, int head, int heads) {
-    Piece v{};
-    if (head + group < heads)
-      v = load_piece<T, E, FORM>(static_cast<const T*>(base) + token * stride + (int64_t)(head + group) * D + sub * E);
-    return v;
+  // The warp's turns: its key rows, its value rows, its query rows.
+  auto turns_of = [&](int head, int heads) { return (max(heads - head, 0) + step - 1) / step; };
+  const int k_turns = turns_of(k0, a.kv_heads), kv_turns = k_turns + turns_of(v0, a.kv_heads);
+  const int turns = kv_turns + turns_of(q0, a.heads);
+  // The lane's elements of a turn, NULL where the group has no row.
+  auto piece_of = [&](int turn) -> const T* {
+    const bool key = turn < k_turns, query = turn >= kv_turns;
+    const int head = group + (key ? k0 + turn * step : query ? q0 + (turn - kv_turns) * step : v0 + (turn - k_turns) * step);
+    if (head >= (query ? a.heads : a.kv_heads)) return nullptr;
+    const void* base = key ? a.k : query ? a.q : a.v;
+    return static_cast<const T*>(base) + token * (key ? a.k_stride : query ? a.q_stride : a.v_stride) + (int64_t)head * D + sub * E;
   };
-  Piece qs[kQueriesAhead], ks[1], vs[1];
+  auto ask = [&](int turn) {
+    if constexpr (FORM != kAny) {
+      const T* p = turn < turns ? piece_of(turn) : nullptr;
+      if (p)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(&pieces[turn % kAhead][threadIdx.x])),
+                     "l"(p)
+                     : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  auto take = [&](int turn, float (&x)[E]) {
+    Piece v{};
+    if constexpr (FORM != kAny) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+      v = pieces[turn % kAhead][threadIdx.x];  // (of no use where the group has no row)
+      ask(turn + kAhead);
+    } else if (const T* p = piece_of(turn)) {
+#pragma unroll
+      for (int i = 0; i < E; i++) v.v[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < E; i++) x[i] = to_f32(v.v[i]);
+  };
   int64_t at = -1;
   if (live) {
-    ks[0] = load(a.k, a.k_stride, k0, a.kv_heads);  // on its way while the angles are computed
+    for (int turn = 0; turn < kAhead; turn++) ask(turn);  // on their way while the angles are computed
     const int slot = a.slots[token], entry = a.entries[token];
     if (slot >= 0 && slot < a.slot_count && entry >= 0 && entry < a.capacity)
       at = (int64_t)slot * a.kv_heads * a.capacity + entry;
@@ -247,6 +271,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
     __syncwarp();
   if (!live) return;
 
+  int turn = 0;
   auto keep = [&](float (&x)[E], int head, int8_t* codes, float* scales, void* out, int64_t stride) {
     float top = 0.0f;
 #pragma unroll
@@ -291,32 +316,19 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
     }
     if (out) store_piece<T, E, FORM>(static_cast<T*>(out) + token * stride + (int64_t)(head + group) * D + sub * E, x);
   };
-  // body(x, head) for the heads of a kind, the loads of the next ones in flight.
-  auto walk = [&](auto& ahead, const void* base, int64_t stride, int head, int heads, auto body) {
-    constexpr int kAhead = sizeof(ahead) / sizeof(Piece);
-    for (;;) {
-#pragma unroll
-      for (int j = 0; j < kAhead; j++) {
-        if (head >= heads) return;
-        float x[E];
-#pragma unroll
-        for (int i = 0; i < E; i++) x[i] = to_f32(ahead[j].v[i]);
-        ahead[j] = load(base, stride, head + kAhead * step, heads);
-        body(x, head);
-        head += step;
-      }
-    }
-  };
   const Turn<double, D, E, FORM> turn_key(a.k_norm != nullptr, k_factors, angles[mine], sub, a.rotary_dim,
                                           a.interleaved);
-  walk(ks, a.k, a.k_stride, k0, a.kv_heads, [&](float (&x)[E], int head) {
+  for (int head = k0; head < a.kv_heads; head += step, turn++) {
+    float x[E];
+    take(turn, x);
     turn_key(x);
     keep(x, head, a.key_codes, a.key_scales, a.k_out, a.k_out_stride);
-  });
-  vs[0] = load(a.v, a.v_stride, v0, a.kv_heads);
-  walk(vs, a.v, a.v_stride, v0, a.kv_heads, [&](float (&x)[E], int head) {
+  }
+  for (int head = v0; head < a.kv_heads; head += step, turn++) {
+    float x[E];
+    take(turn, x);
     keep(x, head, a.value_codes, a.value_scales, a.v_out, a.v_out_stride);
-  });
+  }
   const auto* query_angles = [&] {
     if constexpr (kNarrow)
       return angles32[mine];
@@ -324,13 +336,13 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
       return angles[mine];
   }();
   const Turn<Query, D, E, FORM> turn_query(a.q_norm != nullptr, q_factors, query_angles, sub, a.rotary_dim, a.interleaved);
-#pragma unroll
-  for (int i = 0; i < kQueriesAhead; i++) qs[i] = load(a.q, a.q_stride, q0 + i * step, a.heads);
-  walk(qs, a.q, a.q_stride, q0, a.heads, [&](float (&x)[E], int head) {
+  for (int head = q0; head < a.heads; head += step, turn++) {
+    float x[E];
+    take(turn, x);
     turn_query(x);
     if (head + group < a.heads)
       store_piece<T, E, FORM>(static_cast<T*>(a.q_out) + token * a.q_out_stride + (int64_t)(head + group) * D + sub * E, x);
-  });
+  }
 }
 
 cudaError_t launch_rope(RopeArgs& args, cudaStream_t s) {
@@ -346,7 +358,8 @@ cudaError_t launch_rope(RopeArgs& args, cudaStream_t s) {
   return with_type(a.type, [&](auto zero) {
     using T = decltype(zero);
     auto go = [&](auto* interleaved, auto* halves, auto* any) {
-      auto* kernel = !all_wide || (a.interleaved ? 2 : 1) * half % (16 / e) != 0 ? any : a.interleaved ? interleaved : halves;
+      // (one pair is the same pair either way)
+      auto* kernel = !all_wide ? any : a.interleaved || half == 1 ? interleaved : half % (16 / e) == 0 ? halves : any;
       kernel<<<grid, kRopeThreads, 0, s>>>(args);
       return cudaGetLastError();
     };

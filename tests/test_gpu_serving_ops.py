@@ -165,6 +165,15 @@ def test_rope_append_tokens_shared_by_fewer_warps(torch, name, tokens, heads, kv
     test_rope_append(torch, name, tokens, heads, kv_heads, dim, rotary, interleaved, norm, fused)
 
 
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,rotary,interleaved", [
+    (5, 3, 2, 64, 2, False), (400, 3, 2, 64, 2, False), (9, 2, 1, 128, 2, True), (9, 4, 1, 64, 6, True), (7, 1, 2, 128, 10, True),
+    (7, 1, 2, 128, 10, False), (6, 2, 2, 64, 0, True)])
+def test_rope_append_few_rotated_dimensions(torch, name, tokens, heads, kv_heads, dim, rotary, interleaved):
+    """Rotations that end inside a lane's elements, in rows that allow wide accesses."""
+    test_rope_append(torch, name, tokens, heads, kv_heads, dim, rotary, interleaved, True, True)
+
+
 def test_rope_append_codes_next_to_a_border(torch):
     """Values of half a step and of whole ones: the quotients that binary32 cannot place are divided exactly."""
     d = 128
