@@ -15,11 +15,10 @@
 // a part through a ring of its own in shared memory, filled by bulk copies that run on over the ends of parts
 // and rows: the copies never pause, and no barrier is needed for them.
 //
-// Bytes bound the stream, the lists' chains of dependent accesses the rest.  Without rules, 512 rows of 50001 bf16 ids
-// (102 MB) take 17 us, a copy's rate; with histories of up to 1000 ids, 50 biases and masks 42 us (2.4 TB/s of
-// logits).  Select: 4096 rows of 8192 binary32 ids with histories of 256: 61 us (2.2 TB/s), 37 us without rules;
+// Bytes bound the stream, the lists' chains of dependent accesses the rest.  512 rows of 50001 bf16 ids (102 MB) with
+// histories of up to 1000 ids, 50 biases and masks take 32 us, 23 us without rules.  Select: 4096 rows of 8192 binary32 ids with histories of 256: 61 us (2.2 TB/s), 37 us without rules;
 // 200 rows of 128000 fp16 ids with histories of 2000: 46 us (1.1 TB/s; each of a row's two CTAs builds a table).
-// Measured beside it: chunks of a row in registers, direct tables of counts instead of the hash, one CTA a chunk:
+// Measured beside it (the three sizes, before the rules had list warps: 42, 61, 46 us): chunks of a row in registers, direct tables of counts instead of the hash, one CTA a chunk:
 // 47, 72, 63 us; the hash twice as large as its list (5/4: 50, 66, 55 us, probes; 4 times: 71, 66, 129 us, fewer
 // CTAs resident); one warp a row: 110 us for the 4096 rows (too few warps hide the lists' latency); parts of 32 KB
 // in shared memory with the lists ruled there, 8 warps: 51, 81, 85 us (every warp repeats a part's fixed work).
@@ -38,16 +37,17 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnits = 4;                        // 16-byte units of a thread in a step of the stream
-constexpr int kStages = 2;                       // steps of a warp's ring
-constexpr int kSliceBytes = 32 * kUnits * 16;    // of a warp in a step
+constexpr int kRingBytes = kWarps * 32 * 16 * 8;  // of a CTA: eight 16-byte units a thread, in two steps or four
 constexpr int kPartIds = 65536;                  // most ids of a part: 8 KB of bits
 constexpr int kListIds = 2;                      // list ids of a thread loaded at once
 constexpr int kMostEntries = 4096;               // hash entries of a part; a part of as many ids never has more
 
-__host__ __device__ constexpr int step_ids(size_t element) { return kWarps * kSliceBytes / int(element); }
+// Ids of a step of the stream with `units` 16-byte units a thread.
+__host__ __device__ constexpr int step_ids(size_t element, int units) { return kThreads * units * 16 / int(element); }
+constexpr int kRulesUnits = 2, kSelectUnits = 4;
 // CTAs of an SM by their registers: a thread holds 16 binary32 logits of a step, or 32 of 16 bits.
 __host__ __device__ constexpr int resident(size_t element) { return element == 4 ? 6 : 4; }
+constexpr int kRulesResident = 4;  // of k_logits_rules, with its list warps
 
 // The hash table of a part's ids with a rule.  word: bit 31 the mask allows the id, bit 0 it is in the prompt,
 // bits 1..30 how often it was answered.
@@ -139,16 +139,19 @@ __device__ __forceinline__ RowRules row_rules(const needle_logits_rules& a, int6
   return r;
 }
 
-// Slot of an id of the part (claimed for it when it has none yet).
+// Slot of an id of the part (claimed for it when it has none yet).  CLAIM: the id leaves the stream.
+template <bool CLAIM>
 __device__ __forceinline__ int slot_of(const Table& t, int id, int low) {
   const uint32_t key = (uint32_t)id + 1u;
   uint32_t s = __umulhi((uint32_t)id * 2654435761u, (uint32_t)t.slots);  // multiplicative hashing
   for (;;) {
     const uint32_t k = atomicCAS(&t.key[s], 0u, key);
-    if (k == 0u) {  // this thread's: the id leaves the stream
-      const int p = id - low;
-      const uint32_t bit = 1u << (p & 31);
-      if (atomicAnd(&t.free[p >> 5], ~bit) & bit) atomicOr(&t.word[s], 0x80000000u);
+    if (k == 0u) {
+      if (CLAIM) {
+        const int p = id - low;
+        const uint32_t bit = 1u << (p & 31);
+        if (atomicAnd(&t.free[p >> 5], ~bit) & bit) atomicOr(&t.word[s], 0x80000000u);
+      }
       return (int)s;
     }
     if (k == key) return (int)s;
@@ -156,42 +159,39 @@ __device__ __forceinline__ int slot_of(const Table& t, int id, int low) {
   }
 }
 
-// The thread's share of a list, kListIds loads at a time, the first of them issued by begin().
+// The share of thread `tid` of kThreads in a list, kListIds loads at a time, the first of them issued by begin().
 struct List {
   const int32_t* list;
-  int length;
-  int32_t first[kListIds];
+  int length, tid;
+  int32_t ids[kListIds];
 
-  __device__ __forceinline__ void load(int i0, int32_t (&ids)[kListIds]) const {
+  __device__ __forceinline__ void load(int i0) {
 #pragma unroll
     for (int k = 0; k < kListIds; k++)
       if (i0 + k * kThreads < length) ids[k] = __ldg(list + i0 + k * kThreads);
   }
-  __device__ __forceinline__ void begin(const int32_t* l, int n) {
+  __device__ __forceinline__ void begin(const int32_t* l, int n, int thread) {
     list = l;
     length = n;
-    load(threadIdx.x, first);
+    tid = thread;
+    load(tid);
   }
   // Calls f(id, position).
   template <class F>
   __device__ __forceinline__ void each(F f) {
-    for (int i0 = threadIdx.x; i0 < length; i0 += kListIds * kThreads) {
-      if (i0 != (int)threadIdx.x) load(i0, first);
+    for (int i0 = tid; i0 < length; i0 += kListIds * kThreads) {
+      if (i0 != tid) load(i0);
 #pragma unroll
       for (int k = 0; k < kListIds; k++)
-        if (i0 + k * kThreads < length) f(first[k], i0 + k * kThreads);
+        if (i0 + k * kThreads < length) f(ids[k], i0 + k * kThreads);
     }
   }
 };
 
-// Builds the table and the bits of ids [low, low + len) of a row (low may be below 0 by less than a unit).  Ends
-// with a barrier; gives the lowest id the thread found allowed, 0xffffffff for none.
-__device__ __forceinline__ uint32_t build_table(const RowRules& r, const Table& t, int vocab, int low, int len) {
-  const int tid = threadIdx.x, from = max(low, 0), to = min(vocab - low, len) + low;  // the part's ids
+// The bits of ids [low, low + len) of a row (low may be below 0 by less than a unit): allowed by the mask.  Gives the
+// lowest id the thread found allowed, 0xffffffff for none.
+__device__ __forceinline__ uint32_t allowed_bits(const RowRules& r, const Table& t, int vocab, int low, int len, int tid) {
   uint32_t lowest = 0xffffffffu;
-  List history, biases;  // on their way beside the mask
-  history.begin(r.history, r.length);
-  biases.begin(r.bias_ids, r.biases);
   const int words = (vocab + 31) >> 5;
 #pragma unroll 4
   for (int w = tid; w < len / 32; w += kThreads) {
@@ -210,31 +210,36 @@ __device__ __forceinline__ uint32_t build_table(const RowRules& r, const Table& 
     t.free[w] = bits;
     if (bits) lowest = min(lowest, (uint32_t)(first + __ffs(bits) - 1));
   }
-  const bool listed = r.length > 0 || r.biases > 0;
-  if (listed)  // key, word and, where there are biases, bias lie behind one another
-    for (int s = tid * 4; s < t.slots * (t.bias ? 3 : 2); s += kThreads * 4)
-      *reinterpret_cast<uint4*>(t.key + s) = make_uint4(0, 0, 0, 0);
-  __syncthreads();
-  if (!listed) return lowest;
+  return lowest;
+}
+
+__device__ __forceinline__ void clear_table(const Table& t, int tid) {
+  // key, word and, where there are biases, bias lie behind one another
+  for (int s = tid * 4; s < t.slots * (t.bias ? 3 : 2); s += kThreads * 4)
+    *reinterpret_cast<uint4*>(t.key + s) = make_uint4(0, 0, 0, 0);
+}
+
+// The lists' ids among [low, low + len) into a cleared table (CLAIM: behind the part's bits).
+template <bool CLAIM>
+__device__ __forceinline__ void fill_table(const RowRules& r, const Table& t, int vocab, int low, int len, List& history,
+                                           List& biases) {
+  const int from = max(low, 0), to = min(vocab - low, len) + low;
   history.each([&](int id, int i) {
     if (id < from || id >= to) return;
-    const int s = slot_of(t, id, low);
+    const int s = slot_of<CLAIM>(t, id, low);
     if (i >= r.prompt) atomicAdd(&t.word[s], 2u);
     else atomicOr(&t.word[s], 1u);
   });
   biases.each([&](int id, int i) {
-    if (id >= from && id < to) atomicMax(&t.bias[slot_of(t, id, low)], (uint32_t)i + 1u);
+    if (id >= from && id < to) atomicMax(&t.bias[slot_of<CLAIM>(t, id, low)], (uint32_t)i + 1u);
   });
-  __syncthreads();
-  return lowest;
 }
 
-// Calls f(slot, id, raw logit, ruled logit) for the thread's share of the part's allowed ids with a rule.  Four
-// gathers at a time are in flight.  Keys of ids that are not allowed go.
-template <class T, class F>
-__device__ __forceinline__ void for_ruled(const RowRules& r, const Table& t, const T* row, F f) {
-  if (r.length == 0 && r.biases == 0) return;
-  for (int s0 = threadIdx.x; s0 < t.slots; s0 += 4 * kThreads) {
+// Calls f(slot, id, raw logit, ruled logit) for the share of thread `tid` of kThreads in the table's ids (CLAIM: those
+// allowed).  Four gathers at a time are in flight.
+template <bool CLAIM, class T, class F>
+__device__ __forceinline__ void for_ruled(const RowRules& r, const Table& t, const T* row, int tid, F f) {
+  for (int s0 = tid; s0 < t.slots; s0 += 4 * kThreads) {
     uint32_t key[4], word[4];
     float raw[4];
 #pragma unroll
@@ -242,10 +247,7 @@ __device__ __forceinline__ void for_ruled(const RowRules& r, const Table& t, con
       const int s = s0 + k * kThreads;
       key[k] = s < t.slots ? t.key[s] : 0;
       word[k] = key[k] ? t.word[s] : 0;
-      if (key[k] && !(word[k] & 0x80000000u)) {
-        t.key[s] = 0;
-        key[k] = 0;
-      }
+      if (CLAIM && !(word[k] & 0x80000000u)) key[k] = 0;
       raw[k] = key[k] ? to_f32(row[key[k] - 1u]) : 0.0f;
     }
 #pragma unroll
@@ -268,12 +270,15 @@ __device__ __forceinline__ void for_ruled(const RowRules& r, const Table& t, con
   }
 }
 
+// A barrier of kThreads threads, all stream or all list warps.
+__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(kThreads) : "memory"); }
+
 // The table lies behind the warps' rings.
 template <class T>
 __device__ __forceinline__ Table table_in(unsigned char* smem, const needle_logits_rules& a, const LogitsPlan& plan) {
   Table t;
   t.slots = plan.slots;
-  t.key = reinterpret_cast<uint32_t*>(smem + kWarps * kStages * kSliceBytes);
+  t.key = reinterpret_cast<uint32_t*>(smem + kRingBytes);
   t.word = t.key + plan.slots;
   t.bias = a.bias_ids ? t.word + plan.slots : nullptr;
   t.free = t.key + plan.slots * (a.bias_ids ? 3 : 2);
@@ -281,7 +286,7 @@ __device__ __forceinline__ Table table_in(unsigned char* smem, const needle_logi
 }
 
 // The steps a CTA streams: the rows blockIdx.y, + gridDim.y, ..., of each the parts blockIdx.x, + gridDim.x, ...
-template <class T>
+template <class T, int UNITS>
 struct Steps {
   const T* in;   // the row
   int64_t row;
@@ -303,7 +308,7 @@ struct Steps {
     }
   }
   __device__ __forceinline__ void next(const needle_logits_rules& a, const LogitsPlan& plan) {
-    at += step_ids(sizeof(T));
+    at += step_ids(sizeof(T), UNITS);
     if (at < end) return;
     part += gridDim.x;
     begin_part(a, plan);
@@ -314,12 +319,13 @@ struct Steps {
 };
 
 // A warp's stream: its slice of every step, kStages of them in shared memory or on their way.
-template <class T>
+template <class T, int UNITS>
 struct Stream {
-  static constexpr int VEC = 16 / sizeof(T), N = kUnits, kSlice = 32 * VEC * N;  // ids of a 16-byte unit, units of a lane, ids of a step
+  static constexpr int VEC = 16 / sizeof(T), N = UNITS, kSlice = 32 * VEC * N;  // ids of a 16-byte unit, units of a lane, ids of a step
+  static constexpr int kStages = 8 / UNITS;  // steps of the ring
   T* ring;
   uint64_t* bars;  // kStages of them
-  Steps<T> steps;  // what is copied next
+  Steps<T, UNITS> steps;  // what is copied next
   int stage;       // of the next step to be read
   uint32_t parity;
   bool ok;
@@ -406,17 +412,23 @@ struct Stream {
   }
 };
 
+// Four warps stream; where there are lists, four more build the part's table and rule its ids meanwhile: the stream
+// writes the ids that the mask allows as they are, ruled or not, so it waits for no list, and the ruled logits are
+// written behind it.  (out may be logits: an allowed logit that is gathered is the same before and after it was
+// written.)  512 x 50001 bf16 with lists: 32 us (3.2 TB/s of logits in and out), 41.7 us with four warps that do one
+// after the other.  Steps of two units a thread: 64 registers hold them, with four units 39.5 us, with one 38.9 us.
 template <class T>
-__global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_rules(const __grid_constant__ needle_logits_rules a,
-                                                            const LogitsPlan plan, T* out, int64_t out_stride,
-                                                            uint32_t* wait_words) {
-  using S = Stream<T>;
+__global__ void __launch_bounds__(2 * kThreads, kRulesResident) k_logits_rules(const __grid_constant__ needle_logits_rules a,
+                                                                               const LogitsPlan plan, T* out,
+                                                                               int64_t out_stride, uint32_t* wait_words) {
+  using S = Stream<T, kRulesUnits>;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[kWarps * kStages];
+  __shared__ __align__(8) uint64_t bars[kWarps * S::kStages];
   const Table t = table_in<T>(smem, a, plan);
-  const int tid = threadIdx.x, lane = tid & 31, slice = (tid >> 5) * S::kSlice;
+  const bool lists = threadIdx.x >= kThreads;  // a list warp
+  const int tid = threadIdx.x & (kThreads - 1), lane = tid & 31, slice = (tid >> 5) * S::kSlice;
   S stream;
-  stream.begin(a, plan, smem, bars);
+  if (!lists) stream.begin(a, plan, smem, bars);
   for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
     T* to = out + row * out_stride;
@@ -428,41 +440,53 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_rules(
     for (int part = blockIdx.x; part < plan.parts; part += gridDim.x) {
       const int low = part * plan.part - off, end = min(low + plan.part, a.vocab);
       if (low >= a.vocab) break;
-      build_table(r, t, a.vocab, low, plan.part);
-      // ruled logits are taken before the stream writes (out may be the logits) and written behind it
-      for_ruled(r, t, in, [&](int s, int, float, float x) { t.word[s] = __float_as_uint(x); });
-      if (listed) __syncthreads();
-      for (int at = low; at < end; at += step_ids(sizeof(T))) {
-        Vec<T, S::VEC> x[S::N];
-        stream.read(in, at, a.vocab, x);
-        stream.advance(a, plan);
-        const int e0 = at + slice + lane * S::VEC;
-        const bool whole = same && at + slice >= 0 && at + slice <= a.vocab - S::kSlice;
+      if (lists) {
+        if (listed) {
+          List history, biases;
+          history.begin(r.history, r.length, tid);
+          biases.begin(r.bias_ids, r.biases, tid);
+          clear_table(t, tid);
+          group_sync(1);
+          fill_table<false>(r, t, a.vocab, low, plan.part, history, biases);
+          group_sync(1);
+          for_ruled<false>(r, t, in, tid, [&](int s, int, float, float x) { t.word[s] = __float_as_uint(x); });
+        }
+      } else {
+        allowed_bits(r, t, a.vocab, low, plan.part, tid);
+        group_sync(2);
+        for (int at = low; at < end; at += step_ids(sizeof(T), kRulesUnits)) {
+          Vec<T, S::VEC> x[S::N];
+          stream.read(in, at, a.vocab, x);
+          stream.advance(a, plan);
+          const int e0 = at + slice + lane * S::VEC;
+          const bool whole = same && at + slice >= 0 && at + slice <= a.vocab - S::kSlice;
 #pragma unroll
-        for (int u = 0; u < S::N; u++) {
-          const int e = e0 + u * 32 * S::VEC, p = e - low;
-          const uint32_t free = t.free[p >> 5] >> (p & 31);
-          keep_free(x[u], free);
-          if (whole || (same && e >= 0 && e <= a.vocab - S::VEC)) {
-            *reinterpret_cast<Vec<T, S::VEC>*>(to + e) = x[u];
-          } else {
+          for (int u = 0; u < S::N; u++) {
+            const int e = e0 + u * 32 * S::VEC, p = e - low;
+            const uint32_t free = t.free[p >> 5] >> (p & 31);
+            keep_free(x[u], free);
+            if (whole || (same && e >= 0 && e <= a.vocab - S::VEC)) {
+              *reinterpret_cast<Vec<T, S::VEC>*>(to + e) = x[u];
+            } else {
 #pragma unroll
-            for (int i = 0; i < S::VEC; i++)
-              if (e + i >= 0 && e + i < a.vocab) to[e + i] = x[u].v[i];
+              for (int i = 0; i < S::VEC; i++)
+                if (e + i >= 0 && e + i < a.vocab) to[e + i] = x[u].v[i];
+            }
           }
         }
       }
       __syncthreads();
       if (listed) {
-        for (int s = tid; s < t.slots; s += kThreads) {
+        for (int s = threadIdx.x; s < t.slots; s += 2 * kThreads) {
           const uint32_t key = t.key[s];
-          if (key) to[key - 1u] = from_f32<T>(__uint_as_float(t.word[s]));
+          const int id = (int)(key - 1u), p = id - low;
+          if (key && (t.free[p >> 5] >> (p & 31) & 1u)) to[id] = from_f32<T>(__uint_as_float(t.word[s]));
         }
         __syncthreads();
       }
     }
   }
-  stream.finish(wait_words);
+  if (!lists) stream.finish(wait_words);
 }
 
 // One cluster per row (and the rows gridDim.y on); its CTAs take the row's parts in turn.
@@ -470,13 +494,13 @@ template <class T>
 __global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_select(const __grid_constant__ needle_logits_rules a,
                                                              const LogitsPlan plan, int32_t* __restrict__ ids,
                                                              float* __restrict__ log_probabilities, uint32_t* wait_words) {
-  using S = Stream<T>;
+  using S = Stream<T, kSelectUnits>;
   struct Best {  // of a warp, of a CTA
     float top, sum, raw;
     uint32_t key, id, lowest;
   };
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ __align__(8) uint64_t bars[kWarps * kStages];
+  __shared__ __align__(8) uint64_t bars[kWarps * S::kStages];
   __shared__ Best of_warp[kWarps], of_cta;
   const Table t = table_in<T>(smem, a, plan);
   cg::cluster_group cluster = cg::this_cluster();
@@ -504,6 +528,7 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_select
     const T* in = static_cast<const T*>(a.logits) + row * a.logits_stride;
     const int off = row_offset(in);
     const RowRules r = row_rules(a, row);
+    const bool listed = r.length > 0 || r.biases > 0;
     // the warp's best of the stream; the thread's best of the ids with a rule and its raw logit; the thread's
     // largest raw logit and sum of exponentials
     float best = -INFINITY, ruled_best = -INFINITY, raw = 0.0f, top = -INFINITY, sum = 0.0f;
@@ -513,8 +538,19 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_select
       const int low = part * plan.part - off, end = min(low + plan.part, a.vocab);
       if (low >= a.vocab) break;
       if (part != (int)blockIdx.x) __syncthreads();  // the table of the part before has been read
-      lowest = min(lowest, build_table(r, t, a.vocab, low, plan.part));
-      for (int at = low; at < end; at += step_ids(sizeof(T))) {
+      {
+        List history, biases;  // on their way beside the mask
+        history.begin(r.history, r.length, tid);
+        biases.begin(r.bias_ids, r.biases, tid);
+        lowest = min(lowest, allowed_bits(r, t, a.vocab, low, plan.part, tid));
+        if (listed) clear_table(t, tid);
+        __syncthreads();
+        if (listed) {
+          fill_table<true>(r, t, a.vocab, low, plan.part, history, biases);
+          __syncthreads();
+        }
+      }
+      for (int at = low; at < end; at += step_ids(sizeof(T), kSelectUnits)) {
         float x[S::N][S::VEC];
         {
           Vec<T, S::VEC> v[S::N];
@@ -582,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_select
           }
         }
       }
-      for_ruled(r, t, in, [&](int, int id_of, float l, float v) {
+      if (listed) for_ruled<true>(r, t, in, tid, [&](int, int id_of, float l, float v) {
         const uint32_t i = (uint32_t)id_of;
         if (v > ruled_best || (v == ruled_best && i < ruled_id && v > -INFINITY)) {
           ruled_best = v;
@@ -628,28 +664,28 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_select
 }
 
 size_t smem_bytes(const needle_logits_rules& a, const LogitsPlan& p) {
-  return size_t(kWarps * kStages * kSliceBytes) + size_t(p.slots) * (a.bias_ids ? 12 : 8) + size_t(p.part) / 8;
+  return size_t(kRingBytes) + size_t(p.slots) * (a.bias_ids ? 12 : 8) + size_t(p.part) / 8;
 }
 
 // CTAs that the GPU holds at once: by shared memory, and by registers.
-int64_t resident_ctas(const needle_logits_rules& a, size_t smem) {
-  return 148 * std::max<int64_t>(1, std::min<int64_t>(resident(type_bytes(a.type)), int64_t(226 * 1024 / (smem + 1536))));
+int64_t resident_ctas(int by_registers, size_t smem) {
+  return 148 * std::max<int64_t>(1, std::min<int64_t>(by_registers, int64_t(226 * 1024 / (smem + 1536))));
 }
 
 // Rows a CTA (or cluster) of `parts` CTAs takes side by side with the others: as few turns as the GPU can hold,
 // all of them full.
-unsigned rows_at_once(const needle_logits_rules& a, size_t smem, int parts) {
-  const int64_t fit = std::max<int64_t>(1, resident_ctas(a, smem) / parts), turns = (a.rows + fit - 1) / fit;
+unsigned rows_at_once(const needle_logits_rules& a, int by_registers, size_t smem, int parts) {
+  const int64_t fit = std::max<int64_t>(1, resident_ctas(by_registers, smem) / parts), turns = (a.rows + fit - 1) / fit;
   return unsigned((a.rows + turns - 1) / turns);
 }
 
-LogitsPlan plan_for(const needle_logits_rules& a, int most_parts) {
+LogitsPlan plan_for(const needle_logits_rules& a, int units, int most_parts) {
   LogitsPlan p{};
   const int64_t element = int64_t(type_bytes(a.type));
   const bool lined_up = aligned_to(a.logits, 16) && (a.rows == 1 || a.logits_stride * element % 16 == 0);
   const int64_t ids = int64_t(a.vocab) + (lined_up ? 0 : 16 / element - 1);  // with those before a row's first unit
   const int64_t entries = (a.history ? a.history_stride : 0) + (a.bias_ids ? a.bias_stride : 0);
-  const int64_t step = step_ids(size_t(element)), steps = (ids + step - 1) / step;
+  const int64_t step = step_ids(size_t(element), units), steps = (ids + step - 1) / step;
   // parts: as many as keep the GPU busy, each rescanning the lists; small enough for their bits and, with long
   // lists, for a table that has room for every id of the part
   const int64_t most = (entries > kMostEntries ? kMostEntries : kPartIds) / step;
@@ -697,7 +733,7 @@ int check_rules_buffers(const needle_logits_rules* a, Buffers outputs, int* devi
 
 // Always the same limit, so that calls at the same time cannot lower each other's: rings, a table of kMostEntries
 // with their biases, and a bit an id of the largest part.
-constexpr size_t kMostSmem = kWarps * kStages * kSliceBytes + (kMostEntries * 2 + 36) * 12 + kPartIds / 8;
+constexpr size_t kMostSmem = kRingBytes + (kMostEntries * 2 + 36) * 12 + kPartIds / 8;
 template <class K>
 cudaError_t set_smem(K kernel) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kMostSmem));
@@ -719,13 +755,14 @@ extern "C" int needle_cuda_logits_rules_dev(const needle_logits_rules* a, void* 
     int device = 0;
     if (int rc = check_rules_buffers(a, {{out, "out", type_bytes(a->type)}}, &device, "logits_rules")) return rc;
     if (check_wait_status(device) != NEEDLE_OK) return int(NEEDLE_BACKEND_UNAVAILABLE);
-    const LogitsPlan plan = plan_for(*a, 1 << 30);
+    const LogitsPlan plan = plan_for(*a, kRulesUnits, 1 << 30);
     const size_t smem = smem_bytes(*a, plan);
     const cudaError_t e = with_type(a->type, [&](auto zero) {
       using T = decltype(zero);
       const cudaError_t err = set_smem(k_logits_rules<T>);
       if (err != cudaSuccess) return err;
-      k_logits_rules<T><<<dim3(plan.parts, rows_at_once(*a, smem, plan.parts)), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
+      const dim3 grid(plan.parts, rows_at_once(*a, kRulesResident, smem, plan.parts));
+      k_logits_rules<T><<<grid, plan.slots > 0 ? 2 * kThreads : kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
           *a, plan, static_cast<T*>(out), out_stride, wait_status_words(device));
       return cudaGetLastError();
     });
@@ -744,7 +781,7 @@ extern "C" int needle_cuda_logits_select_dev(const needle_logits_rules* a, int32
     if (int rc = check_rules_buffers(a, {{ids, "ids", 4}, {log_probabilities, "log_probabilities", 4}}, &device, "logits_select"))
       return rc;
     if (check_wait_status(device) != NEEDLE_OK) return int(NEEDLE_BACKEND_UNAVAILABLE);
-    const LogitsPlan plan = plan_for(*a, 8);  // a row's CTAs are one cluster
+    const LogitsPlan plan = plan_for(*a, kSelectUnits, 8);  // a row's CTAs are one cluster
     const size_t smem = smem_bytes(*a, plan);
     const cudaError_t e = with_type(a->type, [&](auto zero) {
       using T = decltype(zero);
@@ -757,7 +794,7 @@ extern "C" int needle_cuda_logits_select_dev(const needle_logits_rules* a, int32
       attribute.val.clusterDim.y = 1;
       attribute.val.clusterDim.z = 1;
       cudaLaunchConfig_t config{};
-      config.gridDim = dim3(cluster, rows_at_once(*a, smem, cluster));
+      config.gridDim = dim3(cluster, rows_at_once(*a, resident(sizeof(T)), smem, cluster));
       config.blockDim = dim3(kThreads);
       config.dynamicSmemBytes = smem;
       config.stream = static_cast<cudaStream_t>(stream);
