@@ -7,21 +7,24 @@
 //   x = x + bias;  ids the mask leaves out: x = -inf       (every step rounded to binary32)
 //   id = argmax x, the lowest on ties;  log p = l[id] - max l - log sum exp(l - max l)
 //
-// A row is read once.  What the rules touch is sparse, so the stream over a row knows only one bit an id:
-// "free", allowed by the mask and without a rule.  The ids with a rule (history, biases) go into a hash table in
-// shared memory, which counts them and keeps their last bias; its entries are ruled one by one from a second,
-// gathered read of their logits.  CTAs of four warps take parts of rows (at most kPartIds ids; several CTAs or
-// one a row as the batch needs), one after another, and build the table for each.  Every warp streams its slice of
-// a part through a ring of its own in shared memory, filled by bulk copies that run on over the ends of parts
-// and rows: the copies never pause, and no barrier is needed for them.
+// A row is read once.  What the rules touch is sparse, so the stream over a row knows only one bit an id (allowed by
+// the mask; in selection, without a rule too).  The ids with a rule (history, biases) go into a hash table in shared
+// memory, which counts them and keeps their last bias; its entries are ruled one by one from a second, gathered read
+// of their logits.  CTAs take parts of rows (at most kPartIds ids; several CTAs or one a row as the batch needs), one
+// after another, and build the table for each.  Each of the four warps that stream has its slice of a part come through
+// a ring of its own in shared memory, filled by bulk copies that run on over the ends of parts and rows: the copies
+// never pause, and no barrier is needed for them.
 //
 // Bytes bound the stream, the lists' chains of dependent accesses the rest.  512 rows of 50001 bf16 ids (102 MB) with
-// histories of up to 1000 ids, 50 biases and masks take 32 us, 23 us without rules.  Select: 4096 rows of 8192 binary32 ids with histories of 256: 61 us (2.2 TB/s), 37 us without rules;
-// 200 rows of 128000 fp16 ids with histories of 2000: 46 us (1.1 TB/s; each of a row's two CTAs builds a table).
-// Measured beside it (the three sizes, before the rules had list warps: 42, 61, 46 us): chunks of a row in registers, direct tables of counts instead of the hash, one CTA a chunk:
-// 47, 72, 63 us; the hash twice as large as its list (5/4: 50, 66, 55 us, probes; 4 times: 71, 66, 129 us, fewer
-// CTAs resident); one warp a row: 110 us for the 4096 rows (too few warps hide the lists' latency); parts of 32 KB
-// in shared memory with the lists ruled there, 8 warps: 51, 81, 85 us (every warp repeats a part's fixed work).
+// histories of up to 1000 ids, 50 biases and masks take 32 us, 23 us without rules.  Select: 4096 rows of 8192
+// binary32 ids with histories of 256: 60 us (2.2 TB/s), 41 us without rules; 200 rows of 128000 fp16 ids with
+// histories of 2000: 46 us (1.1 TB/s; each of a row's two CTAs builds a table), 25 us without.
+// Measured beside it (the three sizes; 42, 61, 46 us then, before the rules had list warps): chunks of a row in
+// registers, direct tables of counts instead of the hash, one CTA a chunk: 47, 72, 63 us; the hash 5/4 of its lists
+// instead of twice: 50, 66, 55 us (probes), four times: 71, 66, 129 us (fewer CTAs resident); one warp a row: 110 us
+// for the 4096 rows (too few warps hide the lists' latency); parts of 32 KB in shared memory with the lists ruled
+// there, 8 warps: 51, 81, 85 us (every warp repeats a part's fixed work); twice the parts: 48, 66, 87 us (each
+// rescans the lists).
 #include <cooperative_groups.h>
 
 #include <algorithm>
