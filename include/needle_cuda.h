@@ -447,6 +447,7 @@ typedef struct needle_logits_rules {
   const uint32_t* masks;          /* [mask_count][ceil(vocab / 32)] */
   const int32_t* mask_slots;      /* [rows] */
   int32_t mask_count, type, rows /* at most 65535 */, vocab /* at most 2^30 */;
+  /* history_stride and bias_stride: below 2^30 */
 } needle_logits_rules;
 
 /* The ruled logits, rounded to `type`, rows out_stride elements apart; out may be logits (same stride). */

@@ -166,6 +166,14 @@ def test_logits_operators_refuse_misaligned_lists(name):
     refused(native.lib().needle_cuda_logits_select_dev(C.byref(a), P, P, None), name + " is not aligned")
 
 
+def test_logits_operators_refuse_lists_whose_counts_would_not_fit():
+    for change in (dict(history=P, history_lengths=P, history_stride=1 << 30),
+                   dict(bias_ids=P, bias_values=P, bias_counts=P, bias_stride=1 << 30), dict(vocab=(1 << 30) + 1, logits_stride=1 << 31)):
+        a = logits_args(**change)
+        refused(native.lib().needle_cuda_logits_rules_dev(C.byref(a), P, 1 << 31, None), "2^30")
+        refused(native.lib().needle_cuda_logits_select_dev(C.byref(a), P, P, None), "2^30")
+
+
 def test_logits_outputs_are_refused():
     a = logits_args(logits=P, logits_stride=120)
     refused(native.lib().needle_cuda_logits_rules_dev(C.byref(a), P, 100, None), "same row stride")
