@@ -914,3 +914,51 @@ def test_calls_from_two_threads_at_once(torch):
     assert not failures
     for s, w in zip([s for mine in states for s in mine], wanted):
         assert all(torch.equal(a, s[k]) for a, k in zip(w, OUTPUTS))
+
+
+def test_offsets_past_32_bits(torch):
+    """Caches and rows of logits whose elements lie more than 2^32 from the first: what a small copy of the same
+    gives.  (Only what is read is written first.)"""
+    from needle_b200 import native
+    g = torch.Generator().manual_seed(8)
+    heads, kv, dim, cap, n = 16, 8, 128, 1 << 21, 40
+    small = [t.cuda() for t in (*random_cache(torch, g, 1, kv, n, dim), *random_cache(torch, g, 1, kv, n, dim))]
+    large = [torch.empty(3, kv, cap, dim, dtype=torch.int8, device="cuda") if t.dim() == 4 else
+             torch.empty(3, kv, cap, device="cuda") for t in small]
+    assert large[0][2].data_ptr() - large[0].data_ptr() >= 1 << 32
+    for a, b in zip(large, small):
+        a[2, :, :n] = b[0]
+    x = torch.randn(1, (heads + 2 * kv) * dim, generator=g).cuda()
+    q, k, v = x.split([heads * dim, kv * dim, kv * dim], 1)
+    inverse = [10000.0 ** (-2.0 * i / dim) for i in range(dim // 2)]
+    at = lambda i: torch.tensor([i], dtype=torch.int32).cuda()  # noqa: E731
+    results = []
+    for cache, slot in ((small, 0), (large, 2)):
+        q_out, out, lse = torch.zeros(1, heads * dim).cuda(), torch.zeros(1, heads * dim).cuda(), torch.zeros(1, heads).cuda()
+        rope_call(torch, "f32", q, k, v, q_out, None, None, None, None, at(n - 1), at(slot), at(n - 1), cache, heads, kv, dim,
+                  dim, False, inverse, 1.0)
+        attention_call(torch, "f32", q_out, out, lse, [None] * 4, cache, at(slot), at(n), heads, kv, dim, 0)
+        results.append((out, lse))
+    rope_call(torch, "f32", q, k, v, torch.zeros_like(q_out), None, None, None, None, at(n - 1), at(2), at(cap - 1), large, heads,
+              kv, dim, dim, False, inverse, 1.0)
+    torch.cuda.synchronize()
+    for a, b in zip(large, small):
+        assert torch.equal(a[2, :, :n], b[0]) and torch.equal(a[2, :, cap - 1], b[0, :, n - 1])
+    assert all(torch.allclose(a, b, rtol=0, atol=64 * U * float(a.abs().max())) for a, b in zip(*results))
+    del large
+    rows, vocab, stride = 3, 5000, (1 << 31) + 8
+    logits = torch.randn(rows, vocab, generator=g).half().cuda()
+    far = torch.empty(rows * stride, dtype=torch.float16, device="cuda").view(rows, stride)
+    far[:, :vocab] = logits
+    rules = make_rules(torch, rows, vocab, 4)
+    chosen, outs = [], []
+    for d in (logits, far[:, :vocab]):
+        a = rules_args(torch, "f16", d, rules)
+        ids, lps = torch.zeros(rows, dtype=torch.int32).cuda(), torch.zeros(rows).cuda()
+        native.check(native.lib().needle_cuda_logits_select_dev(C.byref(a), ids.data_ptr(), lps.data_ptr(), stream_of(torch)))
+        native.check(native.lib().needle_cuda_logits_rules_dev(C.byref(a), d.data_ptr(), d.stride(0), stream_of(torch)))
+        torch.cuda.synchronize()
+        chosen.append((ids, lps))
+        outs.append(d)
+    assert torch.equal(chosen[0][0], chosen[1][0]) and torch.equal(chosen[0][1], chosen[1][1])
+    assert torch.equal(*outs)
