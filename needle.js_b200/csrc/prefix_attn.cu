@@ -24,6 +24,9 @@
 // A unit (row, KV head, 8 heads, split of the positions) has a CTA of 2 to 8 warps, merged in shared memory, or,
 // where units are many, one warp, beside those of the row's other KV heads: caches of one age end together.
 // Splits and the prefix's parts are merged from the workspace.
+// Measured: 4096 rows x 4 KV heads of 64, 0..256 own positions (302 MB) beside a prefix of 160: 77 us, 70 us of them the
+// stream's: 4.3 TB/s, bound by its instructions (67% issued).  333 rows x 8 KV heads of 128, 0..500 (176 MB): 50 us,
+// 3.5 TB/s, bound by latency at the 13 warps whose rings an SM holds.  One row of 160 + 256: 4.2 us.
 #include <algorithm>
 #include <cmath>
 
