@@ -654,7 +654,7 @@ extern "C" int needle_cuda_prefix_attention_workspace(const needle_prefix_attent
   return entry([&] {
     if (int rc = check_attention(a)) return rc;
     if (!bytes) return refuse("null argument");
-    *bytes = workspace_bytes_for(*a, plan_for(*a));
+    *bytes = a->rows == 0 ? 0 : workspace_bytes_for(*a, plan_for(*a));  // (an empty batch has no plan)
     return int(NEEDLE_OK);
   });
 }
