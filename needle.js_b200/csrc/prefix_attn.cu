@@ -284,8 +284,8 @@ __device__ __forceinline__ void store_out(T* p, const float* x, bool vec) {
 // What becomes of N output dimensions of a head, from g * N on, held by lane g of its eight.
 template <int N>
 __device__ __forceinline__ void store_part(const Parts& parts, int64_t part, float m, float l, const float* o, int g) {
-  if (g == 0) parts.ml[part] = make_float2(m, l);
-  if (m == -INFINITY) return;  // an empty part: its values are never read
+  if (g == 0) parts.ml[part] = part_of(m, l);
+  if (l == 0.0f) return;  // an empty part: its values are never read
 #pragma unroll
   for (int i = 0; i < N; i += 4)
     *reinterpret_cast<float4*>(parts.o + part * (8 * N) + g * N + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);

@@ -14,12 +14,16 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kRaise = 7.0f;
 
 // Parts of the softmax: M and l of every (part, row, head), and the weighted values.  A part is 2^M times
-// its l and values; an empty one has M = -inf and its values are not read.
+// its l and values; an empty one has M = -inf and l = 0, and its values are not read (part_of).
 struct Parts {
   float2* ml;
   float* o;
   int64_t per_part;  // rows * heads
 };
+
+// A part's M and l as they are stored.  Maxima pass over NaN: a part whose scores are all NaN has M = -inf too, and its
+// l, which is NaN, says that it is not an empty one.
+__device__ __forceinline__ float2 part_of(float M, float l) { return make_float2(l == l ? M : 0.0f, l); }
 
 // The prefix on the tensor cores (prefix_attn_tc.cu): parts 0 .. parts - 1 of `out`, `part_len` positions each.
 // part_len is a multiple of prefix_tile().

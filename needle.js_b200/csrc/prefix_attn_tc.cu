@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const bool bad = !ok || !done || *(volatile int*)&failed != 0;
       if (bad && lane == 0) report_wait_timeout(wait_words, kWaitAttention);
       const int64_t part = blockIdx.z * parts.per_part + (int64_t)row * a.heads + head;
-      if (live) parts.ml[part] = bad ? make_float2(0.0f, NAN) : make_float2(M, l);
+      if (live) parts.ml[part] = part_of(M, bad ? NAN : l);
       // 32 columns at a time through shared memory (the operands are done with), so that rows are written
       // 128 bytes at once
       float* turn = reinterpret_cast<float*>(smem) + warp * 32 * kTurnRow;
