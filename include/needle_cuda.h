@@ -343,9 +343,13 @@ typedef enum needle_type { NEEDLE_TYPE_F32 = 0, NEEDLE_TYPE_F16 = 1, NEEDLE_TYPE
  * Per head: y = (1 + norm) x / sqrt(mean x^2 + 1e-6) where a norm is given; pairs (i, i + rotary_dim / 2),
  * or (2i, 2i + 1) when `interleaved`, of the first rotary_dim dimensions turn by position * inverse
  * frequency i and grow by `magnitude`; q_out gets the queries.  Keys and values are rounded to int8 with
- * scale max(1e-12, max |y|) / 127 and stored at (slot, entry) of
- *   codes [slot_count][kv_heads][capacity][head_dim], scales [slot_count][kv_heads][capacity];
- * a token whose slot or entry is out of range (-1: padding) is rotated but not stored.  Two tokens of one
+ * scale max(1e-12, max |y|) / 127 (binary64) and stored at (slot, entry) of
+ *   codes [slot_count][kv_heads][capacity][head_dim], scales [slot_count][kv_heads][capacity].
+ * Rows of NEEDLE_TYPE_F32 get the engine's codes and scales.  For rows of 16-bit types the codes come from the
+ * product max(1e-12, max |y|) * (1 / 127): a value exactly between two codes (half of the row's largest) may
+ * get the other of the two, scales are the same.  Where the engine's codes of such rows are wanted, widen them to
+ * binary32.
+ * A token whose slot or entry is out of range (-1: padding) is rotated but not stored.  Two tokens of one
  * call must not name the same (slot, entry).  k_out / v_out (optional) get the keys and values as the
  * cache holds them, code * scale: what an attention over the new tokens themselves has to read.  q_out may
  * be q, k_out k and v_out v. */

@@ -8,8 +8,12 @@
 //
 // Keys are computed in binary64 and rounded to binary32 exactly where the engine stores them, so the
 // codes are the engine's: a key one ulp off would round to the other code next to a border.  The scale is
-// the binary64 product with 1 / 127, at most one binary64 ulp from the quotient and several times cheaper;
-// only a value within 2^-52 of a border between codes could tell the two apart.
+// the binary64 product with 1 / 127, several times cheaper than the quotient; rounded to binary32, as it is
+// stored, it is the same for every binary32 maximum (all of them were compared).  The two differ by one
+// binary64 ulp in one row of ten, which only a value exactly on a border between codes can tell: half of a
+// row's largest value, in most rows.  There binary32 rows, the engine's type, are divided by the quotient and
+// get the engine's codes; 16-bit rows, where such values are common (one in 2.4% of bf16 rows of 128 normal
+// values gets another code), keep the product: 63 or 64 for 63.5 steps, equally near.
 // Queries in binary32 are computed the same way; 16-bit queries in binary32, whose error (2^-23) is far
 // below the rounding to 16 bits (2^-11, 2^-8).
 //
@@ -281,7 +285,8 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
     const double scale = fmax(1e-12, (double)top) * (1.0 / 127.0);
     const float scale32 = (float)scale, inverse = 1.0f / scale32;
     // The quotient in binary32 is within 2^-15 of the exact one; adding 1.5 * 2^23 rounds it to an integer,
-    // which the sum's lowest byte holds.  One that near a border between codes, or a NaN, is divided in binary64.
+    // which the sum's lowest byte holds.  One that near a border between codes, or a NaN, is divided in binary64
+    // (by the quotient in binary32 rows, whose division only these few pay for).
     constexpr float kRound = 12582912.0f;
     uint32_t border = 0;
     float r[E];
@@ -297,7 +302,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeResident) k_rope_append(con
       float value = x[0];
 #pragma unroll
       for (int i = 1; i < E; i++) value = i == at ? x[i] : value;
-      float code = (float)rint((double)value / scale);
+      float code = (float)rint((double)value / (kNarrow ? scale : fmax(1e-12, (double)top) / 127.0));
       code = code != code ? 0.0f : fminf(fmaxf(code, -127.0f), 127.0f);
 #pragma unroll
       for (int i = 0; i < E; i++) r[i] = i == at ? code + kRound : r[i];

@@ -6,9 +6,10 @@ Tolerances.  u = 2^-24 (half a binary32 step), h = half a step of the element ty
 """
 import math
 
+import numpy as np
 import pytest
 
-from test_gpu_serving_ops import TYPES, attention_call, dtype_of, random_cache
+from test_gpu_serving_ops import TYPES, attention_call, dtype_of, random_cache, rope_call, to_numpy
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +72,78 @@ def test_queries_that_are_not_finite_give_nan(torch, name, rows, heads, kv_heads
         want[r, h], want_lse[r, h] = 0.0, 0.0
         got[r, h], lse[r, h] = 0.0, 0.0
     assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
+# ------------------------------------------------------------------ rope_append
+
+def quotients(x):
+    """Codes and scales by division, as the engine's append computes them (numpy, binary64)."""
+    x = x.astype(np.float64)
+    scale = np.maximum(np.abs(x).max(-1), 1e-12) / 127.0
+    return np.rint(x / scale[..., None]).astype(np.int8), scale.astype(np.float32)
+
+
+def products(x):
+    x = x.astype(np.float64)
+    scale = np.maximum(np.abs(x).max(-1), 1e-12) * (1.0 / 127.0)
+    return np.rint(x / scale[..., None]).astype(np.int8), scale.astype(np.float32)
+
+
+def append(torch, name, rows, dim):
+    """Codes and scales of `rows` [tokens, dim] appended as keys and as values, without norm and rotation."""
+    t = rows.shape[0]
+    d = rows.cuda()
+    cache = [torch.zeros(1, 1, t, dim, dtype=torch.int8).cuda(), torch.zeros(1, 1, t).cuda(),
+             torch.zeros(1, 1, t, dim, dtype=torch.int8).cuda(), torch.zeros(1, 1, t).cuda()]
+    at = torch.arange(t, dtype=torch.int32).cuda()
+    rope_call(torch, name, d, d, d, torch.zeros_like(d), None, None, None, None, at, at * 0, at, cache, 1, 1, dim, 0, False, [], 1.0)
+    torch.cuda.synchronize()
+    return [c[0, 0].cpu().numpy() for c in cache]
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_codes_of_half_the_largest_value(torch, name, dim):
+    """Half of a row's largest value is 63.5 steps.  Binary32 rows: the code is what dividing by (largest / 127) gives, as
+    in the engine.  16-bit rows: what dividing by (largest * (1 / 127)) gives, which on such a border alone is the other
+    neighbour of 63.5 in one row of ten."""
+    g = torch.Generator().manual_seed(dim)
+    x = torch.rand(4000, dim, generator=g) - 0.5
+    top = 0.5 + torch.rand(4000, generator=g)
+    x = x.to(dtype_of(torch, name))
+    x[:, 3] = top.to(x.dtype) * torch.where(torch.arange(4000) % 2 == 0, 1.0, -1.0).to(x.dtype)
+    x[:, 9], x[:, 20] = x[:, 3] / 2, -x[:, 3] / 2
+    rows = to_numpy(x)
+    exact, other = quotients(rows), products(rows)
+    assert (exact[0] != other[0]).any(1).mean() > 0.02  # the two definitions are told apart here
+    np.testing.assert_array_equal(exact[1], other[1])
+    want, scales = exact if name == "f32" else other
+    got = append(torch, name, x, dim)
+    for codes, stored in (got[:2], got[2:]):
+        np.testing.assert_array_equal(codes, want)
+        np.testing.assert_array_equal(stored, scales)
+
+
+def test_codes_and_scales_are_the_engine_s(torch):
+    """The keys and values that an engine with a float cache holds, appended by the operator, against an engine with an
+    int8 cache that read the same tokens (first layer: nothing before it depends on the cache)."""
+    from needle_b200 import synth
+    from needle_b200.backend import CudaEngine, StepRequest
+    archive = synth.build_archive(3, synth.small_geometry(layers=2, vocab=512), probe_heads=False)
+    tokens = np.random.default_rng(5).integers(0, 512, 48)
+    held = {}
+    for kind in ("float32", "int8"):
+        with CudaEngine(archive, device=0, max_seqs=1, max_len=64, max_sink=0, kv_cache=kind) as eng:
+            eng.reset(0, 64, 0)
+            for t in tokens:
+                eng.step([StepRequest(0, int(t), False)])
+            held[kind] = eng.read_kv_f32(0, 0) if kind == "float32" else eng.read_kv(0, 0)
+    n, dim = len(tokens), held["float32"][0].shape[-1]
+    kc, vc, ks, vs = held["int8"]
+    for floats, codes, scales in ((held["float32"][0], kc, ks), (held["float32"][1], vc, vs)):
+        rows = np.ascontiguousarray(floats[:, :n]).reshape(-1, dim)
+        assert np.abs(rows).max() > 0
+        got = append(torch, "f32", torch.from_numpy(rows), dim)
+        for k in (0, 2):
+            np.testing.assert_array_equal(got[k], codes[:, :n].reshape(-1, dim))
+            np.testing.assert_array_equal(got[k + 1], scales[:, :n].reshape(-1))
