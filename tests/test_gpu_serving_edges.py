@@ -4,12 +4,13 @@ definitions in binary64.
 
 Tolerances.  u = 2^-24 (half a binary32 step), h = half a step of the element type (2^-24, 2^-11, 2^-8).
 """
+import ctypes as C
 import math
 
 import numpy as np
 import pytest
 
-from test_gpu_serving_ops import TYPES, attention_call, dtype_of, random_cache, rope_call, to_numpy
+from test_gpu_serving_ops import TYPES, U, attention_call, dtype_of, random_cache, rope_call, rules_args, stream_of, to_numpy
 
 pytestmark = pytest.mark.gpu
 
@@ -72,6 +73,58 @@ def test_queries_that_are_not_finite_give_nan(torch, name, rows, heads, kv_heads
         want[r, h], want_lse[r, h] = 0.0, 0.0
         got[r, h], lse[r, h] = 0.0, 0.0
     assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
+# ------------------------------------------------------------------ logits_select
+
+@pytest.mark.parametrize("name,offset", [
+    ("f32", 0.0), ("f32", 1e3), ("f32", -1e3), ("f32", 1e4), ("f32", -65504.0), ("f32", 1e6), ("f32", 1e8), ("f32", -1e9),
+    ("f32", 3e10), ("f32", -1e30), ("f32", 1e38), ("f16", 1e3), ("f16", -2e4), ("f16", 6e4), ("bf16", 1e3), ("bf16", -1e9),
+    ("bf16", 1e30)])
+@pytest.mark.parametrize("rows,vocab", [(3, 8192), (2, 50001)])
+def test_log_probabilities_do_not_depend_on_an_offset(torch, name, offset, rows, vocab):
+    """l - max - log sum exp(l - max): an offset of all logits cancels in l - max.  Tolerance: that of logits around zero:
+    a thread adds at most ceil(vocab / 4096) * 16 terms, 30 merges follow, every term is off by 2 u relative to the
+    sum and its addition by as much; the logarithm makes that absolute; 4 u of the value itself."""
+    from needle_b200 import native
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(rows, vocab, generator=g)
+    # on the grid of the type at the offset: neighbouring values where it is coarse
+    x = (offset + (3.0 if abs(offset) < 1e7 else abs(offset) * 2.0 ** -24 * 3) * x).to(dtype_of(torch, name))
+    x[-1] = torch.where(torch.arange(vocab) % 3 == 0, x[-1], torch.full((), offset).to(x.dtype))
+    d = x.cuda()
+    a = rules_args(torch, name, d, {})
+    ids, lps = torch.zeros(rows, dtype=torch.int32).cuda(), torch.zeros(rows).cuda()
+    native.check(native.lib().needle_cuda_logits_select_dev(C.byref(a), ids.data_ptr(), lps.data_ptr(), stream_of(torch)))
+    torch.cuda.synchronize()
+    raw = x.double()
+    terms = -(-vocab // 4096) * 16 + 30
+    for r in range(rows):
+        best = int((raw[r] == raw[r].max()).nonzero()[0, 0])
+        want = float(torch.log_softmax(raw[r], 0)[best])
+        assert int(ids[r]) == best
+        assert abs(float(lps[r]) - want) <= (2 * terms + 4 * abs(want)) * U, (r, float(lps[r]), want)
+
+
+def test_log_probabilities_of_logits_that_climb(torch):
+    """Rows whose maximum rises all the way, and a row whose ids but a few are at -1e9 (masked by addition)."""
+    from needle_b200 import native
+    v = 20000
+    x = torch.stack((torch.linspace(-1e5, 1e5, v), torch.linspace(3e4, -3e4, v), torch.full((v,), -1e9)))
+    x[0, -40:] = 1e5
+    x[2, 777] = -1e9 + 64
+    x[2, 9000:9007] = -1e9 + 128
+    d = x.cuda()
+    a = rules_args(torch, "f32", d, {})
+    ids, lps = torch.zeros(3, dtype=torch.int32).cuda(), torch.zeros(3).cuda()
+    native.check(native.lib().needle_cuda_logits_select_dev(C.byref(a), ids.data_ptr(), lps.data_ptr(), stream_of(torch)))
+    torch.cuda.synchronize()
+    want = torch.log_softmax(x.double(), 1)
+    best = [v - 40, 0, 9000]
+    assert ids.tolist() == best
+    for r in range(3):
+        w = float(want[r, best[r]])
+        assert abs(float(lps[r]) - w) <= (2 * 110 + 4 * abs(w)) * U, (r, float(lps[r]), w)
 
 
 # ------------------------------------------------------------------ rope_append
