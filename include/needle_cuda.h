@@ -352,7 +352,7 @@ typedef enum needle_type { NEEDLE_TYPE_F32 = 0, NEEDLE_TYPE_F16 = 1, NEEDLE_TYPE
  * A token whose slot or entry is out of range (-1: padding) is rotated but not stored.  Two tokens of one
  * call must not name the same (slot, entry).  k_out / v_out (optional) get the keys and values as the
  * cache holds them, code * scale: what an attention over the new tokens themselves has to read.  q_out may
- * be q, k_out k and v_out v. */
+ * be q, k_out k and v_out v (same row stride); outputs overlap nothing else of the call. */
 typedef struct needle_rope_append {
   const void *q, *k, *v;        /* [tokens][heads | kv_heads | kv_heads][head_dim] of `type` */
   void *q_out, *k_out, *v_out;  /* k_out, v_out may be NULL */

@@ -400,6 +400,11 @@ extern "C" int needle_cuda_rope_append_dev(const needle_rope_append* a, const do
                           a->v_stride < a->kv_heads * d || (a->k_out && a->k_out_stride < a->kv_heads * d) ||
                           (a->v_out && a->v_out_stride < a->kv_heads * d)))
       return refuse("a row stride is shorter than its row");
+    // (with another stride a token's output would be another token's input)
+    if (a->tokens > 1 && ((a->q_out == a->q && a->q_out_stride != a->q_stride) ||
+                          (a->k_out == a->k && a->k_out_stride != a->k_stride) ||
+                          (a->v_out == a->v && a->v_out_stride != a->v_stride)))
+      return refuse("q_out may be q, k_out k and v_out v only with the same row stride");
     const size_t e = type_bytes(a->type);
     const Buffers buffers = {{a->q, "q", e}, {a->k, "k", e}, {a->v, "v", e}, {a->q_out, "q_out", e}, {a->k_out, "k_out", e},
                              {a->v_out, "v_out", e}, {a->q_norm, "q_norm", 4}, {a->k_norm, "k_norm", 4},

@@ -53,3 +53,26 @@ print("sized")
     done = subprocess.run([sys.executable, "-c", code, ROOT, os.path.dirname(os.path.abspath(__file__))],
                           capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "sized" in done.stdout, (done.returncode, done.stderr[-2000:])
+
+
+P = 1 << 20  # an aligned address that nothing reads
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+@pytest.mark.parametrize("more", [64, -64])
+def test_rope_append_in_place_needs_one_row_stride(name, more):
+    """A token's output over another token's input: refused, in the order of the tokens or against it."""
+    a = native.RopeAppend()
+    for n in ("positions", "slots", "entries", "key_codes", "key_scales", "value_codes", "value_scales"):
+        setattr(a, n, P)
+    for i, n in enumerate(("q", "k", "v")):  # views of one fused buffer, written in place
+        setattr(a, n, P + i * 2048)
+        setattr(a, n + "_out", P + i * 2048)
+        setattr(a, n + "_stride", 2048)
+        setattr(a, n + "_out_stride", 2048)
+    a.magnitude = 1.0
+    a.tokens, a.heads, a.kv_heads, a.head_dim, a.rotary_dim, a.slot_count, a.capacity = 2, 8, 4, 64, 64, 1, 4
+    setattr(a, name + "_out_stride", 2048 + more)
+    ones = (C.c_double * 32)(*[1.0] * 32)
+    with pytest.raises(native.NeedleError, match="same row stride"):
+        native.check(native.lib().needle_cuda_rope_append_dev(C.byref(a), ones, None))
