@@ -417,8 +417,8 @@ typedef struct needle_prefix_attention {
   int32_t type, rows, heads, kv_heads, head_dim /* 64 or 128 */, prefix_length, prefix_capacity, slot_count, capacity;
 } needle_prefix_attention;
 
-/* Bytes of workspace a call with these arguments needs.  Reads no device memory; depends only on the sizes
- * (type, rows, heads, prefix_length, capacity).  A smaller batch may need more, since it is split more: one
+/* Bytes of workspace a call with these arguments needs.  Reads no device memory; depends only on rows, heads,
+ * kv_heads, head_dim, prefix_length and capacity.  A smaller batch may need more, since it is split more: one
  * workspace for several sizes is the largest of theirs. */
 int needle_cuda_prefix_attention_workspace(const needle_prefix_attention* args, size_t* bytes);
 

@@ -55,6 +55,22 @@ print("sized")
     assert done.returncode == 0 and "sized" in done.stdout, (done.returncode, done.stderr[-2000:])
 
 
+def test_workspace_depends_on_what_the_header_names():
+    """Each of the six sizes alone changes the workspace; the element type, the slots and their order do not."""
+    for sizes in (dict(rows=256, prefix_length=700, capacity=24), dict(rows=2, capacity=20000),
+                  dict(rows=2, prefix_length=9000, capacity=500)):
+        n = workspace(**sizes)
+        assert n > 0
+        for other in (dict(type=native.TYPE_BF16), dict(type=native.TYPE_F16), dict(slot_count=77), dict(scale=0.5),
+                      dict(slots=P, counts=P, lse=P), dict(q_stride=4096, out_stride=512)):
+            assert workspace(**{**sizes, **other}) == n, other
+    base = dict(rows=256, prefix_length=700, capacity=24)
+    for other in (dict(rows=255), dict(heads=16), dict(head_dim=128), dict(prefix_length=8000)):
+        assert workspace(**{**base, **other}) != workspace(**base), other
+    assert len({workspace(rows=2, capacity=20000), workspace(rows=2, capacity=2000),
+                workspace(rows=2, capacity=20000, kv_heads=1)}) == 3
+
+
 P = 1 << 20  # an aligned address that nothing reads
 
 
