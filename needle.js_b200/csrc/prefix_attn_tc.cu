@@ -447,7 +447,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             }
           }
         }
-        const float2 inverse2 = make_float2(inverse, inverse), minus = make_float2(-M, -M);
+        const float base = M == -INFINITY ? 0.0f : M;  // (no score above -inf yet)
+        const float2 inverse2 = make_float2(inverse, inverse), minus = make_float2(-base, -base);
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int c = 0; c < kNT; c += 32) {

@@ -10,7 +10,8 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_serving_ops import TYPES, U, attention_call, dtype_of, random_cache, rope_call, rules_args, stream_of, to_numpy
+from test_gpu_serving_ops import (TYPES, U, attention_call, attention_reference, dtype_of, random_cache, rope_call,
+                                  rules_args, stream_of, to_numpy)
 
 pytestmark = pytest.mark.gpu
 
@@ -73,6 +74,32 @@ def test_queries_that_are_not_finite_give_nan(torch, name, rows, heads, kv_heads
         want[r, h], want_lse[r, h] = 0.0, 0.0
         got[r, h], lse[r, h] = 0.0, 0.0
     assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
+# One position with the whole weight and a score beyond 2^24: the reference maximum, a binary32 number of that size, has
+# steps of 2 and more and rounds the exponent of the value scales away that it should cover.  The weight is then not
+# some 2^6 but the value scale itself, and its fp16 tail ends at 2^-24: half of that for each of at most 127 steps.
+WHOLE_WEIGHT = 127 * 2.0 ** -25
+
+
+def test_scores_below_the_range_of_binary32_have_no_weight(torch):
+    """Prefix scores that overflow to -inf leave the row's own positions, in the dense product and in the stream.
+    Tolerance: WHOLE_WEIGHT."""
+    for rows in (3, 170):
+        g = torch.Generator().manual_seed(rows)
+        heads, kv_heads, dim, prefix_length, capacity = 8, 4, 64, 210, 16
+        prefix, own = caches(torch, g, rows, kv_heads, dim, prefix_length, capacity)
+        q = torch.zeros(rows, heads * dim)
+        q[:, ::dim] = 1e30
+        prefix[0][..., 0] = torch.randint(-127, -1, (kv_heads, prefix_length), generator=g).to(torch.int8)
+        prefix[1][:] = 1e10  # scores of -1e40
+        counts = [1 + (5 * r) % capacity for r in range(rows)]
+        out, lse = attend(torch, "f32", q, prefix, own, counts, heads, kv_heads, dim, prefix_length)
+        for r in range(rows):
+            want, want_lse, _, vmax = attention_reference(torch, q[r], prefix, own, r, counts[r], heads, kv_heads, dim, 0, 0.125)
+            # neighbouring scores are 1e26 apart and more: one position takes it all
+            assert bool((out[r].double() - want).abs().le(4 * U * vmax + WHOLE_WEIGHT).all()), r
+            assert bool((lse[r].double() - want_lse).abs().le(16 * U * want_lse.abs()).all()), r
 
 
 # ------------------------------------------------------------------ logits_select
