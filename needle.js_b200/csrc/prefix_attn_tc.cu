@@ -448,7 +448,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           }
         }
         const float base = M == -INFINITY ? 0.0f : M;  // (no score above -inf yet)
-        const float2 inverse2 = make_float2(inverse, inverse), minus = make_float2(-base, -base);
+        // A weight is 2^(x inverse - M) of an unrounded product.  Where steps of M reach 1/8, and may be far above 1,
+        // the product is rounded first, as M's was: else no position would meet M, whose weight has to be near 1.
+        float times = inverse;
+        const bool far = fabsf(base) > 1048576.0f;
+        if (__any_sync(0xffffffffu, far)) {
+          const float2 round = make_float2(far ? inverse : 1.0f, far ? inverse : 1.0f);
+#pragma unroll
+          for (int j = 0; j < kNT / 2; j++) x[j] = __fmul2_rn(x[j], round);
+          times = far ? 1.0f : inverse;
+        }
+        const float2 inverse2 = make_float2(times, times), minus = make_float2(-base, -base);
         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int c = 0; c < kNT; c += 32) {

@@ -102,6 +102,33 @@ def test_scores_below_the_range_of_binary32_have_no_weight(torch):
             assert bool((lse[r].double() - want_lse).abs().le(16 * U * want_lse.abs()).all()), r
 
 
+@pytest.mark.parametrize("size", [1e5, 1e7, 3e9, 1e12, 1e30])
+def test_scores_of_any_size_choose_their_largest(torch, size):
+    """Scores of one product each, five roundings off at most, the largest 5% above the next: it takes all the weight,
+    though neighbouring binary32 scores are far more than 1 apart.  In the dense product and in the stream; the largest
+    among the prefix, or of the row's own.  Tolerance: WHOLE_WEIGHT."""
+    for rows in (3, 170):
+        g = torch.Generator().manual_seed(rows)
+        heads, kv_heads, dim, prefix_length, capacity = 8, 4, 64, 210, 16
+        prefix, own = caches(torch, g, rows, kv_heads, dim, prefix_length, capacity)
+        q = torch.zeros(rows, heads * dim)
+        q[:, ::dim] = size
+        q[1::2] *= -1.0  # (codes are as negative as they are positive)
+        for codes, scales in (prefix[:2], own[:2]):
+            codes[..., 0] = codes[..., 0].clamp(-100, 100)
+            scales[:] = 0.011
+        for h in range(kv_heads):
+            prefix[0][h, 71 * h % prefix_length, 0], prefix[0][h, (71 * h + 100) % prefix_length, 0] = 110, -110
+        own[0][2::3, :, 5, 0], own[0][2::3, :, 4, 0] = 127, -127
+        counts = [(5 * r) % capacity for r in range(rows)]
+        out, lse = attend(torch, "f32", q, prefix, own, counts, heads, kv_heads, dim, prefix_length)
+        for r in range(rows):
+            want, want_lse, _, vmax = attention_reference(torch, q[r], prefix, own, r, counts[r], heads, kv_heads, dim, prefix_length,
+                                                          0.125)
+            assert bool((out[r].double() - want).abs().le(8 * U * vmax + WHOLE_WEIGHT).all()), (r, float((out[r].double() - want).abs().max()))
+            assert bool((lse[r].double() - want_lse).abs().le(16 * U * want_lse.abs()).all()), r
+
+
 # ------------------------------------------------------------------ logits_select
 
 @pytest.mark.parametrize("name,offset", [
