@@ -129,7 +129,7 @@ __device__ __forceinline__ void attend_block(Rows<D, NG>& r, const Stage<D>& b, 
       }
   }
   vtop = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(vtop)));
-  const float ev = (float)(min(max(exponent_of(vtop), -100), 100) - 6);
+  const float ev = value_reach(vtop);
   float reach[NG];
   bool raise = false;
 #pragma unroll

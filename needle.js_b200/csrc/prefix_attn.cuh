@@ -51,6 +51,10 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& head, uint
 __device__ __forceinline__ float power2(int e) { return __int_as_float((e + 127) << 23); }
 // Exponent of |v| (0 and subnormals -127, infinities and NaN 128).
 __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255u) - 127; }
+// What a block whose largest value scale is `top` adds to the reference maximum.  Scales below 2^-60 (rope_append's
+// smallest is 2^-47) count as that: a block of values that are all zero keeps a reference 2^-65 below its scores', near
+// enough for its weights not to be flushed beside a block with large values, nor to sum up to infinity.
+__device__ __forceinline__ float value_reach(float top) { return (float)(min(max(exponent_of(top), -60), 100) - 6); }
 
 // The next kernel of the stream may be started (when it was launched to overlap) / the kernel before has ended
 // and its writes are visible.

@@ -422,8 +422,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           most4[1 + (j & 2)] = max3(most4[1 + (j & 2)], x[j + 1].x, x[j + 1].y);
         }
         const float most = fmaxf(fmaxf(most4[0], most4[1]), fmaxf(most4[2], most4[3]));
-        const int ev = min(max(exponent_of(fmaxf(vtop.x, vtop.y)), -100), 100) - 6;
-        const float reach = most * inverse + (float)ev;  // weights are below 2^(reach - M + 7)
+        const float reach = most * inverse + value_reach(fmaxf(vtop.x, vtop.y));  // weights are below 2^(reach - M + 7)
         const bool raise = reach > M + kRaise;
         if (__any_sync(0xffffffffu, raise)) {
           const float Mn = raise ? reach + 1.0f : M;

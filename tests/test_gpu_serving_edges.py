@@ -129,6 +129,30 @@ def test_scores_of_any_size_choose_their_largest(torch, size):
             assert bool((lse[r].double() - want_lse).abs().le(16 * U * want_lse.abs()).all()), r
 
 
+def test_positions_whose_values_are_zero_keep_their_weight(torch):
+    """Positions with a value scale of 0 count in the softmax beside positions with large ones.  Nothing of their own
+    bounds their weights; they are far from binary32's largest all the same."""
+    for rows in (3, 170):
+        g = torch.Generator().manual_seed(rows)
+        heads, kv_heads, dim, prefix_length, capacity = 8, 4, 64, 300, 16
+        prefix, own = caches(torch, g, rows, kv_heads, dim, prefix_length, capacity)
+        prefix[0][:] = 0
+        prefix[1][:] = 0.7
+        prefix[0][:, 296:, 0] = 127  # 4 positions whose scores are 11 above the 296 without values
+        prefix[3][:, :296] = 0.0
+        prefix[3][:, 296:] *= 2.0 ** 17
+        q = torch.zeros(rows, heads * dim)
+        q[:, ::dim] = 1.0
+        counts = [0] * rows
+        out, lse = attend(torch, "f32", q, prefix, own, counts, heads, kv_heads, dim, prefix_length)
+        for r in (0, rows - 1):
+            want, want_lse, big, vmax = attention_reference(torch, q[r], prefix, own, r, 0, heads, kv_heads, dim, prefix_length, 0.125)
+            bound = (2 * (dim + 8) * big + prefix_length + 32) * U * vmax + U * want.abs()
+            assert bool((out[r].double() - want).abs().le(bound).all()), r
+            bound = ((dim + 8) * big + prefix_length) * U + 4 * U * want_lse.abs()
+            assert bool((lse[r].double() - want_lse).abs().le(bound).all()), (r, float((lse[r].double() - want_lse).abs().max()))
+
+
 # ------------------------------------------------------------------ logits_select
 
 @pytest.mark.parametrize("name,offset", [
