@@ -10,7 +10,7 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_serving_ops import (TYPES, U, attention_call, attention_reference, dtype_of, random_cache, rope_call,
+from test_gpu_serving_ops import (HALF, TYPES, U, attention_call, attention_reference, dtype_of, random_cache, rope_call,
                                   rules_args, stream_of, to_numpy)
 
 pytestmark = pytest.mark.gpu
@@ -151,6 +151,66 @@ def test_positions_whose_values_are_zero_keep_their_weight(torch):
             assert bool((out[r].double() - want).abs().le(bound).all()), r
             bound = ((dim + 8) * big + prefix_length) * U + 4 * U * want_lse.abs()
             assert bool((lse[r].double() - want_lse).abs().le(bound).all()), (r, float((lse[r].double() - want_lse).abs().max()))
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("small", [2.0 ** -10, 2.0 ** -20, 2.0 ** -30])
+def test_small_values_that_dominate(torch, name, small):
+    """One position takes nearly all the weight and its values are `small` times the others'.  Weights are held as
+    fp16 part(s) of at least 2^-25 next to the largest value scale: a reference M is at most 5 - e below the largest
+    score (2^e the largest value scale), so n weights bring an error of n 127 2^-25 2^(e - 5) <= n 2^-30 max |v| on top of
+    what binary32 has (relative to sum w |v|), and 2^-11 of that sum where 16-bit weights are rounded to fp16 once."""
+    for rows, prefix_length, capacity in ((3, 37, 40), (170, 300, 16)):
+        g = torch.Generator().manual_seed(rows + prefix_length)
+        heads, kv_heads, dim = 8, 4, 64
+        prefix, own = caches(torch, g, rows, kv_heads, dim, prefix_length, capacity)
+        q = torch.randn(rows, heads * dim, generator=g).to(dtype_of(torch, name))
+        q[:, ::dim] = 8.0
+        prefix[0][:, 7] = 0
+        prefix[0][:, 7, 0] = 127
+        prefix[1][:, 7] = 0.25  # a score of 8 * 127 * 0.25 / 8 = 32 above the others' order of 1
+        prefix[0][:, :7, 0] = 0
+        prefix[0][:, 8:, 0] = 0
+        own[0][..., 0] = 0
+        prefix[3][:, 7] *= small
+        counts = [capacity - r % 3 for r in range(rows)]
+        out, lse = attend(torch, name, q, prefix, own, counts, heads, kv_heads, dim, prefix_length)
+        keys = prefix[0].double() * prefix[1][..., None].double()
+        values = prefix[2].double() * prefix[3][..., None].double()
+        for r in {0, rows // 2, rows - 1}:
+            k = torch.cat((keys, own[0][r, :, :counts[r]].double() * own[1][r, :, :counts[r], None].double()), 1)
+            v = torch.cat((values, own[2][r, :, :counts[r]].double() * own[3][r, :, :counts[r], None].double()), 1)
+            qr = q[r].double().view(kv_heads, heads // kv_heads, dim)
+            s = torch.einsum("kgd,kpd->kgp", qr, k) / 8
+            big = float((torch.einsum("kgd,kpd->kgp", qr.abs(), k.abs()) / 8).max())
+            w = torch.softmax(s, -1)
+            want = torch.einsum("kgp,kpd->kgd", w, v).reshape(heads, dim)
+            size = torch.einsum("kgp,kpd->kgd", w, v.abs()).reshape(heads, dim)
+            n, vmax = v.shape[1], 127 * float(torch.cat((prefix[3], own[3][r]), 1).max())
+            bound = (2 * (dim + 8) * big + n + 32) * U * size + n * 2.0 ** -30 * vmax + HALF[name] * want.abs()
+            if name != "f32":
+                bound += 2.0 ** -11 * size
+            if name == "f16":
+                bound += 2.0 ** -25  # half a step of fp16 below its normal range
+            assert bool((out[r].double() - want).abs().le(bound).all()), (r, float(((out[r].double() - want).abs() / bound).max()))
+            want_lse = torch.logsumexp(s, -1).reshape(heads)
+            bound = ((dim + 8) * big + n) * U + 4 * U * want_lse.abs()
+            assert bool((lse[r].double() - want_lse).abs().le(bound).all()), r
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,prefix_length,capacity", PLANS)
+def test_the_softmax_denominator_is_binary32_in_every_type(torch, name, rows, heads, kv_heads, dim, prefix_length, capacity):
+    """lse takes no part in the rounding of weights: (D + 8) u S for the largest score, n u for the sum, 4 u of itself."""
+    g = torch.Generator().manual_seed(3 * rows + dim)
+    prefix, own = caches(torch, g, rows, kv_heads, dim, prefix_length, capacity)
+    counts = [capacity - (3 * r) % (capacity + 1) for r in range(rows)]
+    q = torch.randn(rows, heads * dim, generator=g).to(dtype_of(torch, name))
+    _, lse = attend(torch, name, q, prefix, own, counts, heads, kv_heads, dim, prefix_length)
+    for r in range(rows):
+        _, want, big, _ = attention_reference(torch, q[r], prefix, own, r, counts[r], heads, kv_heads, dim, prefix_length, dim ** -0.5)
+        bound = ((dim + 8) * big + prefix_length + counts[r]) * U + 4 * U * want.abs()
+        assert bool((lse[r].double() - want).abs().le(bound).all()), (r, float(((lse[r].double() - want).abs() / bound).max()))
 
 
 # ------------------------------------------------------------------ logits_select
