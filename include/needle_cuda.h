@@ -400,12 +400,9 @@ int needle_cuda_rope_frequencies(const needle_rope_scaling* scaling, int32_t rot
  * nothing to attend to gets zeros and lse -inf; a head whose scores are NaN gets NaN.  lse (optional,
  * [rows][heads]): the natural logarithm of each head's softmax denominator, with which outputs over different
  * prefixes can be merged.  out must not overlap q.
- * Accuracy.  Scores, their sums and lse are binary32 for every type.  Weights meet the codes on the tensor cores as
- * two fp16 parts, which keep binary32's accuracy, but for 16-bit types in calls with enough rows and prefix for
- * the prefix to be a dense product: there a prefix weight is rounded to fp16 once, which adds at most 2^-11
- * of sum w |v| to an output that is rounded to 16 bits itself, so the last bit of such a row may depend on the batch.
- * fp16 parts end at 2^-25 of the largest value scale that a head attends to: n positions add at most n 2^-30
- * of the largest |v|, which shows where a position with values 2^10 times smaller than others' has nearly all the weight. */
+ * Accuracy.  Binary32 for every type: weights meet the codes on the tensor cores as two fp16 parts.  The parts end at
+ * 2^-25 of the largest value scale that a head attends to: n positions add at most n 2^-30 of the largest |v|,
+ * which shows where a position whose values are 2^10 times smaller than others' has nearly all the weight. */
 typedef struct needle_prefix_attention {
   const void* q;   /* [rows][heads][head_dim] of `type`, rows q_stride elements apart */
   void* out;       /* the same shape, rows out_stride elements apart */

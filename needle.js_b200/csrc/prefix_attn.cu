@@ -1,7 +1,7 @@
 // prefix_attn.cu -- decode attention of a batch whose sequences share a prompt prefix: every row
 // attends over the prefix's int8 keys and values, held once, and over its own int8 cache
 // (#attention, packages/needle.js/src/model/runtime.ts:719-786, with the prefix taken out of the
-// per-sequence caches; any head layout, binary32 scores and sums).
+// per-sequence caches; any head layout, binary32 arithmetic).
 //
 //   s_j = scale * (q . code_j) * ks_j,  o = sum_j e^(s_j - m) vs_j code_j / sum_j e^(s_j - m),
 //   j over the prefix and the row's own positions;  lse = m + log sum_j e^(s_j - m)

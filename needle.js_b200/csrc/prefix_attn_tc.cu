@@ -18,9 +18,10 @@
 // products hide behind them.  64 rows x 2 heads x 2048 positions of 64: 15.3 us with the stream and the merge.
 // The reference M of a row covers the value scale too: a weight is 2^(s - M) vs <= 2^15, inside fp16, and
 // sums and outputs share the factor, which cancels.  16-bit queries are exact in fp16 after their row's
-// power of two (the score scale comes after the product), and their weights are rounded to fp16 once (2^-12
-// each, averaged over the positions; the output's own rounding is 2^-12 or more).  Binary32 queries (SPLIT)
-// and their weights are split into fp16 heads and tails, two MMAs each.
+// power of two (the score scale comes after the product); binary32 queries (SPLIT) are split into fp16 heads and
+// tails, two MMAs each.  So are the weights, for every type: rounded to fp16 once (2^-12 each) they would show in fp16
+// outputs where one position dominates, and a row's result would depend on which kernel its batch reaches; it costs
+// 333 rows x 32 heads x 8191 positions 130.6 us a call, 123.3 us without the tails.
 // Every wait is bounded (2 s): a wait that runs out is reported through the wait-status words, and the
 // rows' parts become NaN.
 #include "prefix_attn.cuh"
@@ -40,7 +41,7 @@ constexpr int kTurnRow = 36;      // floats of a row in the epilogue's transposi
 template <int D, bool SPLIT>
 struct PrefixShape {
   static constexpr int kHalves = D / 64;
-  static constexpr int kParts = SPLIT ? 2 : 1;       // fp16 parts of a query or weight
+  static constexpr int kParts = SPLIT ? 2 : 1;       // fp16 parts of a query
   static constexpr int kStages = D == 128 && SPLIT ? 3 : 4;  // of K and V tiles: two ahead in scores, one in values
   static constexpr uint32_t kQHalf = 128 * 128;                       // bytes of 128 rows x 64 dimensions
   static constexpr uint32_t kQTile = kQHalf * kHalves * kParts;       // [part][half]
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     auto values = [&](int t, int i) {  // O_t += P_t V_i
       const uint64_t v = descriptor(sm + P::kV + (i % P::kStages) * P::kKvTile, P::kKvHalf);
 #pragma unroll
-      for (int part = 0; part < P::kParts; part++)
+      for (int part = 0; part < 2; part++)  // heads, tails
 #pragma unroll
         for (int s = 0; s < kNT / 16; s++)
           mma_tensor(tm + o_column(t, D), tm + s_column(t, i & 1) + part * (kNT / 2) + s * 8, v + ((s * 2048) >> 4), pv,
@@ -472,12 +473,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
               p.y = power2f(p.y);
               sum = __fadd2_rn(sum, p);
               const float2 w = __fmul2_rn(p, o ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y));
-              if constexpr (SPLIT) split_f16(w.x, w.y, heads[j + o], tails[j + o]);
-              else heads[j + o] = half2_bits(__floats2half2_rn(w.x, w.y));
+              split_f16(w.x, w.y, heads[j + o], tails[j + o]);
             }
           }
           tensor_store16(s_at + c / 2, heads);
-          if constexpr (SPLIT) tensor_store16(s_at + kNT / 2 + c / 2, tails);
+          tensor_store16(s_at + kNT / 2 + c / 2, tails);
         }
         l += sum.x + sum.y;
         tensor_wait_stores();

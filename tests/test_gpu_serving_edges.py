@@ -45,6 +45,20 @@ def caches(torch, g, rows, kv_heads, dim, prefix_length, capacity):
     return prefix, own
 
 
+def exactly(torch, q, prefix, own, slot, count, heads, kv_heads, dim):
+    """One row in binary64: out and lse, the largest sum |q k| scale, sum w |v| (as out), the largest |v| that codes of 127
+    would have."""
+    sides = [(prefix, slice(None), slice(None)), (own, slot, slice(0, count))]
+    k, v = (torch.cat([c[i][at][:, n].double() * c[i + 1][at][:, n, None].double() for c, at, n in sides], 1) for i in (0, 2))
+    q = q.double().view(kv_heads, heads // kv_heads, dim)
+    s = torch.einsum("kgd,kpd->kgp", q, k) * dim ** -0.5
+    big = float((torch.einsum("kgd,kpd->kgp", q.abs(), k.abs()) * dim ** -0.5).max())
+    w = torch.softmax(s, -1)
+    out, size = (torch.einsum("kgp,kpd->kgd", w, x).reshape(heads, dim) for x in (v, v.abs()))
+    vmax = 127 * max(float(prefix[3].max()), float(own[3][slot, :, :count].max()) if count else 0.0)
+    return out, torch.logsumexp(s, -1).reshape(heads), big, size, vmax
+
+
 # rows, heads, kv_heads, dim, prefix, capacity: one part; splits; the prefix as a dense product, beside rows that have
 # nothing of their own; both
 PLANS = [(5, 8, 4, 64, 37, 20), (2, 8, 4, 64, 5, 5000), (1, 4, 1, 128, 0, 3001), (170, 8, 4, 64, 210, 16),
@@ -154,12 +168,33 @@ def test_positions_whose_values_are_zero_keep_their_weight(torch):
 
 
 @pytest.mark.parametrize("name", TYPES)
+def test_weights_are_binary32_in_every_type(torch, name):
+    """One position of a dense prefix has nearly all the weight: an output is off by what scores, weights and sums in
+    binary32 leave, relative to sum w |v|, and half a step of its type (a weight of 11 bits would double fp16's)."""
+    g = torch.Generator().manual_seed(12)
+    rows, heads, kv_heads, dim, prefix_length, capacity = 170, 16, 4, 64, 300, 8
+    prefix, own = caches(torch, g, rows, kv_heads, dim, prefix_length, capacity)
+    q = (0.05 * torch.randn(rows, heads * dim, generator=g)).to(dtype_of(torch, name))
+    q[:, ::dim] = (8.0 + torch.rand(rows, heads, generator=g)).to(q.dtype)
+    prefix[0][..., 0], own[0][..., 0] = 0, 0
+    prefix[0][:, 7], prefix[1][:, 7] = 0, 0.1
+    prefix[0][:, 7, 0] = 127  # a score of 12.7 and more
+    counts = [r % 9 for r in range(rows)]
+    out, _ = attend(torch, name, q, prefix, own, counts, heads, kv_heads, dim, prefix_length)
+    for r in range(rows):
+        want, _, big, size, vmax = exactly(torch, q[r], prefix, own, r, counts[r], heads, kv_heads, dim)
+        bound = (2 * (dim + 8) * big + prefix_length + capacity + 32) * U * size + (prefix_length + capacity) * 2.0 ** -30 * vmax
+        bound += HALF[name] * want.abs() + 2.0 ** -25
+        assert bool((out[r].double() - want).abs().le(bound).all()), (r, float(((out[r].double() - want).abs() / bound).max()))
+
+
+@pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("small", [2.0 ** -10, 2.0 ** -20, 2.0 ** -30])
 def test_small_values_that_dominate(torch, name, small):
     """One position takes nearly all the weight and its values are `small` times the others'.  Weights are held as
     fp16 part(s) of at least 2^-25 next to the largest value scale: a reference M is at most 5 - e below the largest
     score (2^e the largest value scale), so n weights bring an error of n 127 2^-25 2^(e - 5) <= n 2^-30 max |v| on top of
-    what binary32 has (relative to sum w |v|), and 2^-11 of that sum where 16-bit weights are rounded to fp16 once."""
+    what binary32 has (relative to sum w |v|)."""
     for rows, prefix_length, capacity in ((3, 37, 40), (170, 300, 16)):
         g = torch.Generator().manual_seed(rows + prefix_length)
         heads, kv_heads, dim = 8, 4, 64
@@ -175,25 +210,13 @@ def test_small_values_that_dominate(torch, name, small):
         prefix[3][:, 7] *= small
         counts = [capacity - r % 3 for r in range(rows)]
         out, lse = attend(torch, name, q, prefix, own, counts, heads, kv_heads, dim, prefix_length)
-        keys = prefix[0].double() * prefix[1][..., None].double()
-        values = prefix[2].double() * prefix[3][..., None].double()
         for r in {0, rows // 2, rows - 1}:
-            k = torch.cat((keys, own[0][r, :, :counts[r]].double() * own[1][r, :, :counts[r], None].double()), 1)
-            v = torch.cat((values, own[2][r, :, :counts[r]].double() * own[3][r, :, :counts[r], None].double()), 1)
-            qr = q[r].double().view(kv_heads, heads // kv_heads, dim)
-            s = torch.einsum("kgd,kpd->kgp", qr, k) / 8
-            big = float((torch.einsum("kgd,kpd->kgp", qr.abs(), k.abs()) / 8).max())
-            w = torch.softmax(s, -1)
-            want = torch.einsum("kgp,kpd->kgd", w, v).reshape(heads, dim)
-            size = torch.einsum("kgp,kpd->kgd", w, v.abs()).reshape(heads, dim)
-            n, vmax = v.shape[1], 127 * float(torch.cat((prefix[3], own[3][r]), 1).max())
+            want, want_lse, big, size, vmax = exactly(torch, q[r], prefix, own, r, counts[r], heads, kv_heads, dim)
+            n = prefix_length + counts[r]
             bound = (2 * (dim + 8) * big + n + 32) * U * size + n * 2.0 ** -30 * vmax + HALF[name] * want.abs()
-            if name != "f32":
-                bound += 2.0 ** -11 * size
             if name == "f16":
                 bound += 2.0 ** -25  # half a step of fp16 below its normal range
             assert bool((out[r].double() - want).abs().le(bound).all()), (r, float(((out[r].double() - want).abs() / bound).max()))
-            want_lse = torch.logsumexp(s, -1).reshape(heads)
             bound = ((dim + 8) * big + n) * U + 4 * U * want_lse.abs()
             assert bool((lse[r].double() - want_lse).abs().le(bound).all()), r
 
