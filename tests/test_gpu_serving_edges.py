@@ -361,3 +361,26 @@ def test_codes_and_scales_are_the_engine_s(torch):
         for k in (0, 2):
             np.testing.assert_array_equal(got[k], codes[:, :n].reshape(-1, dim))
             np.testing.assert_array_equal(got[k + 1], scales[:, :n].reshape(-1))
+
+
+@pytest.mark.parametrize("name,size", [("f32", 1e30), ("f16", 6e4), ("bf16", 1e18), ("bf16", 1e19), ("bf16", 3e38), ("bf16", 1e-30)])
+def test_norms_of_large_and_small_queries(torch, name, size):
+    """Squares that overflow or vanish in binary32: (1 + s) x / sqrt(mean x^2 + 1e-6) is within its range all the same."""
+    g = torch.Generator().manual_seed(6)
+    t, dim = 40, 128
+    x = ((torch.rand(t, dim, generator=g) - 0.5) * 2 * size).to(dtype_of(torch, name))
+    x[1::2] = torch.randn(t // 2, dim, generator=g).to(x.dtype)  # ordinary rows beside them, in the same warp
+    norm = 0.2 * torch.randn(dim, generator=g)
+    d = x.cuda()
+    out = torch.zeros_like(d)
+    cache = [torch.zeros(1, 1, t, dim, dtype=torch.int8).cuda(), torch.zeros(1, 1, t).cuda(),
+             torch.zeros(1, 1, t, dim, dtype=torch.int8).cuda(), torch.zeros(1, 1, t).cuda()]
+    at = torch.arange(t, dtype=torch.int32).cuda()
+    small = torch.zeros_like(d)
+    rope_call(torch, name, d, small, small, out, None, None, norm.cuda(), None, at, at * 0, at, cache, 1, 1, dim, 0, False, [], 1.0)
+    torch.cuda.synchronize()
+    y = x.double()
+    want = (1.0 + norm.double()) * y / ((y * y).mean(-1, keepdim=True) + 1e-6).sqrt()
+    # a sum of 128 squares, a root and two products in binary32, and the rounding to the type
+    bound = (200 * U + HALF[name]) * want.abs() + (2.0 ** -25 if name == "f16" else 1e-38)
+    assert bool((out.double().cpu() - want).abs().le(bound).all())
