@@ -73,20 +73,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr float kLog2eL = 1.4426950408889634f;
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-__device__ __forceinline__ float exp2_of(float v) {  // 2^v, relative error 2^-22
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-__device__ __forceinline__ float exp_below(float v) { return exp2_of(v * kLog2eL); }  // e^v, v <= 0
+__device__ __forceinline__ float exp_below(float v) { return power2f(v * kLog2e); }  // e^v, v <= 0
 
 // First id (possibly below 0) of 16-byte unit 0 of the row: rows that do not start on a 16-byte
 // boundary are taken from the boundary before them, with the ids outside the row left out.
@@ -580,19 +567,19 @@ __global__ void __launch_bounds__(kThreads, resident(sizeof(T))) k_logits_select
           // 2^(x log2 e - p) with p = m log2 e rounded: a term is 2^off times its value, off = m log2 e - p up to
           // 2^-24 |m|, exact in a fused product.  The factor goes out once a step (no slower: 200 x 128000 45.6 us).
           // Further from zero, where binary32 logits are 2^-4 apart and more, m is subtracted first
-          const float2 scale = make_float2(kLog2eL, kLog2eL), minus = make_float2(-base * kLog2eL, -base * kLog2eL);
-          const float off = fmaf(base, kLog2eL, minus.x);
+          const float2 scale = make_float2(kLog2e, kLog2e), minus = make_float2(-base * kLog2e, -base * kLog2e);
+          const float off = fmaf(base, kLog2e, minus.x);
           float2 more = make_float2(0.0f, 0.0f);
 #pragma unroll
           for (int u = 0; u < S::N; u++)
 #pragma unroll
             for (int i = 0; i < S::VEC; i += 2) {
               float2 d = __ffma2_rn(make_float2(x[u][i], x[u][i + 1]), scale, minus);
-              d.x = exp2_of(d.x);
-              d.y = exp2_of(d.y);
+              d.x = power2f(d.x);
+              d.y = power2f(d.y);
               more = __fadd2_rn(more, d);
             }
-          sum += (more.x + more.y) * exp2_of(-off);
+          sum += (more.x + more.y) * power2f(-off);
         } else {
 #pragma unroll
           for (int u = 0; u < S::N; u++)

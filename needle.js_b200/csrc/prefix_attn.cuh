@@ -6,7 +6,6 @@
 
 namespace needle {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // The reference maximum of a head covers the value scales too: a weight is 2^(s - M) vs, s and M base 2.  M is
 // raised, and what was summed rescaled, only when a block could bring weights of 2^15 (fp16 ends at 65504);
@@ -51,6 +50,7 @@ __device__ __forceinline__ void split_f16(float a, float b, uint32_t& head, uint
 __device__ __forceinline__ float power2(int e) { return __int_as_float((e + 127) << 23); }
 // Exponent of |v| (0 and subnormals -127, infinities and NaN 128).
 __device__ __forceinline__ int exponent_of(float v) { return (int)((__float_as_uint(v) >> 23) & 255u) - 127; }
+
 // What a block whose largest value scale is `top` adds to the reference maximum.  Scales below 2^-60 (rope_append's
 // smallest is 2^-47) count as that: a block of values that are all zero keeps a reference 2^-65 below its scores', near
 // enough for its weights not to be flushed beside a block with large values, nor to sum up to infinity.
@@ -60,11 +60,5 @@ __device__ __forceinline__ float value_reach(float top) { return (float)(min(max
 // and its writes are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_prior() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-__device__ __forceinline__ float power2f(float v) {  // 2^v, relative error 2^-22, 0 below 2^-126
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 
 }  // namespace needle

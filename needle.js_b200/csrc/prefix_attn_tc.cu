@@ -127,12 +127,6 @@ __device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fen
 // Shared-memory writes of this thread before reads of the tensor cores.
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // Scores from position `valid` on become -inf.
 template <int N>
 __device__ __forceinline__ void hide(float2* x, int valid) {

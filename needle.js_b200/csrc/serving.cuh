@@ -1,5 +1,5 @@
 // serving.cuh -- what the serving operators (rope.cu, prefix_attn.cu, logits.cu) share: element
-// types, vector access, argument checks and the guard of their C entries.
+// types, vector access, powers of two, argument checks and the guard of their C entries.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -33,6 +33,19 @@ template <class T, int N>
 struct alignas(sizeof(T) * N) Vec {
   T v[N];
 };
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float power2f(float v) {  // 2^v, relative error 2^-22, 0 below 2^-126
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
