@@ -436,11 +436,14 @@ int needle_cuda_prefix_attention_dev(const needle_prefix_attention* args, void* 
  *   an id in the row's history: l / repetition where l > 0, else l * repetition;
  *   an id answered c > 0 times (history entries from prompt_lengths[r] on): - frequency * c, - presence;
  *   an id with a bias: + its value (of several biases of one id the last counts);
- *   an id that mask slot mask_slots[r] leaves out: -inf (masks as in the device mask pool: bit id % 32 of
- *   word id / 32, ceil(vocab / 32) words per slot; slot -1: every id is allowed; a slot of mask_count or
- *   more allows none).
+ *   an id that mask slot mask_slots[r] leaves out: -inf (laid out as the device mask pool, in memory of the
+ *   caller's own: bit id % 32 of word id / 32, ceil(vocab / 32) words per slot; a negative slot: every id is
+ *   allowed; a slot of mask_count or more allows none).
  * Ids outside [0, vocab) in the lists (-1: padding) are left out; lengths and counts are taken within
- * [0, stride].  Any list or array of rules may be NULL: that rule does not apply. */
+ * [0, stride].  Any list or array of rules may be NULL: that rule does not apply.
+ * The tables that the lists go into are sized by history_stride + bias_stride, whatever the lengths: strides near what
+ * is in use are fastest, and above 4096 together a call takes many times longer (every 4096 ids of a row read the
+ * lists once more). */
 typedef struct needle_logits_rules {
   const void* logits;             /* [rows][vocab] of `type`, rows logits_stride elements apart */
   int64_t logits_stride;

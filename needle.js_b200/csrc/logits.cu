@@ -18,7 +18,8 @@
 // Bytes bound the stream, the lists' chains of dependent accesses the rest.  512 rows of 50001 bf16 ids (102 MB) with
 // histories of up to 1000 ids, 50 biases and masks take 32 us, 23 us without rules.  Select: 4096 rows of 8192
 // binary32 ids with histories of 256: 60 us (2.2 TB/s), 41 us without rules; 200 rows of 128000 fp16 ids with
-// histories of 2000: 46 us (1.1 TB/s; each of a row's two CTAs builds a table), 25 us without.
+// histories of 2000: 46 us (1.1 TB/s; each of a row's two CTAs builds a table), 25 us without.  Binary32 rules: 60 us for
+// 4096 rows of 8192 ids (4.5 TB/s), 46 us for 512 rows of 50001.
 // Measured beside it (the three sizes; 42, 61, 46 us then, before the rules had list warps): chunks of a row in
 // registers, direct tables of counts instead of the hash, one CTA a chunk: 47, 72, 63 us; the hash 5/4 of its lists
 // instead of twice: 50, 66, 55 us (probes), four times: 71, 66, 129 us (fewer CTAs resident); one warp a row: 110 us
@@ -683,7 +684,10 @@ LogitsPlan plan_for(const needle_logits_rules& a, int units, int most_parts) {
   const int64_t entries = (a.history ? a.history_stride : 0) + (a.bias_ids ? a.bias_stride : 0);
   const int64_t step = step_ids(size_t(element), units), steps = (ids + step - 1) / step;
   // parts: as many as keep the GPU busy, each rescanning the lists (148 * 8: 512 x 50001 32 -> 38 us, 200 x 128000
-  // 46 -> 86 us); small enough for their bits and, with long lists, for a table that has room for every id of the part
+  // 46 -> 86 us); small enough for their bits and, with long lists, for a table that has room for every id of the part.
+  // What counts is the lists' room, not their lengths, which are on the device.  200 x 128000, 100 biases, histories of
+  // up to 2000 ids (of 10): room for 2000: 47 us; 3900: 121 us (72): a table twice as large, cleared and walked whole, and
+  // half the CTAs; 5000 and 32768: 943 us (662): 32 parts a row.  512 x 50001, up to 1000 (10): 31 us, 761 us (351).
   const int64_t most = (entries > kMostEntries ? kMostEntries : kPartIds) / step;
   int64_t parts = std::max<int64_t>(1, std::min<int64_t>({steps, 148 * 4 / a.rows, most_parts}));
   parts = std::max(parts, (steps + most - 1) / most);

@@ -14,8 +14,11 @@
 // S is double-buffered, so the softmax warps never wait for the products of their own scores: with one buffer
 // of 128 positions a tile went through softmax (3700 cycles) and products (1900) in turn, 91 us for
 // 333 rows x 32 heads x 8191 positions of 128 dimensions.
-// Now 70 us (613 TFLOP/s, 38% of the measured rate): a pair of tiles takes the softmax warps 2080 cycles, and the
-// products hide behind them.  64 rows x 2 heads x 2048 positions of 64: 15.3 us with the stream and the merge.
+// Two ahead, a pair of tiles took the softmax warps 2080 cycles (weights in one fp16 part): 70 us.  With heads and tails
+// of the weights 84 us, the merge of its parts and the start of the stream included (520 TFLOP/s of useful products, 32%
+// of the measured rate; tensor pipe 43% busy, issue slots 46%): the softmax warps' exponentials and conversions, and
+// the products behind them, which the tails make half as many again.  64 rows x 2 heads x 2048 positions of 64:
+// 15.4 us with the stream and the merge.
 // The reference M of a row covers the value scale too: a weight is 2^(s - M) vs <= 2^15, inside fp16, and
 // sums and outputs share the factor, which cancels.  16-bit queries are exact in fp16 after their row's
 // power of two (the score scale comes after the product); binary32 queries (SPLIT) are split into fp16 heads and

@@ -27,8 +27,9 @@
 // with a warp a token; 64 us with the exact division only for quotients next to a border, in a loop over them (inlined
 // for every element it held registers), and accesses whose width is known at compile time; 48 us = 4.5 TB/s, 69% of a
 // copy's rate, with the loads in shared memory (in registers: 61 us; 8 ahead instead of 4: 49 us).  4 resident CTAs of
-// 64 registers: 3 take 51 us, 5 take 60 us (spills).  4096 tokens of 8 / 4 heads of 64 in binary32 (36 MB): 14.6 us,
-// bound by conversions; 4 tokens: 3.5 us.
+// 64 registers: 3 take 51 us, 5 take 60 us (spills).  4096 tokens of 8 / 4 heads of 64 in binary32 (36 MB): 13.9 us,
+// bound by conversions; 4 tokens: 3.7 us.
+// At 64 registers the 16-bit kernels spill 16 bytes (pairs), 36 (halves) and 160 (any), those of binary32 none.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -48,7 +49,8 @@ constexpr int kAhead = 4;            // 16-byte loads of a lane in flight
 
 // What a kernel is built for, E being the elements of a lane: pairs (2i, 2i + 1) and 16-byte accesses; pairs
 // (i, i + half), half a multiple of E (a lane's partners are then one lane), and 16-byte accesses; or any pairs and
-// any alignment.
+// any alignment, an element an access and nothing loaded ahead: halves that are no multiple of E (a rotary size of 24,
+// 40 or 50 in 16 bits), and rows that do not begin on 16 bytes.
 enum Form { kInterleaved, kHalves, kAny };
 
 struct RopeArgs {
