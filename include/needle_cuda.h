@@ -400,9 +400,11 @@ int needle_cuda_rope_frequencies(const needle_rope_scaling* scaling, int32_t rot
  * nothing to attend to gets zeros and lse -inf; a head whose scores are NaN gets NaN.  lse (optional,
  * [rows][heads]): the natural logarithm of each head's softmax denominator, with which outputs over different
  * prefixes can be merged.  out must not overlap q.
- * Accuracy.  Binary32 for every type: weights meet the codes on the tensor cores as two fp16 parts.  The parts end at
- * 2^-25 of the largest value scale that a head attends to: n positions add at most n 2^-30 of the largest |v|,
- * which shows where a position whose values are 2^10 times smaller than others' has nearly all the weight. */
+ * Accuracy.  Binary32 for every type: weights meet the codes on the tensor cores as two fp16 parts.  Exponents of the
+ * value scales are part of the reference that powers are taken against: near 0, lse is off by up to some 2^-20.  The
+ * fp16 parts end at 2^-25 of the largest value scale that a head attends to: n positions add at most n 2^-30 of the
+ * largest |v|, which shows where a position whose values are 2^10 times smaller than others' has nearly all the
+ * weight. */
 typedef struct needle_prefix_attention {
   const void* q;   /* [rows][heads][head_dim] of `type`, rows q_stride elements apart */
   void* out;       /* the same shape, rows out_stride elements apart */
