@@ -463,13 +463,14 @@ typedef struct needle_logits_rules {
   /* history_stride and bias_stride: below 2^30 */
 } needle_logits_rules;
 
-/* The ruled logits, rounded to `type`, rows out_stride elements apart; out may be logits (same stride). */
+/* The ruled logits, rounded to `type`, rows out_stride elements apart; out may be logits (same stride), and overlaps
+ * nothing of the call otherwise. */
 int needle_cuda_logits_rules_dev(const needle_logits_rules* args, void* out, int64_t out_stride, void* stream);
 
 /* selectToken (runtime.ts:880-899) on the ruled logits, which are not written: ids[r] is the allowed id with
  * the largest ruled logit, the lowest on ties (NaN counts as -inf), and log_probabilities[r] its log
- * probability under the raw logits, l - max - log sum exp(l - max), as needle_selected.  A row whose mask
- * leaves nothing gets id -1 and -inf. */
+ * probability under the raw logits, l - max - log sum exp(l - max), as needle_selected (NaN where one of them is NaN).
+ * A row whose mask leaves nothing gets id -1 and -inf. */
 int needle_cuda_logits_select_dev(const needle_logits_rules* args, int32_t* ids, float* log_probabilities, void* stream);
 
 /* ---- Bounded device waits ----

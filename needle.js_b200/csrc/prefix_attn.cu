@@ -536,7 +536,7 @@ constexpr int kSplitWarps = 148 * 8;
 // When the prefix goes to k_attend_prefix, whose launch, partial results and merge take about 4 us (packed rows = rows
 // times heads of a KV head).  By scores, packed rows x positions, heads of 64, 4 KV heads (stream, prefix kernel):
 // 128 x 256: 7.3, 9.8 us; 64 x 1024: 11.4, 10.6 us; 128 x 1024: 12.1, 12.5 us; 128 x 4096: 29.7, 16.0 us; heads of 128,
-// 8 KV heads: 256 x 128: 22.7, 32 us; 64 x 1024: 19.2, 17.5 us; 256 x 4096: 114, 42.9 us.  By positions, 8192 packed
+// 8 KV heads: 256 x 128: 22.7, 32 us; 64 x 1024: 19.2, 18.4 us; 256 x 4096: 114, 44.4 us.  By positions, 8192 packed
 // rows: x 64: 79, 75 us; 2048: x 64: 28.1, 31.2 us, x 127: 34.0, 31.5 us.  By rows: 16 x 4096: 11.5, 12.5 us; 32 x
 // 4096: 14.6, 14.4 us.
 constexpr int64_t kPrefixLeastRows = 32, kPrefixLeastPositions = 96, kPrefixLeastScores = 65536;
